@@ -13,8 +13,14 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <ATen/MemoryOverlap.h>
+
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <unordered_map>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/fpemu_hip.h"
 
@@ -160,6 +166,244 @@ at::Tensor quantize_per_tensor(const at::Tensor &input, bool inplace, int64_t fm
   return quantize_per_tensor_impl(input, inplace, fmt, rmode, flt_max, clamp, seed, offset, ws);
 }
 
+// ---- operators of a language model's training step (mpemu.functional, which checks types, shapes and devices) -----------
+
+at::Tensor scratch(uint64_t bytes, const at::Tensor &like) {
+  return at::empty({(int64_t)(bytes < 16 ? 16 : bytes)}, like.options().dtype(at::kByte));
+}
+
+struct OnStream {   // the tensor's device made current, and torch's current stream there
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard;
+  void *stream;
+  explicit OnStream(const at::Tensor &t)
+      : guard(t.device()), stream((void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream()) {}
+};
+
+// Their gradients are raw kernels: a second derivative would silently be missing, so it is refused.
+void once_only(const char *who) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), who, ": differentiable once (create_graph is not supported)");
+}
+
+// A leaf that an eager autograd graph still holds has its accumulation node on the eager stream.  A backward pass captured
+// into a HIP graph would make the capture wait for that stream, which ends the process when the capture ends: such a
+// forward is refused.  Looked for while a capture runs only: every accumulation node behind the inputs.
+void refuse_live_leaves(const char *who, std::initializer_list<at::Tensor> inputs, void *raw) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing((hipStream_t)raw, &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
+  using torch::autograd::Node;
+  std::unordered_set<Node *> seen;
+  std::vector<std::shared_ptr<Node>> todo;
+  for (const at::Tensor &t : inputs) {
+    if (!t.requires_grad()) continue;
+    todo.push_back(t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t));
+  }
+  while (!todo.empty()) {
+    const std::shared_ptr<Node> node = todo.back();
+    todo.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    const auto on = node->stream();
+    if (node->num_outputs() == 0 && on.has_value()) {
+      const c10::Stream now = c10::impl::VirtualGuardImpl(on->device_type()).getStream(on->device());
+      TORCH_CHECK(*on == now, who, ": an eager autograd graph of the same leaves is still alive; drop its outputs (losses) before "
+                  "a backward pass is captured");
+    }
+    for (const auto &edge : node->next_edges()) todo.push_back(edge.function);
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor> group_rows(const at::Tensor &ids_in, int64_t groups) {
+  at::Tensor ids = ids_in.contiguous();
+  const OnStream on(ids);
+  const uint64_t n = (uint64_t)ids.numel();
+  at::Tensor order = at::empty({(int64_t)n}, ids.options().dtype(at::kInt));
+  at::Tensor offsets = at::empty({groups + 1}, ids.options().dtype(at::kInt));
+  at::Tensor ws = scratch(fpemu_group_rows_workspace_bytes(n, (uint64_t)groups), ids);
+  check(fpemu_group_rows(ids.data_ptr(), (int)ids.element_size(), n, (uint64_t)groups, (int32_t *)order.data_ptr(),
+                         (int32_t *)offsets.data_ptr(), ws.data_ptr(), (uint64_t)ws.numel(), on.stream));
+  return {order, offsets};
+}
+
+at::Tensor embedding_impl(const at::Tensor &ids, const at::Tensor &weight_in, double scale) {
+  at::Tensor weight = weight_in.contiguous();
+  const OnStream on(weight);
+  std::vector<int64_t> shape = ids.sizes().vec();
+  shape.push_back(weight.size(1));
+  at::Tensor out = at::empty(shape, weight.options());
+  check(fpemu_embedding(weight.data_ptr(), ids.data_ptr(), (int)ids.element_size(), out.data_ptr(), (uint64_t)ids.numel(),
+                        (uint64_t)weight.size(0), (uint64_t)weight.size(1), dtype_id(weight), (float)scale, on.stream));
+  return out;
+}
+
+struct EmbeddingOp : public torch::autograd::Function<EmbeddingOp> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &ids, const at::Tensor &weight, double scale,
+                            int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["entries"] = weight.size(0);
+    ctx->saved_data["width"] = weight.size(1);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embedding_impl(ids, weight, scale);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    once_only("embedding");
+    const at::Tensor ids = ctx->get_saved_variables()[0];
+    const at::Tensor dout = grads[0].contiguous();
+    const OnStream on(dout);
+    const int64_t entries = ctx->saved_data["entries"].toInt(), width = ctx->saved_data["width"].toInt();
+    at::Tensor dweight = at::empty({entries, width}, dout.options());
+    const uint64_t n = (uint64_t)ids.numel();
+    at::Tensor ws = scratch(fpemu_embedding_grad_workspace_bytes(n, (uint64_t)entries, (uint64_t)width), dout);
+    check(fpemu_embedding_grad(dout.data_ptr(), ids.data_ptr(), (int)ids.element_size(), dweight.data_ptr(), n,
+                               (uint64_t)entries, (uint64_t)width, dtype_id(dout), (float)ctx->saved_data["scale"].toDouble(),
+                               ctx->saved_data["padding"].toInt(), ws.data_ptr(), (uint64_t)ws.numel(), on.stream));
+    return {at::Tensor(), dweight, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor embedding(const at::Tensor &ids_in, const at::Tensor &weight, double scale, int64_t padding) {
+  const at::Tensor ids = ids_in.contiguous();
+  if (needs_graph(weight)) {
+    { const OnStream on(weight); refuse_live_leaves("embedding", {weight}, on.stream); }
+    return EmbeddingOp::apply(ids, weight, scale, padding);
+  }
+  return embedding_impl(ids, weight, scale);
+}
+
+at::Tensor grouped_impl(const at::Tensor &x, const at::Tensor &w, const at::Tensor &offsets, bool trans) {
+  const OnStream on(x);
+  const int64_t N = trans ? w.size(1) : w.size(2), K = trans ? w.size(2) : w.size(1);
+  at::Tensor y = at::empty({x.size(0), N}, x.options());
+  check(fpemu_grouped_gemm(y.data_ptr(), x.data_ptr(), w.data_ptr(), (const int32_t *)offsets.data_ptr(), x.size(0), N, K,
+                           w.size(0), dtype_id(x), trans ? 1 : 0, on.stream));
+  return y;
+}
+
+struct GroupedOp : public torch::autograd::Function<GroupedOp> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w, const at::Tensor &offsets,
+                            bool trans) {
+    ctx->save_for_backward({x, w, offsets});
+    ctx->saved_data["trans"] = trans;
+    return grouped_impl(x, w, offsets, trans);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    once_only("grouped_mm");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
+    const bool trans = ctx->saved_data["trans"].toBool();
+    const at::Tensor dy = grads[0].contiguous();
+    at::Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = grouped_impl(dy, w, offsets, !trans);
+    if (ctx->needs_input_grad(1)) {
+      const OnStream on(x);
+      dw = at::empty(w.sizes(), w.options());
+      const at::Tensor &a = trans ? dy : x, &b = trans ? x : dy;
+      check(fpemu_grouped_gemm_wgrad(dw.data_ptr(), a.data_ptr(), b.data_ptr(), (const int32_t *)offsets.data_ptr(), x.size(0),
+                                     w.size(1), w.size(2), w.size(0), dtype_id(x), on.stream));
+    }
+    return {dx, dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor grouped_mm(const at::Tensor &x_in, const at::Tensor &weight, const at::Tensor &offsets) {
+  // contiguous() and transpose() are differentiable steps outside the node: its operands are what the kernels read
+  const at::Tensor x = x_in.contiguous();
+  at::Tensor w = weight;
+  bool trans = false;
+  if (!weight.is_contiguous()) {
+    w = weight.transpose(1, 2);
+    trans = w.is_contiguous();
+    if (!trans) w = weight.contiguous();
+  }
+  if (needs_graph(x) || needs_graph(w)) {
+    { const OnStream on(x); refuse_live_leaves("grouped_mm", {x, w}, on.stream); }
+    return GroupedOp::apply(x, w, offsets, trans);
+  }
+  return grouped_impl(x, w, offsets, trans);
+}
+
+// the elements of a gradient as one run of memory, in whatever order: itself where it is one, else a copy
+std::vector<at::Tensor> dense_list(const std::vector<at::Tensor> &ts) {
+  std::vector<at::Tensor> d;
+  d.reserve(ts.size());
+  for (const at::Tensor &t : ts) d.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+  return d;
+}
+
+std::vector<fpemu_grad_t> grad_table(const std::vector<at::Tensor> &in, const std::vector<at::Tensor> &out) {
+  std::vector<fpemu_grad_t> tab(in.size());
+  for (size_t i = 0; i < in.size(); i++)
+    tab[i] = {in[i].data_ptr(), out[i].data_ptr(), (uint64_t)in[i].numel(), (int32_t)dtype_id(in[i]), (int32_t)dtype_id(out[i])};
+  return tab;
+}
+
+// true where an output shares memory with another entry's gradient or output
+bool overlap(const std::vector<fpemu_grad_t> &tab) {
+  struct Span { uintptr_t lo, hi; bool out; };
+  std::vector<Span> spans;
+  spans.reserve(2 * tab.size());
+  const auto bytes = [](const fpemu_grad_t &g, int32_t dt) { return (uintptr_t)g.n * (dt == FPEMU_F32 ? 4u : 2u); };
+  for (const fpemu_grad_t &g : tab) {
+    if (g.n == 0) continue;
+    spans.push_back({(uintptr_t)g.out, (uintptr_t)g.out + bytes(g, g.out_dtype), true});
+    if (g.in != g.out) spans.push_back({(uintptr_t)g.in, (uintptr_t)g.in + bytes(g, g.in_dtype), false});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.lo < b.lo || (a.lo == b.lo && a.hi < b.hi); });
+  uintptr_t top = 0, top_out = 0;
+  for (const Span &s : spans) {
+    if (s.lo < (s.out ? top : top_out)) return true;
+    top = std::max(top, s.hi);
+    if (s.out) top_out = std::max(top_out, s.hi);
+  }
+  return false;
+}
+
+at::Tensor norm_of(const std::vector<fpemu_grad_t> &tab, int64_t order, const at::Tensor &sum, at::Tensor *norm, const OnStream &on) {
+  const uint64_t bytes = fpemu_grad_norm_workspace_bytes(tab.size());
+  at::Tensor ws = at::empty({(int64_t)(bytes / 8)}, sum.options());
+  check(fpemu_grad_norm_multi(tab.data(), tab.size(), (int)order, (double *)sum.data_ptr(),
+                              norm ? (float *)norm->data_ptr() : nullptr, ws.data_ptr(), bytes, on.stream));
+  return ws;
+}
+
+at::Tensor grad_norm(const std::vector<at::Tensor> &grads, int64_t order) {
+  const std::vector<at::Tensor> dense = dense_list(grads);
+  const OnStream on(grads[0]);
+  at::Tensor sum = at::empty({1}, grads[0].options().dtype(at::kDouble));
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  norm_of(grad_table(dense, dense), order, sum, &norm, on);
+  return norm;
+}
+
+at::Tensor clip_grads(const std::vector<at::Tensor> &grads, const std::vector<at::Tensor> &outs, double max_norm, int64_t order,
+                      bool finite_only) {
+  at::NoGradGuard no_grad;
+  const std::vector<at::Tensor> dense = dense_list(grads);
+  std::vector<at::Tensor> to;
+  to.reserve(grads.size());
+  for (size_t i = 0; i < grads.size(); i++) {
+    const bool copied = !dense[i].is_same(grads[i]), in_place = outs[i].is_same(grads[i]);
+    TORCH_CHECK_VALUE(!copied || in_place, "clip_grads_: out needs gradients that fill their memory without gaps");
+    TORCH_CHECK_VALUE(!copied || at::has_internal_overlap(grads[i]) != at::MemOverlap::Yes,
+                      "clip_grads_: a gradient or output shares memory with another output (or with itself)");
+    to.push_back(in_place ? dense[i] : outs[i]);
+  }
+  const std::vector<fpemu_grad_t> tab = grad_table(dense, to);
+  TORCH_CHECK_VALUE(!overlap(tab), "clip_grads_: a gradient or output shares memory with another output (or with itself)");
+  const OnStream on(grads[0]);
+  at::Tensor sum = at::empty({1}, grads[0].options().dtype(at::kDouble));
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  norm_of(tab, order, sum, finite_only ? &norm : nullptr, on);
+  if (finite_only) {
+    const float value = norm.item<float>();
+    TORCH_CHECK(std::isfinite(value), "clip_grads_: the norm of the gradients is ", value);
+  }
+  check(fpemu_clip_multi(tab.data(), tab.size(), (int)order, (const double *)sum.data_ptr(), (float)max_norm,
+                         (float *)norm.data_ptr(), on.stream));
+  for (size_t i = 0; i < grads.size(); i++)
+    if (!dense[i].is_same(grads[i])) grads[i].copy_(dense[i]);
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -171,4 +415,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("flt_max"), py::arg("clamp"), py::arg("seed"), py::arg("offset"), py::arg("workspace") = py::none());
   m.def("quantize_rows", &quantize_rows, py::arg("input"), py::arg("inplace"), py::arg("fmt"), py::arg("rmode"),
         py::arg("flt_max"), py::arg("rows"), py::arg("clamp"), py::arg("seed"), py::arg("offset"));
+  m.def("group_rows", &group_rows, py::arg("ids"), py::arg("groups"));
+  m.def("embedding", &embedding, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("padding"));
+  m.def("grouped_mm", &grouped_mm, py::arg("x"), py::arg("weight"), py::arg("offsets"));
+  m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("order"));
+  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("outs"), py::arg("max_norm"), py::arg("order"),
+        py::arg("finite_only"));
 }

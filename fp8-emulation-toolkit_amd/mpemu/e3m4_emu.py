@@ -3,12 +3,13 @@ construction-time default already scales weights per channel and inputs per tens
 import torch
 
 from .emulator_base import EmulatorBase
+from .module_wrappers import GroupedLinear
 
 
 class E3M4Emulator(EmulatorBase):
     tag = "e3m4_emulator"
     training_recipe = False
-    weights_only_for = (torch.nn.Conv2d, torch.nn.Linear)
+    weights_only_for = (torch.nn.Conv2d, torch.nn.Linear, GroupedLinear)
     defaults = {"emb": ("e3m4", "rne", "per-channel"), "wt": ("e3m4", "rne", "per-channel"),
                 "iact": ("e3m4", "rne", "per-tensor"), "oact": None}
     calibration = {"emb": ("e3m4", "rne", "per-tensor"), "wt": ("e3m4", "rne", "per-tensor"),

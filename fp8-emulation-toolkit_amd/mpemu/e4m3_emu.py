@@ -4,12 +4,13 @@ per-tensor input activations (e4m3_emu.py:181-185)."""
 import torch
 
 from .emulator_base import EmulatorBase
+from .module_wrappers import GroupedLinear
 
 
 class E4M3Emulator(EmulatorBase):
     tag = "e4m3_emulator"
     training_recipe = False
-    weights_only_for = (torch.nn.Conv2d, torch.nn.Linear)
+    weights_only_for = (torch.nn.Conv2d, torch.nn.Linear, GroupedLinear)
     defaults = {"emb": ("e4m3", "rne"), "wt": ("e4m3", "rne"), "iact": ("e4m3", "rne"), "oact": None}
     calibration = {"emb": ("e4m3", "rne", "per-channel"), "wt": ("e4m3", "rne", "per-channel"),
                    "iact": ("e4m3", "rne", "per-tensor"), "oact": None}

@@ -20,15 +20,17 @@ norm with one element per block -- that is what the reference executes, so that 
 """
 import torch
 
-from .module_wrappers import (AddMatmul, BatchMatmul, EltwiseAdd, EltwiseDiv, EltwiseMul, Matmul,
-                              SparseConv2d, SparseLinear)
+from .functional import clip_grad_norm_
+from .module_wrappers import (AddMatmul, BatchMatmul, EltwiseAdd, EltwiseDiv, EltwiseMul, GroupedLinear, GroupedMatmul,
+                              Matmul, ScaledEmbedding, SparseConv2d, SparseLinear)
 from .qutils import (ModuleQuantConfig, TensorQuantConfig, add_quantization_hooks,
                      get_or_update_model_quant_config_dict, quantize_model_weights,
                      reset_quantization_setup, set_quantize_weights_flag)
 from .scale_shift import replace_batchnorms_with_scaleshifts
 
 _COMMON_TYPES = [torch.nn.Conv2d, torch.nn.Linear, torch.nn.Embedding, torch.nn.EmbeddingBag]
-_WRAPPER_TYPES = [Matmul, BatchMatmul, AddMatmul, EltwiseAdd, EltwiseMul, EltwiseDiv, SparseConv2d, SparseLinear]
+_WRAPPER_TYPES = [Matmul, BatchMatmul, AddMatmul, EltwiseAdd, EltwiseMul, EltwiseDiv, SparseConv2d, SparseLinear,
+                  GroupedMatmul, GroupedLinear, ScaledEmbedding]
 _EMB_MODES = {"e5m2": "E5M2_STOCHASTIC", "BF8": "E5M2_STOCHASTIC",
               "e4m3": "E4M3_STOCHASTIC", "HF8": "E4M3_STOCHASTIC",
               "e4m3_2": "E3M4_STOCHASTIC", "HF8_2": "E3M4_STOCHASTIC"}
@@ -173,10 +175,16 @@ class EmulatorBase(object):
         elif self.use_e5m2_master:
             self.update_e5m2_master_params(optimizer)
 
-    def optimizer_step(self, optimizer):
+    def optimizer_step(self, optimizer, max_grad_norm=None, norm_type=2.0):
+        """optimizer.step(), then the master parameters re-quantised.  max_grad_norm: clip the master gradients to that norm
+        first; the norm before clipping (a device tensor, no synchronisation) is returned then."""
+        norm = None
+        if max_grad_norm is not None:
+            norm = clip_grad_norm_(self._master_params(optimizer), max_grad_norm, norm_type)
         optimizer.step()
         self.update_master_params(optimizer)
         self.global_steps += 1
+        return norm
 
     def set_master_param_precision(self, master_params):
         if master_params in ("fp16", "FP16"):
@@ -225,7 +233,7 @@ class EmulatorBase(object):
             if not keeps_weight:
                 d[name].wt_qconfig = None
                 d[name].wtgrad_qconfig = None
-            if kind in (torch.nn.Embedding, torch.nn.EmbeddingBag):
+            if kind in (torch.nn.Embedding, torch.nn.EmbeddingBag, ScaledEmbedding):
                 d[name].wt_qconfig = self.emb_qconfig
                 d[name].iact_qconfig = None
                 d[name].igrad_qconfig = None

@@ -1,0 +1,308 @@
+"""mpemu.functional -- operators of a language model's training step, beside the emulated cast.
+
+    order, offsets = group_rows(expert_ids, num_experts)     # the router's tokens, expert by expert
+    h = embedding(token_ids, table, scale=d ** 0.5)          # scaled lookup; the table's gradient by sorted tokens
+    y = grouped_mm(x[order], w, offsets)                     # one product per expert over ragged runs of rows
+    norm = clip_grad_norm_(model.parameters(), 1.0)          # one norm over all gradients, no host synchronisation
+
+Every operator runs in hand-written gfx950 kernels (libfpemu_hip.so) on torch's current stream; tensors live on a ROCm
+device, float32 / float16 / bfloat16.  Nothing here synchronises with the host: group sizes, norms and coefficients stay
+on the device, so the operators (and their gradients) can be captured into a HIP graph; a capture whose leaves an eager
+autograd graph still holds is refused.  Sums run in 32 bits or more and
+are rounded once, in a fixed order: the same inputs give the same bits.
+
+The module forms that the quantisation hooks attach to are module_wrappers.{ScaledEmbedding, GroupedMatmul,
+GroupedLinear}; the emulators clip through optimizer_step(optimizer, max_grad_norm=...).
+"""
+import math
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .pytquant.hip import _binding as _hip
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _floating(t, what, who):
+    if not torch.is_tensor(t) or t.dtype not in _FLOATS:
+        raise TypeError("%s: %s must be a float32, float16 or bfloat16 tensor" % (who, what))
+
+
+def _integers(t, what, who):
+    if not torch.is_tensor(t) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError("%s: %s must be an int32 or int64 tensor" % (who, what))
+
+
+def _one_device(who, *ts):
+    for t in ts:
+        if not t.is_cuda:
+            raise RuntimeError("%s: tensors must live on a ROCm device (got %s); this build has no CPU path" % (who, t.device))
+        if t.device != ts[0].device:
+            raise ValueError("%s: tensors on different devices (%s, %s)" % (who, ts[0].device, t.device))
+
+
+def _native():
+    """The C++ front of these operators (one call with checks, allocation, launches and the autograd node), or None:
+    then the same kernels are reached through ctypes."""
+    return None if _hip.tracing() else _hip.ext()
+
+
+def _refuse_capture(who, *ts):
+    """Without the native front the stream of a leaf's accumulation node is unknown, and a captured backward pass of a leaf
+    that an eager graph still holds ends the process: no captured gradients there."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("%s: capturing a backward pass needs the native extension (_mpemu_torch.so)" % who)
+
+
+# ---- rows by group ------------------------------------------------------------------------------------------------------
+def group_rows(ids, num_groups):
+    """Stable order of rows by group id: (order, offsets), both int32.
+
+    ids: integer tensor, any shape (taken flat).  order[i] is the row at place i when the rows are sorted by id, rows of
+    one group in their own order; offsets has num_groups + 1 entries, group g holds places offsets[g] .. offsets[g + 1].
+    Rows whose id is outside [0, num_groups) belong to no group and come last, from offsets[num_groups] on."""
+    _integers(ids, "ids", "group_rows")
+    _one_device("group_rows", ids)
+    num_groups = int(num_groups)
+    if not 1 <= num_groups <= 2 ** 31 - 2:
+        raise ValueError("group_rows: num_groups must be between 1 and 2^31 - 2, got %d" % num_groups)
+    ext = _native()
+    if ext is not None:
+        return ext.group_rows(ids, num_groups)
+    ids = ids.contiguous()
+    order = torch.empty(ids.numel(), dtype=torch.int32, device=ids.device)
+    offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=ids.device)
+    return _hip.group_rows_(ids, num_groups, order, offsets)
+
+
+# ---- embedding ----------------------------------------------------------------------------------------------------------
+class _Embedding(Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.shape, ctx.scale, ctx.padding = weight.shape, scale, padding
+        out = torch.empty(tuple(ids.shape) + (weight.shape[1],), dtype=weight.dtype, device=weight.device)
+        return _hip.embedding_(ids, weight.contiguous(), out, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        dweight = torch.empty(ctx.shape, dtype=grad.dtype, device=grad.device)
+        return None, _hip.embedding_grad_(grad.contiguous(), ids, dweight, ctx.scale, ctx.padding), None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """scale * weight[ids]: ids of any shape, weight [entries, width]; the result has shape ids.shape + (width,).
+
+    The gradient of the table is dense and deterministic: tokens are sorted by entry and every entry's rows are summed in
+    fp32, in token order, and rounded once.  padding_idx (negative: from the end): that entry's gradient is zero.  An id
+    outside the table is not an error that the device could raise: its row of the result is NaN, it adds to no gradient.
+    Differentiable once."""
+    who = "embedding"
+    _integers(ids, "ids", who)
+    _floating(weight, "weight", who)
+    _one_device(who, ids, weight)
+    if weight.dim() != 2:
+        raise ValueError("embedding: weight must be 2-D, got %s" % (tuple(weight.shape),))
+    if not 1 <= weight.shape[0] <= 2 ** 31 - 2:
+        raise ValueError("embedding: the table needs between 1 and 2^31 - 2 entries")
+    padding = -1
+    if padding_idx is not None:
+        padding = int(padding_idx)
+        if not -weight.shape[0] <= padding < weight.shape[0]:
+            raise ValueError("embedding: padding_idx %d is outside the table of %d entries" % (padding, weight.shape[0]))
+        padding %= weight.shape[0]
+    ext = _native()
+    if ext is not None:
+        return ext.embedding(ids, weight, float(scale), padding)
+    _refuse_capture(who, weight)
+    return _Embedding.apply(ids.contiguous(), weight, float(scale), padding)
+
+
+# ---- products by group ----------------------------------------------------------------------------------------------------
+def _laid_out(weight):
+    """(tensor to hand to the kernel, transposed flag): a transposed view of contiguous [G, N, K] matrices -- a linear
+    layer's weights -- is passed as a flag, anything else is made contiguous."""
+    if weight.is_contiguous():
+        return weight, False
+    t = weight.transpose(1, 2)
+    if t.is_contiguous():
+        return t, True
+    return weight.contiguous(), False
+
+
+class _GroupedMm(Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets):
+        x = x.contiguous()
+        w, trans = _laid_out(weight)
+        ctx.save_for_backward(x, w, offsets)
+        ctx.trans = trans
+        y = torch.empty((x.shape[0], weight.shape[2]), dtype=x.dtype, device=x.device)
+        return _hip.grouped_gemm_(y, x, w, offsets, trans)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, w, offsets = ctx.saved_tensors
+        grad = grad.contiguous()
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = _hip.grouped_gemm_(torch.empty_like(x), grad, w, offsets, not ctx.trans)
+        if ctx.needs_input_grad[1]:
+            dw = torch.empty_like(w)
+            if ctx.trans:
+                dw = _hip.grouped_gemm_wgrad_(dw, grad, x, offsets).transpose(1, 2)
+            else:
+                dw = _hip.grouped_gemm_wgrad_(dw, x, grad, offsets)
+        return dx, dw, None
+
+
+def grouped_mm(x, weight, offsets):
+    """y[i] = x[i] @ weight[g] for offsets[g] <= i < offsets[g + 1]: one matrix product per group of rows.
+
+    x [rows, K]; weight [groups, K, N] or a transposed view of [groups, N, K] (taken as it lies, no copy); offsets: int32 or
+    int64, groups + 1 entries, not decreasing, as group_rows returns them.  The sizes stay on the device.  Groups may be
+    empty; rows outside every group are zero in y and in the gradient of x, and add to no gradient of weight.  16-bit types
+    multiply on the matrix cores with fp32 sums; fp32 runs the k-ascending fmaf chain of the c-model
+    (mpemu.cmodel.simple, accumulation "fma"), whatever set_accumulation says.  Differentiable once, in x and weight."""
+    who = "grouped_mm"
+    _floating(x, "x", who)
+    _floating(weight, "weight", who)
+    _integers(offsets, "offsets", who)
+    _one_device(who, x, weight, offsets)
+    if x.dtype != weight.dtype:
+        raise TypeError("grouped_mm: x is %s, weight is %s" % (x.dtype, weight.dtype))
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[1] or weight.shape[0] < 1:
+        raise ValueError("grouped_mm: x [rows, K] and weight [groups, K, N] expected, got %s and %s"
+                         % (tuple(x.shape), tuple(weight.shape)))
+    if offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1:
+        raise ValueError("grouped_mm: offsets must have %d entries, got %s" % (weight.shape[0] + 1, tuple(offsets.shape)))
+    offsets = offsets.to(torch.int32).contiguous()
+    ext = _native()
+    if ext is not None:
+        return ext.grouped_mm(x, weight, offsets)
+    _refuse_capture(who, x, weight)
+    return _GroupedMm.apply(x, weight, offsets)
+
+
+# ---- gradient norm and clipping --------------------------------------------------------------------------------------------
+def _order(norm_type, who):
+    order = {1.0: _hip.NORM_1, 2.0: _hip.NORM_2, math.inf: _hip.NORM_INF}.get(float(norm_type))
+    if order is None:
+        raise ValueError("%s: norm_type must be 1, 2 or inf, got %r" % (who, norm_type))
+    return order
+
+
+def _gradients(grads, who):
+    grads = [grads] if torch.is_tensor(grads) else list(grads)
+    for g in grads:
+        if torch.is_tensor(g) and g.is_sparse:
+            raise TypeError("%s: sparse gradients are not supported" % who)
+        _floating(g, "a gradient", who)
+    _one_device(who, *grads)
+    return grads
+
+
+def _dense(t):
+    """The elements of t as one run of memory, in whatever order: t itself where it is one, else a copy."""
+    t = t.detach()
+    order = sorted(range(t.dim()), key=lambda i: -t.stride(i))
+    return t if t.is_contiguous() or t.permute(order).is_contiguous() else t.contiguous()
+
+
+def _overlap(grads, outs):
+    """True where an output shares memory with another entry's gradient or output."""
+    spans = []
+    for g, o in zip(grads, outs):
+        spans.append((o.data_ptr(), o.data_ptr() + o.numel() * o.element_size(), True))
+        if o.data_ptr() != g.data_ptr():
+            spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size(), False))
+    top = top_out = 0
+    for lo, hi, is_out in sorted(s for s in spans if s[1] > s[0]):
+        if lo < (top if is_out else top_out):
+            return True
+        top = max(top, hi)
+        if is_out:
+            top_out = max(top_out, hi)
+    return False
+
+
+def grad_norm(grads, norm_type=2.0):
+    """The norm (1, 2 or inf) of all elements of a list of tensors as one vector: float32, 0-d, on the device.  The sum runs
+    in 64 bits, so neither large nor many elements overflow or drown it."""
+    who = "grad_norm"
+    order = _order(norm_type, who)
+    grads = _gradients(grads, who)
+    if not grads:
+        return torch.tensor(0.0)
+    ext = _native()
+    if ext is not None:
+        return ext.grad_norm(grads, order)
+    dense = [_dense(g) for g in grads]
+    total = torch.empty(1, dtype=torch.float64, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _hip.grad_norm_multi_(dense, order, total, norm)
+    return norm
+
+
+def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=False):
+    """Scale a list of gradients by min(1, max_norm / (norm + 1e-6)), norm over all of them; returns the norm (float32, 0-d,
+    on the device, before clipping).
+
+    In place, or into `out`: a list of the same shapes and strides, each of the gradient's type or float32 (16-bit model
+    gradients clipped into fp32 master gradients in one pass).  No tensor may share memory with another one's output.  A
+    norm that is not finite gives what the arithmetic gives (NaN, or zeros and NaN), as
+    torch.nn.utils.clip_grad_norm_ does; error_if_nonfinite=True reads the norm on the host first and raises instead,
+    with every gradient as it was."""
+    who = "clip_grads_"
+    order = _order(norm_type, who)
+    grads = _gradients(grads, who)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("clip_grads_: max_norm must not be negative or NaN, got %r" % max_norm)
+    if out is not None:
+        out = [out] if torch.is_tensor(out) else list(out)
+        if len(out) != len(grads):
+            raise ValueError("clip_grads_: %d gradients but %d outputs" % (len(grads), len(out)))
+        for g, o in zip(grads, out):
+            _floating(o, "an output", who)
+            if o.shape != g.shape or o.stride() != g.stride() or o.device != g.device or o.dtype not in (g.dtype, torch.float32):
+                raise ValueError("clip_grads_: an output needs its gradient's shape, strides and device, and its type or float32")
+    if not grads:
+        return torch.tensor(0.0)
+    ext = _native()
+    if ext is not None:
+        return ext.clip_grads(grads, out if out is not None else grads, max_norm, order, bool(error_if_nonfinite))
+    dense = [_dense(g) for g in grads]
+    if out is None:
+        outs = dense
+    else:
+        outs = [o.detach() for o in out]
+        for d, g in zip(dense, grads):
+            if d.data_ptr() != g.data_ptr():
+                raise ValueError("clip_grads_: out needs gradients that fill their memory without gaps")
+    if any(0 in g.stride() and g.numel() > 1 and d.data_ptr() != g.data_ptr() for g, d in zip(grads, dense)) or _overlap(dense, outs):
+        raise ValueError("clip_grads_: a gradient or output shares memory with another output (or with itself)")
+    total = torch.empty(1, dtype=torch.float64, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _hip.grad_norm_multi_(dense, order, total, norm)
+    if error_if_nonfinite and not bool(torch.isfinite(norm)):
+        raise RuntimeError("clip_grads_: the norm of the gradients is %s" % norm.item())
+    _hip.clip_multi_(dense, outs, order, total, max_norm)
+    if out is None:
+        for d, g in zip(dense, grads):
+            if d.data_ptr() != g.data_ptr():
+                g.detach().copy_(d)
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ on these kernels: clips the .grad of the parameters that have one, in place, and
+    returns the norm before clipping.  Two passes over the gradients (one where nothing has to be clipped), a few launches
+    for the whole list, no host synchronisation."""
+    params = [parameters] if torch.is_tensor(parameters) else parameters
+    return clip_grads_([p.grad for p in params if p.grad is not None], max_norm, norm_type, error_if_nonfinite=error_if_nonfinite)

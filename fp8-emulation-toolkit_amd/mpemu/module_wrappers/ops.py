@@ -2,8 +2,12 @@
 signatures as the reference (module_wrappers/matmul.py:12-32, eltwise.py:12-61,
 aggregate.py:12-35).  `EltwiseMul` constructs here (the reference's __init__ has a NameError,
 eltwise.py:34)."""
+import math
+
 import torch
 import torch.nn as nn
+
+from .. import functional as F
 
 
 class Matmul(nn.Module):
@@ -89,3 +93,46 @@ class SparseLinear(nn.Linear):
 
 class SparseConv2d(nn.Conv2d):
     """See SparseLinear: dense Conv2d, kept as a hook-target type."""
+
+
+class GroupedMatmul(nn.Module):
+    """One product per group of rows (functional.grouped_mm).  The hooks quantise a and b; offsets, being integers, pass."""
+
+    def forward(self, a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor):
+        return F.grouped_mm(a, b, offsets)
+
+
+class GroupedLinear(nn.Module):
+    """The experts of a layer: num_groups linear maps without bias, rows offsets[g] .. offsets[g + 1] of the input through
+    the g-th.  weight [num_groups, out_features, in_features]: per-channel scaling gives every expert one scale."""
+
+    def __init__(self, num_groups, in_features, out_features, device=None, dtype=None):
+        super().__init__()
+        self.num_groups, self.in_features, self.out_features = num_groups, in_features, out_features
+        self.weight = nn.Parameter(torch.empty(num_groups, out_features, in_features, device=device, dtype=dtype))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        bound = 1.0 / math.sqrt(self.in_features) if self.in_features > 0 else 0.0
+        nn.init.uniform_(self.weight, -bound, bound)
+
+    def forward(self, x: torch.Tensor, offsets: torch.Tensor):
+        return F.grouped_mm(x, self.weight.transpose(1, 2), offsets)
+
+    def extra_repr(self) -> str:
+        return 'num_groups={}, in_features={}, out_features={}'.format(self.num_groups, self.in_features, self.out_features)
+
+
+class ScaledEmbedding(nn.Embedding):
+    """An embedding whose rows are multiplied by `scale` as they are looked up (functional.embedding); its gradient is
+    dense and deterministic.  max_norm, scale_grad_by_freq and sparse gradients are not offered."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+        self.scale = float(scale)
+
+    def forward(self, input: torch.Tensor):
+        return F.embedding(input, self.weight, scale=self.scale, padding_idx=self.padding_idx)
+
+    def extra_repr(self) -> str:
+        return '{}, scale={}'.format(super().extra_repr(), self.scale)

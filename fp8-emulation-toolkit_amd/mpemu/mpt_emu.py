@@ -2,7 +2,7 @@
 
     model, emulator = mpt_emu.initialize(model, optimizer, training_algo="hybrid" | "direct", ...)
     model, emulator = mpt_emu.quantize_model(model, dtype="e4m3" | "e5m2" | "e3m4" | "hybrid", ...)
-    emulator.optimizer_step(optimizer)
+    emulator.optimizer_step(optimizer)                        # max_grad_norm=1.0: clips the master gradients first
 
 Out of scope in this build and rejected loudly: sparsity / pruning (`pruning_algo` other than
 "none", reference sparse_utils.py / adasparse.py).  Tensors must live on a ROCm device.
@@ -47,8 +47,8 @@ class MPTEmulator(object):
     def whitelist_modules(self, list_modules):
         self.emulator.whitelist_modules(list_modules)
 
-    def optimizer_step(self, optimizer):
-        self.emulator.optimizer_step(optimizer)
+    def optimizer_step(self, optimizer, max_grad_norm=None, norm_type=2.0):
+        return self.emulator.optimizer_step(optimizer, max_grad_norm, norm_type)
 
     def update_global_steps(self, global_steps):
         self.emulator.global_steps = global_steps

@@ -102,7 +102,27 @@ def lib():
         L.fpemu_amax_rows.argtypes = [vp, u64, u64, i32, vp, vp]
         L.fpemu_cast_rows_amax.restype = i32
         L.fpemu_cast_rows_amax.argtypes = [vp, vp, u64, u64, i32, i32, i32, vp, f32, i32, u64, u64, u64, vp]
-        if L.fpemu_abi_version() != 10:
+        L.fpemu_group_rows_workspace_bytes.restype = u64
+        L.fpemu_group_rows_workspace_bytes.argtypes = [u64, u64]
+        L.fpemu_group_rows.restype = i32
+        L.fpemu_group_rows.argtypes = [vp, i32, u64, u64, vp, vp, vp, u64, vp]
+        L.fpemu_embedding.restype = i32
+        L.fpemu_embedding.argtypes = [vp, vp, i32, vp, u64, u64, u64, i32, f32, vp]
+        L.fpemu_embedding_grad_workspace_bytes.restype = u64
+        L.fpemu_embedding_grad_workspace_bytes.argtypes = [u64, u64, u64]
+        L.fpemu_embedding_grad.restype = i32
+        L.fpemu_embedding_grad.argtypes = [vp, vp, i32, vp, u64, u64, u64, i32, f32, i64, vp, u64, vp]
+        L.fpemu_grouped_gemm.restype = i32
+        L.fpemu_grouped_gemm.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, i32, i32, vp]
+        L.fpemu_grouped_gemm_wgrad.restype = i32
+        L.fpemu_grouped_gemm_wgrad.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, i32, vp]
+        L.fpemu_grad_norm_workspace_bytes.restype = u64
+        L.fpemu_grad_norm_workspace_bytes.argtypes = [u64]
+        L.fpemu_grad_norm_multi.restype = i32
+        L.fpemu_grad_norm_multi.argtypes = [vp, u64, i32, vp, vp, vp, u64, vp]
+        L.fpemu_clip_multi.restype = i32
+        L.fpemu_clip_multi.argtypes = [vp, u64, i32, vp, f32, vp, vp]
+        if L.fpemu_abi_version() != 11:
             raise ImportError("libfpemu_hip.so: ABI version mismatch")
         _lib = L
     return _lib
@@ -735,6 +755,131 @@ def conv2d_wu_(grad_weight, grad_output, input, stride, padding, variant=GEMM_FM
         _check(lib().fpemu_conv2d_wu_f32(grad_weight.data_ptr(), grad_output.data_ptr(), input.data_ptr(), *dims,
                                          int(variant), ws.data_ptr(), nbytes, _stream(input)))
     return grad_weight
+
+
+# ---- operators of a language model's training step (mpemu.functional checks the arguments and adds autograd) ----------
+def _scratch(nbytes, like):
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=like.device)
+
+
+def _require_ids(ids, what="ids"):
+    _require_device(ids, what)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("fpemu: %s must be int32 or int64 (got %s)" % (what, ids.dtype))
+
+
+def group_rows_(ids, groups, order, offsets):
+    """order (int32[n]) and offsets (int32[groups + 1]) of the rows sorted by group id, equal ids in their own order;
+    rows whose id is outside [0, groups) come last."""
+    _require_ids(ids)
+    _require_words(order, ids, ids.numel(), "order")
+    _require_words(offsets, ids, groups + 1, "offsets")
+    ws = _scratch(lib().fpemu_group_rows_workspace_bytes(ids.numel(), groups), ids)
+    with _range("fpemu::group_rows"), _on_device(ids):
+        _check(lib().fpemu_group_rows(ids.data_ptr(), ids.element_size(), ids.numel(), groups, order.data_ptr(),
+                                      offsets.data_ptr(), ws.data_ptr(), ws.numel(), _stream(ids)))
+    return order, offsets
+
+
+def _embedding_check(ids, table, rows, what):
+    _require_ids(ids)
+    _require_device(table, what)
+    _require_device(rows, "rows")
+    if table.dim() != 2 or table.dtype != rows.dtype or table.device != ids.device or rows.device != ids.device:
+        raise ValueError("fpemu embedding: %s must be 2-D, with the rows' dtype, on the ids' device" % what)
+    if rows.numel() != ids.numel() * table.shape[1]:
+        raise ValueError("fpemu embedding: %d rows of %d elements expected" % (ids.numel(), table.shape[1]))
+
+
+def embedding_(ids, weight, out, scale=1.0):
+    """out[t] = scale * weight[ids[t]]; an id outside the table yields a row of NaN."""
+    _embedding_check(ids, weight, out, "weight")
+    with _range("fpemu::embedding"), _on_device(weight):
+        _check(lib().fpemu_embedding(weight.data_ptr(), ids.data_ptr(), ids.element_size(), out.data_ptr(), ids.numel(),
+                                     weight.shape[0], weight.shape[1], _dtype_id(weight), float(scale), _stream(weight)))
+    return out
+
+
+def embedding_grad_(dout, ids, dweight, scale=1.0, padding=-1):
+    """dweight[v] = scale * sum of dout[t] over ids[t] = v (fp32 sums); row `padding` is zero."""
+    _embedding_check(ids, dweight, dout, "dweight")
+    ws = _scratch(lib().fpemu_embedding_grad_workspace_bytes(ids.numel(), *dweight.shape), dweight)
+    with _range("fpemu::embedding_grad"), _on_device(dweight):
+        _check(lib().fpemu_embedding_grad(dout.data_ptr(), ids.data_ptr(), ids.element_size(), dweight.data_ptr(),
+                                          ids.numel(), dweight.shape[0], dweight.shape[1], _dtype_id(dweight), float(scale),
+                                          int(padding), ws.data_ptr(), ws.numel(), _stream(dweight)))
+    return dweight
+
+
+def _grouped_check(ts, offsets, groups):
+    first = ts[0][0]
+    for t, what in ts:
+        _require_device(t, what)
+        if t.dtype != first.dtype or t.device != first.device:
+            raise ValueError("fpemu grouped product: %s must have the others' dtype and device" % what)
+    _require_words(offsets, first, groups + 1, "offsets")
+
+
+def grouped_gemm_(y, x, weight, offsets, w_trans=False):
+    """y[i] = x[i] @ W_g for the rows i of group g; weight [G, K, N], or [G, N, K] when w_trans."""
+    G, a, b = weight.shape
+    N, K = (a, b) if w_trans else (b, a)
+    _grouped_check([(y, "y"), (x, "x"), (weight, "weight")], offsets, G)
+    if x.dim() != 2 or x.shape[1] != K or tuple(y.shape) != (x.shape[0], N):
+        raise ValueError("fpemu grouped product: shapes do not match: x %s, weight %s, y %s" % (
+            tuple(x.shape), tuple(weight.shape), tuple(y.shape)))
+    with _range("fpemu::grouped_gemm"), _on_device(x):
+        _check(lib().fpemu_grouped_gemm(y.data_ptr(), x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), x.shape[0], N, K, G,
+                                        _dtype_id(x), int(bool(w_trans)), _stream(x)))
+    return y
+
+
+def grouped_gemm_wgrad_(dweight, a, b, offsets):
+    """dweight[g] = a_g^T @ b_g over the rows of group g; dweight [G, P, Q], a [M, P], b [M, Q]."""
+    G, P, Q = dweight.shape
+    _grouped_check([(dweight, "dweight"), (a, "a"), (b, "b")], offsets, G)
+    if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[0] or a.shape[1] != P or b.shape[1] != Q:
+        raise ValueError("fpemu grouped product: shapes do not match: dweight %s, a %s, b %s" % (
+            tuple(dweight.shape), tuple(a.shape), tuple(b.shape)))
+    with _range("fpemu::grouped_gemm_wgrad"), _on_device(a):
+        _check(lib().fpemu_grouped_gemm_wgrad(dweight.data_ptr(), a.data_ptr(), b.data_ptr(), offsets.data_ptr(), a.shape[0], P,
+                                              Q, G, _dtype_id(a), _stream(a)))
+    return dweight
+
+
+class _GradEntry(ctypes.Structure):  # fpemu_grad_t
+    _fields_ = [("inp", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_uint64), ("in_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32)]
+
+
+NORM_INF, NORM_1, NORM_2 = 0, 1, 2
+
+
+def _grad_table(grads, outs):
+    tab = (_GradEntry * max(1, len(grads)))()
+    for e, g, o in zip(tab, grads, outs):
+        e.inp, e.out, e.n, e.in_dtype, e.out_dtype = g.data_ptr(), o.data_ptr(), g.numel(), _dtype_id(g), _dtype_id(o)
+    return ctypes.cast(tab, ctypes.c_void_p), tab
+
+
+def grad_norm_multi_(grads, order, total, norm=None):
+    """total (float64[1]) <- sum of |g|^p (NORM_1, NORM_2) or max |g| (NORM_INF) over a list of dense device tensors on
+    one device, 16- and 32-bit types mixed; norm (float32[1] or None) <- the norm."""
+    ptr, _keep = _grad_table(grads, grads)
+    ws = _scratch(lib().fpemu_grad_norm_workspace_bytes(len(grads)), total)
+    with _range("fpemu::grad_norm_multi"), _on_device(total):
+        _check(lib().fpemu_grad_norm_multi(ptr, len(grads), order, total.data_ptr(), None if norm is None else norm.data_ptr(),
+                                           ws.data_ptr(), ws.numel(), _stream(total)))
+    return total
+
+
+def clip_multi_(grads, outs, order, total, max_norm, norm=None):
+    """outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) with the norm taken from total on the device."""
+    ptr, _keep = _grad_table(grads, outs)
+    with _range("fpemu::clip_multi"), _on_device(total):
+        _check(lib().fpemu_clip_multi(ptr, len(grads), order, total.data_ptr(), float(max_norm),
+                                      None if norm is None else norm.data_ptr(), _stream(total)))
+    return outs
 
 
 def forward(input, mode, size, inplace, scale, block_norm=False, block_size=1):

@@ -30,6 +30,7 @@ import threading
 
 import torch
 
+from .module_wrappers import GroupedLinear, GroupedMatmul
 from .pytquant.hip import _binding as _hip
 
 _FLT_MAX = {"e5m2": 57344.0, "e4m3": 448.0, "e4m3_ieee": 240.0, "e3m4": 30.0, "fp4": 1.0}
@@ -223,7 +224,7 @@ class ModuleQuantConfig(object):
                 grad.data = quantize_tensor(grad.data, self.wtgrad_qconfig, None, inplace=True)
             return grad
 
-        if type(module) in [torch.nn.Conv2d, torch.nn.Linear]:
+        if type(module) in [torch.nn.Conv2d, torch.nn.Linear, GroupedLinear]:
             if module.weight is not None and module.weight.requires_grad:
                 module.weight.register_hook(quantize_weight_grad)
 
@@ -737,6 +738,11 @@ def _active(qtconfig):
     return qtconfig is not None and qtconfig.is_enabled
 
 
+def _is_offsets(module, t):
+    """Where the groups of a grouped product begin (and what autograd hands back as its gradient): integers, not values."""
+    return type(module) in (GroupedLinear, GroupedMatmul) and torch.is_tensor(t) and not t.is_floating_point()
+
+
 def quantize_module_weights_and_inputs(self, input):
     """forward-pre hook: weights in place, then every positional input out of place."""
     qc = self.qconfig
@@ -751,7 +757,8 @@ def quantize_module_weights_and_inputs(self, input):
         self.weight.data = quantize_tensor(self.weight.data, qc.wt_qconfig, self.qparams.wt_qparams, inplace=True)
     if _active(qc.iact_qconfig):
         with shared_input_memo():   # modules that share an input: the repeat of the last quantisation is its result
-            input = tuple(quantize_tensor(t, qc.iact_qconfig, None, inplace=False) for t in input)
+            input = tuple(t if _is_offsets(self, t) else quantize_tensor(t, qc.iact_qconfig, None, inplace=False)
+                          for t in input)
     return input
 
 
@@ -761,8 +768,8 @@ def quantize_module_gradient(self, grad_input, grad_output):
     if qc.sparse_config is not None and qc.sparse_config.ingrad:
         grad_input = tuple(qc.sparse_config.sparsify_ingrad_tensor(g) for g in grad_input)
     if _active(qc.igrad_qconfig):
-        grad_input = tuple(g if g is None else quantize_tensor(g, qc.igrad_qconfig, self.qparams.igrad_qparams,
-                                                                inplace=False) for g in grad_input)
+        grad_input = tuple(g if g is None or _is_offsets(self, g) else quantize_tensor(g, qc.igrad_qconfig, self.qparams.igrad_qparams,
+                                                                                      inplace=False) for g in grad_input)
     if qc.wt_qconfig is not None and (qc.wt_qconfig.dtype in ["bfloat16"] or qc.device == 'cpu'):
         self.weight.data = copy.deepcopy(qc.weight_master)
     return grad_input

@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define FPEMU_ABI_VERSION 10
+#define FPEMU_ABI_VERSION 11
 
 /* Storage dtype of in/out buffers.  FPEMU_F64 is served by fpemu_cast / fpemu_forward (plain casts, no block norm)
  * only -- the reference's GPU dispatcher takes double tensors (AT_DISPATCH_FLOATING_TYPES_AND_HALF,
@@ -336,6 +336,67 @@ int fpemu_conv2d_bp_f32(float *gin, const float *gout, const float *w, int64_t N
 int fpemu_conv2d_wu_f32(float *gw, const float *gout, const float *in, int64_t N, int64_t C, int64_t H,
                         int64_t W, int64_t K, int64_t R, int64_t S, int64_t stride, int64_t pad, int variant,
                         void *ws, uint64_t ws_bytes, void *stream);
+
+/* ---- operators of a language model's training step --------------------------------------------------------------
+ * What runs beside the emulated cast in such a model: rows in the order of their group, the scaled embedding lookup and
+ * its table's gradient, matrix products by group, the norm and clipping of a list of gradients.  Sums are held in 32
+ * bits or more and rounded once, when they are stored; every sum has one fixed order, so a repeated call gives the same
+ * bits.  Workspaces belong to the caller, need no initialising and are free again, in stream order, after the call.
+ * Storage types: FPEMU_F32, FPEMU_F16, FPEMU_BF16.  Ids are 4- or 8-byte signed integers (id_bytes). */
+
+/* Stable order of n rows by group: order[i] = the row at place i when the rows are sorted by id, equal ids in their own
+ * order; offsets[g] = rows with an id below g, g = 0 .. groups, so group g holds places offsets[g] .. offsets[g + 1) of
+ * order.  A row whose id is outside [0, groups) belongs to no group: such rows come last, from offsets[groups] on.
+ * n <= 2^31 - 1.  ws: fpemu_group_rows_workspace_bytes(n, groups) bytes (may be 0), 16-byte aligned. */
+uint64_t fpemu_group_rows_workspace_bytes(uint64_t n, uint64_t groups);
+int fpemu_group_rows(const void *ids, int id_bytes, uint64_t n, uint64_t groups, int32_t *order, int32_t *offsets,
+                     void *ws, uint64_t ws_bytes, void *stream);
+
+/* out[t][:] = scale * weight[ids[t]][:], t < n; weight [vocab][width], out [n][width], one storage type.  An id outside
+ * [0, vocab) reads nothing: its row of out is NaN. */
+int fpemu_embedding(const void *weight, const void *ids, int id_bytes, void *out, uint64_t n, uint64_t vocab, uint64_t width,
+                    int dtype, float scale, void *stream);
+
+/* The table's gradient: dweight[v][:] = scale * sum of dout[t][:] over ids[t] = v, every row written (zeros where no
+ * token has the id).  Row `padding` is zero (a negative padding: no such row); ids outside [0, vocab) add to no row.
+ * The sum runs in fp32.  ws: fpemu_embedding_grad_workspace_bytes(...) bytes, 16-byte aligned. */
+uint64_t fpemu_embedding_grad_workspace_bytes(uint64_t n, uint64_t vocab, uint64_t width);
+int fpemu_embedding_grad(const void *dout, const void *ids, int id_bytes, void *dweight, uint64_t n, uint64_t vocab,
+                         uint64_t width, int dtype, float scale, int64_t padding, void *ws, uint64_t ws_bytes, void *stream);
+
+/* Matrix products by group: y[i][:] = x[i][:] @ W_g for offsets[g] <= i < offsets[g + 1]; x [M][K], y [M][N].
+ *   w_trans = 0 : w [groups][K][N], W_g = w[g];   w_trans = 1 : w [groups][N][K], W_g = w[g] transposed (the layout of a
+ *   linear layer's weight).  offsets: groups + 1 device words, not decreasing, within [0, M]; rows outside every group
+ *   are zero in y.  The gradient of x is the same call on dy with the other w_trans.  16-bit types multiply on the matrix
+ *   cores with fp32 sums; fp32 runs the k-ascending fmaf chain of fpemu_gemm_f32 (variant 1), bit for bit. */
+int fpemu_grouped_gemm(void *y, const void *x, const void *w, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
+                       int64_t groups, int dtype, int w_trans, void *stream);
+
+/* Gradient of the weights: dw[g] = a_g^T b_g, the sum over group g's rows of a [M][P] and b [M][Q]; dw [groups][P][Q],
+ * zeros for an empty group.  (a, b) = (x, dy) for weights [K][N], (dy, x) for weights [N][K]. */
+int fpemu_grouped_gemm_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, int64_t M, int64_t P, int64_t Q,
+                             int64_t groups, int dtype, void *stream);
+
+/* Norm of a list of gradients as ONE vector, and their clipping; types may differ within a list.  `in` is the gradient,
+ * `out` (fpemu_clip_multi only) receives the clipped one: the same buffer, or another one of the same type or fp32.
+ *   fpemu_grad_norm_multi : *sum = sum of |g|^p (p = 1, 2) or max |g| (infinity) over all elements, in 64 bits; a NaN
+ *                           stays a NaN.  norm (or NULL) receives the norm itself.  ws:
+ *                           fpemu_grad_norm_workspace_bytes(count) bytes, 8-byte aligned.
+ *   fpemu_clip_multi      : out = in * min(1, max_norm / (norm + 1e-6)), the norm taken from *sum on the device (ranks
+ *                           that hold shards add their sums up in between); norm (or NULL) receives it.
+ * The tables are host memory, read before the call returns. */
+enum { FPEMU_NORM_INF = 0, FPEMU_NORM_1 = 1, FPEMU_NORM_2 = 2 };
+typedef struct fpemu_grad {
+  const void *in;
+  void *out;
+  uint64_t n;
+  int32_t in_dtype, out_dtype;
+} fpemu_grad_t;
+uint64_t fpemu_grad_norm_workspace_bytes(uint64_t count);
+int fpemu_grad_norm_multi(const fpemu_grad_t *grads, uint64_t count, int order, double *sum, float *norm, void *ws,
+                          uint64_t ws_bytes, void *stream);
+int fpemu_clip_multi(const fpemu_grad_t *grads, uint64_t count, int order, const double *sum, float max_norm, float *norm,
+                     void *stream);
 
 #ifdef __cplusplus
 }

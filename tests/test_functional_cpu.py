@@ -1,0 +1,138 @@
+"""Refusals of the training operators (mpemu.functional and their C entry points): decided on the host before anything
+is enqueued, so they need no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from mpemu import functional as F
+from mpemu.module_wrappers import GroupedLinear, ScaledEmbedding
+from mpemu.pytquant.hip import _binding as b
+
+INT, FLT = torch.zeros(4, dtype=torch.int64), torch.zeros(4, 4)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: F.group_rows(INT.float(), 4), lambda: F.group_rows([1, 2], 4), lambda: F.group_rows(INT.to(torch.int16), 4),
+    lambda: F.embedding(FLT, FLT), lambda: F.embedding(INT, FLT.double()), lambda: F.embedding(INT, INT),
+    lambda: F.grouped_mm(INT, FLT, INT), lambda: F.grouped_mm(FLT.double(), FLT, INT),
+    lambda: F.clip_grads_([INT], 1.0), lambda: F.clip_grads_([FLT.to_sparse()], 1.0), lambda: F.grad_norm([FLT.double()])])
+def test_wrong_types_raise_type_error(call):
+    with pytest.raises(TypeError):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: F.group_rows(INT, 4), lambda: F.embedding(INT, FLT), lambda: F.grouped_mm(FLT, FLT[None], INT),
+    lambda: F.clip_grads_([FLT], 1.0), lambda: F.grad_norm([FLT])])
+def test_cpu_tensors_raise(call):
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        call()
+
+
+def test_values_refused_without_gpu():
+    with pytest.raises(ValueError):
+        F.grad_norm([], norm_type=3.0)
+    with pytest.raises(ValueError):
+        F.clip_grads_([], -1.0)
+    with pytest.raises(ValueError):
+        F.clip_grads_([], float("nan"))
+    assert float(F.grad_norm([])) == 0.0
+    assert float(F.clip_grad_norm_([torch.nn.Parameter(FLT)], 1.0)) == 0.0    # no gradient yet
+
+
+def test_overlap_rule():
+    t = torch.zeros(64)
+    a, c = t[:16], t[16:32]
+    assert not F._overlap([a, c], [a, c])                 # in place, side by side
+    assert F._overlap([a, a], [a, a])                     # the same buffer twice
+    assert F._overlap([t[:17], c], [t[:17], c])
+    assert not F._overlap([a, a], [t[32:48], t[48:]])     # read twice, written apart
+    assert F._overlap([a, c], [c, t[32:48]])              # an output is another one's gradient
+    assert not F._overlap([t[:0], t[:0]], [t[:0], t[:0]])
+
+
+def test_dense_views():
+    w = torch.zeros(8, 6, 3, 3).contiguous(memory_format=torch.channels_last)
+    assert F._dense(w).data_ptr() == w.data_ptr() and F._dense(w.t() if w.dim() == 2 else w).data_ptr() == w.data_ptr()
+    assert F._dense(torch.zeros(4, 6)[:, ::2]).data_ptr() != 0 and F._dense(torch.zeros(4, 6)[:, ::2]).is_contiguous()
+
+
+def test_c_entries_refuse():
+    L = b.lib()
+    # ids: null, odd sizes, too many rows or groups, misaligned
+    assert L.fpemu_group_rows(None, 8, 4, 4, 16, 16, None, 0, None) == -1
+    assert L.fpemu_group_rows(16, 2, 4, 4, 16, 16, None, 0, None) == -1
+    assert L.fpemu_group_rows(16, 8, 1 << 31, 4, 16, 16, None, 0, None) == -1
+    assert L.fpemu_group_rows(16, 8, 4, 0, 16, 16, None, 0, None) == -1
+    assert L.fpemu_group_rows(16, 8, 4, (1 << 31) - 1, 16, 16, None, 0, None) == -1
+    assert L.fpemu_group_rows(20, 8, 4, 4, 16, 16, None, 0, None) == -4
+    assert L.fpemu_group_rows(16, 8, 4, 4, 16, None, None, 0, None) == -1
+    assert L.fpemu_group_rows(16, 8, 8192, 4, 16, 16, None, 0, None) == -1            # workspace missing
+    assert L.fpemu_group_rows(16, 8, 8192, 4, 16, 16, 16, 64, None) == -1             # workspace too small
+    assert L.fpemu_group_rows_workspace_bytes(8192, 4) > 64
+    # embedding
+    assert L.fpemu_embedding(16, 16, 8, 16, 4, 8, 8, 3, 1.0, None) == -1              # fp64
+    assert L.fpemu_embedding(None, 16, 8, 16, 4, 8, 8, 0, 1.0, None) == -1
+    assert L.fpemu_embedding(18, 16, 8, 16, 4, 8, 8, 0, 1.0, None) == -4
+    assert L.fpemu_embedding(16, 16, 8, 16, 0, 8, 8, 0, 1.0, None) == 0               # nothing to do
+    assert L.fpemu_embedding(16, 16, 8, 16, 4, 8, 0, 0, 1.0, None) == 0
+    assert L.fpemu_embedding_grad(16, 16, 8, 16, 4, 8, 8, 0, 1.0, -1, None, 0, None) == -1
+    assert L.fpemu_embedding_grad(16, 16, 8, 16, 4, 8, 8, 0, 1.0, -1, 16, 8, None) == -1
+    # grouped products
+    assert L.fpemu_grouped_gemm(16, 16, 16, None, 4, 4, 4, 2, 0, 0, None) == -1
+    assert L.fpemu_grouped_gemm(16, 16, 16, 16, 4, 4, 4, 0, 0, 0, None) == -1
+    assert L.fpemu_grouped_gemm(16, 16, 16, 16, -1, 4, 4, 2, 0, 0, None) == -1
+    assert L.fpemu_grouped_gemm(16, 16, 16, 16, 4, 4, 4, 2, 3, 0, None) == -1
+    assert L.fpemu_grouped_gemm(None, 16, 16, 16, 4, 4, 4, 2, 0, 0, None) == -1
+    assert L.fpemu_grouped_gemm(18, 16, 16, 16, 4, 4, 4, 2, 0, 0, None) == -4
+    assert L.fpemu_grouped_gemm(16, 16, 16, 16, 0, 4, 4, 2, 0, 0, None) == 0
+    assert L.fpemu_grouped_gemm_wgrad(16, 16, 16, 16, 4, 0, 4, 2, 0, None) == 0
+    assert L.fpemu_grouped_gemm_wgrad(None, 16, 16, 16, 4, 4, 4, 2, 0, None) == -1
+    # norm and clipping
+    tab = (b._GradEntry * 2)()
+    tab[0].inp, tab[0].out, tab[0].n, tab[0].in_dtype, tab[0].out_dtype = 4096, 4096, 4, 0, 0
+    tp = ctypes.cast(tab, ctypes.c_void_p)
+    assert L.fpemu_grad_norm_multi(tp, 1, 7, 16, None, 16, 1 << 20, None) == -1       # order
+    assert L.fpemu_grad_norm_multi(tp, 1, 2, None, None, 16, 1 << 20, None) == -1
+    assert L.fpemu_grad_norm_multi(tp, 1, 2, 16, None, 16, 8, None) == -1             # workspace too small
+    assert L.fpemu_grad_norm_multi(None, 1, 2, 16, None, 16, 1 << 20, None) == -1
+    assert L.fpemu_clip_multi(tp, 1, 2, 16, -1.0, None, None) == -1
+    assert L.fpemu_clip_multi(tp, 1, 2, 16, float("nan"), None, None) == -1
+    assert L.fpemu_clip_multi(tp, 1, 2, None, 1.0, None, None) == -1
+    tab[0].out = 4104                                                                 # overlaps its gradient
+    assert L.fpemu_clip_multi(tp, 1, 2, 16, 1.0, None, None) == -1
+    assert b"overlap" in L.fpemu_last_error()
+    tab[0].out, tab[0].out_dtype = 8192, 1                                            # fp32 into fp16
+    assert L.fpemu_clip_multi(tp, 1, 2, 16, 1.0, None, None) == -1
+    tab[0].inp = 4098
+    assert L.fpemu_clip_multi(tp, 1, 2, 16, 1.0, None, None) == -4
+
+
+def test_modules_and_their_hooks_configure():
+    """The wrappers are hook targets: experts and embeddings get the configurations of linear layers and embeddings."""
+    from mpemu.e4m3_emu import E4M3Emulator
+    from mpemu.hybrid_emu import HybridEmulator
+    from mpemu.module_wrappers import GroupedMatmul
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.emb = ScaledEmbedding(10, 8, padding_idx=1, scale=2.0)
+            self.experts = GroupedLinear(3, 8, 4)
+            self.product = GroupedMatmul()
+            self.lin = torch.nn.Linear(8, 4)
+
+    model = Model().train()
+    assert "scale=2.0" in repr(model.emb) and "num_groups=3" in repr(model.experts)
+    assert float(model.emb.weight[1].abs().sum()) == 0.0          # nn.Embedding's own rule for the padding entry
+    emu = HybridEmulator(model, None, device="cpu")
+    emu.prepare_model(model, None, None)
+    d = emu.model_qconfig_dict
+    assert repr(d["experts"]) == repr(d["lin"])
+    assert d["emb"].iact_qconfig is None and d["product"].wt_qconfig is None
+    assert model.experts.weight._backward_hooks            # weight gradients are quantised, as a linear layer's
+    emu = E4M3Emulator(Model(), None, device="cpu", train=True)
+    emu.prepare_model(emu.model, None, None)
+    assert emu.model_qconfig_dict["experts"].wt_qconfig is not None
+    assert emu.model_qconfig_dict["product"].wt_qconfig is None

@@ -1,0 +1,601 @@
+"""The training operators (mpemu.functional) against plain implementations in 64 bits.
+
+Tolerances.  A stored value is off by at most half a step of its type, eps(t) / 2 relative to it (fp16: 2^-25 absolute below
+its normal range).  A sum of n terms in fp32 is off by at most n steps of 2^-24 (additions rounded to nearest) or 2^-23 (the
+matrix unit may cut) of the sum of the terms' magnitudes.  Norms are summed in 64 bits and rounded to fp32 once."""
+import math
+
+import pytest
+import torch
+
+from mpemu import functional as F
+from mpemu.cmodel import simple
+from mpemu.pytquant.hip import _binding as hip
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}
+
+
+@pytest.fixture(params=["native", "ctypes"])
+def front(request, monkeypatch):
+    """Both ways to the kernels: the C++ front and the ctypes binding."""
+    if request.param == "ctypes":
+        monkeypatch.setattr(F, "_native", lambda: None)
+    else:
+        assert F._native() is not None
+    return request.param
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def randn(shape, dtype, seed, std=1.0):
+    return (torch.randn(shape, generator=gen(seed), device=DEV) * std).to(dtype)
+
+
+def close(got, want, slack, what=""):
+    """|got - want| <= slack + half a step of got's type."""
+    bound = slack + want.abs() * (torch.finfo(got.dtype).eps / 2) + TINY[got.dtype]
+    d = (got.double() - want).abs()
+    assert got.shape == want.shape
+    assert bool((d <= bound).all()), "%s: off by %g over the bound at %s" % (
+        what, float((d - bound).max()), (d - bound).argmax().item())
+
+
+# ---- rows by group ------------------------------------------------------------------------------------------------------
+def check_group(ids, groups):
+    order, offsets = F.group_rows(ids, groups)
+    flat = ids.reshape(-1).cpu().long()
+    key = torch.where((flat >= 0) & (flat < groups), flat, groups)
+    want = torch.sort(key, stable=True).indices
+    assert order.dtype == offsets.dtype == torch.int32 and tuple(offsets.shape) == (groups + 1,)
+    assert torch.equal(order.cpu().long(), want)
+    assert torch.equal(offsets.cpu().long(), torch.searchsorted(key[want], torch.arange(groups + 1)))
+
+
+@pytest.mark.parametrize("n", [0, 1, 63, 64, 65, 511, 4095, 4096, 4097, 20000, 4096 * 32 + 1, 4096 * 70 + 5])
+@pytest.mark.parametrize("groups", [1, 2, 8, 1023, 1024, 30522])
+def test_group_rows(n, groups):
+    ids = torch.randint(0, groups, (n,), generator=gen(n + groups), device=DEV)
+    check_group(ids, groups)
+
+
+@pytest.mark.parametrize("groups", [(1 << 20) - 1, 1 << 20, (1 << 22) + 3])
+@pytest.mark.parametrize("n", [1, 3000, 9000])
+def test_group_rows_many_groups(n, groups):
+    """One digit more than two passes hold, and the sizes around it."""
+    check_group(torch.randint(0, groups, (n,), generator=gen(n), device=DEV), groups)
+
+
+def test_group_rows_outside_int32_and_shapes(front):
+    ids = torch.tensor([[3, -1, 0, 9], [2 ** 40, 3, -2 ** 63, 0]], device=DEV)
+    check_group(ids, 4)
+    check_group(ids.clamp(-5, 100).int(), 4)
+    check_group(ids.t(), 4)                                  # not contiguous
+    check_group(torch.full((5000,), 7, device=DEV), 3)       # nobody has a group
+    check_group(torch.full((9000,), 1, device=DEV, dtype=torch.int32)[::3], 3)
+
+
+# ---- embedding ----------------------------------------------------------------------------------------------------------
+def embedding_reference(ids, weight, scale, padding, dout):
+    flat, wide = ids.reshape(-1), weight.double()
+    known = (flat >= 0) & (flat < weight.shape[0])
+    out = wide[flat.clamp(0, weight.shape[0] - 1)] * scale
+    out[~known] = math.nan
+    counted = known if padding is None else known & (flat != padding % weight.shape[0])
+    d = dout.double().reshape(-1, weight.shape[1])[counted] * scale
+    dweight = torch.zeros_like(wide).index_add_(0, flat[counted], d)
+    size = torch.zeros_like(wide).index_add_(0, flat[counted], d.abs())
+    count = torch.bincount(flat[counted], minlength=weight.shape[0]).double()
+    return out.reshape(tuple(ids.shape) + (weight.shape[1],)), dweight, size * (count + 2).unsqueeze(1) * 2.0 ** -24
+
+
+def check_embedding(ids, weight, scale, padding, seed=5):
+    weight = weight.detach().requires_grad_(True)
+    out = F.embedding(ids, weight, scale=scale, padding_idx=padding)
+    dout = randn(out.shape, out.dtype, seed)
+    dweight, = torch.autograd.grad(out, (weight,), dout)
+    want, dwant, slack = embedding_reference(ids, weight.detach(), scale, padding, dout)
+    nan = want.isnan()
+    assert torch.equal(out.isnan(), nan) and out.dtype == weight.dtype
+    close(out.detach()[~nan], want[~nan], want[~nan].abs() * 2.0 ** -24, "out")
+    close(dweight, dwant, slack, "dweight")
+    with torch.no_grad():
+        assert torch.equal(F.embedding(ids, weight, scale=scale)[~nan], out.detach()[~nan])
+    return dweight
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,vocab,width", [(1, 30522, 768), (7, 1, 5), (64, 100, 64), (1023, 50, 33), (5000, 1000, 130),
+                                                (300, 70000, 8), (2048, 512, 1), (100, 300, 4100)])
+def test_embedding(dtype, tokens, vocab, width):
+    ids = torch.randint(0, vocab, (tokens,), generator=gen(tokens), device=DEV)
+    check_embedding(ids, randn((vocab, width), dtype, 1), 27.75, None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_frequent_entries(dtype):
+    """Runs that fill chunks, end inside one, begin inside one, and one entry with nearly everything."""
+    ids = torch.cat([torch.full((31,), 3), torch.full((33,), 4), torch.full((640,), 9), torch.full((32,), 11),
+                     torch.full((9000,), 40), torch.arange(0, 60)])
+    ids = ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(3))].to(DEV)
+    check_embedding(ids, randn((64, 200), dtype, 2), 1.0, None)
+    check_embedding(torch.full((70000,), 2, device=DEV), randn((5, 24), dtype, 2), 0.5, None)
+
+
+def test_embedding_padding_outside_shapes(front):
+    ids = torch.tensor([[0, 5, 5, 0], [-1, 9, 10, 2 ** 40], [1, 1, 1, 0]], device=DEV)
+    w = randn((10, 12), torch.float32, 3)
+    dweight = check_embedding(ids, w, 2.0, 0)
+    assert float(dweight[0].abs().sum()) == 0.0 and float(dweight[1].abs().sum()) > 0.0
+    check_embedding(ids.clamp(-1, 10).int(), w.half(), 2.0, -1)          # the last entry pads
+    check_embedding(ids.t(), w.bfloat16(), 1.5, None)                      # ids not contiguous
+    check_embedding(ids, randn((12, 10), torch.float32, 4).t(), 1.0, None)   # weight not contiguous
+    check_embedding(torch.zeros(0, 3, dtype=torch.int64, device=DEV), w, 1.0, None)
+    check_embedding(torch.tensor(4, device=DEV), w, 1.0, None)             # 0-d
+
+
+def test_embedding_views_at_odd_addresses():
+    for dtype in TYPES:
+        flat = randn((1 + 50 * 16,), dtype, 6)
+        check_embedding(torch.randint(0, 50, (90,), generator=gen(1), device=DEV), flat[1:].view(50, 16), 3.0, None)
+
+
+def test_embedding_broadcast_gradient(front):
+    """A sum's gradient is one number seen through strides of zero."""
+    w = randn((20, 16), torch.float32, 7).requires_grad_(True)
+    ids = torch.tensor([1, 1, 2, 19], device=DEV)
+    F.embedding(ids, w, scale=0.5).sum().backward()
+    want = torch.zeros(20, 16, device=DEV)
+    want[1], want[2], want[19] = 1.0, 0.5, 0.5
+    assert torch.equal(w.grad, want)
+
+
+def test_embedding_gradient_against_differences():
+    w = randn((6, 4), torch.float32, 8)
+    ids, v = torch.tensor([0, 3, 3, 5], device=DEV), randn((4, 4), torch.float32, 9)
+
+    def f(t):
+        return float((F.embedding(ids, t, scale=1.25).double() * v.double()).sum())
+
+    g, = torch.autograd.grad((F.embedding(ids, w.requires_grad_(True), scale=1.25) * v).sum(), (w,))
+    w = w.detach()
+    for i, j in ((0, 0), (3, 2), (5, 3), (1, 1)):
+        d = torch.zeros_like(w)
+        d[i, j] = 0.5    # linear: any step will do; fp32 products of about 1 are off by 2^-24 each
+        assert abs((f(w + d) - f(w - d)) - float(g[i, j])) < 32 * 2.0 ** -22
+
+
+def test_embedding_refusals(front):
+    w, ids = randn((10, 4), torch.float32, 1), torch.tensor([1], device=DEV)
+    for bad in (lambda: F.embedding(ids, w[0]), lambda: F.embedding(ids, w, padding_idx=10), lambda: F.embedding(ids, w, padding_idx=-11),
+                lambda: F.embedding(ids, w[:0])):
+        with pytest.raises(ValueError):
+            bad()
+    out = F.embedding(ids, w.requires_grad_(True))
+    with pytest.raises(RuntimeError):   # once only: no silent zero for the second derivative
+        g, = torch.autograd.grad(out.sum(), (w,), create_graph=True)
+        torch.autograd.grad(g.sum(), (w,))
+
+
+# ---- products by group --------------------------------------------------------------------------------------------------------
+def offsets_of(sizes, first=0, dtype=torch.int32):
+    return torch.tensor([first] + [first + sum(sizes[:i + 1]) for i in range(len(sizes))], dtype=dtype, device=DEV)
+
+
+def check_grouped(x, weight, offsets, seed=11):
+    """y and both gradients; dy is random.  Rows of no group get zeros whatever x holds there."""
+    x, weight = x.detach().requires_grad_(True), weight.detach().requires_grad_(True)
+    y = F.grouped_mm(x, weight, offsets)
+    dy = randn(y.shape, y.dtype, seed)
+    dx, dw = torch.autograd.grad(y, (x, weight), dy)
+    X, W, DY, o = x.detach().double(), weight.detach().double(), dy.double(), offsets.tolist()
+    want = [torch.zeros(t.shape, dtype=torch.float64, device=DEV) for t in (y, x, weight)]
+    slack = [torch.zeros_like(t) for t in want]
+    u = 2.0 ** -24 if x.dtype == torch.float32 else 2.0 ** -23
+    for g in range(weight.shape[0]):
+        r = slice(o[g], o[g + 1])
+        for k, (a, b, at) in enumerate(((X[r], W[g], r), (DY[r], W[g].t(), r), (X[r].t(), DY[r], g))):
+            want[k][at] = a @ b
+            slack[k][at] = (a.abs() @ b.abs()) * ((a.shape[1] + 1) * u)
+    for got, w, s, what in zip((y.detach(), dx, dw), want, slack, ("y", "dx", "dweight")):
+        assert got.dtype == x.dtype
+        close(got, w, s, what)
+    with torch.no_grad():
+        assert torch.equal(F.grouped_mm(x, weight, offsets), y.detach())
+    return y.detach(), dx, dw
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("linear", [False, True])
+@pytest.mark.parametrize("sizes,K,N", [([1], 64, 64), ([1, 0, 2, 0], 128, 96), ([130, 1, 255, 0, 64], 200, 264), ([5, 300], 33, 65),
+                                       ([257, 128, 129], 64, 520), ([16] * 70, 256, 48), ([3, 1], 1, 1), ([0, 0], 40, 24),
+                                       ([700, 0, 5], 1032, 136)])
+def test_grouped_mm(dtype, linear, sizes, K, N):
+    M, G = sum(sizes), len(sizes)
+    x = randn((M, K), dtype, 1)
+    w = randn((G, N, K), dtype, 2).transpose(1, 2) if linear else randn((G, K, N), dtype, 2)
+    check_grouped(x, w, offsets_of(sizes))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_mm_rows_of_no_group(dtype):
+    """Rows before the first and behind the last group hold infinities and NaN: they reach nothing, and come out zero."""
+    x = randn((300, 64), dtype, 3)
+    x[:7], x[290:] = math.inf, math.nan
+    y, dx, dw = check_grouped(x, randn((3, 64, 72), dtype, 4), offsets_of([100, 0, 183], first=7))
+    for t in (y, dx):
+        assert float(t[:7].abs().sum()) == 0.0 and float(t[290:].abs().sum()) == 0.0
+    assert bool(torch.isfinite(dw).all())
+    check_grouped(randn((50, 64), dtype, 3), randn((2, 64, 8), dtype, 4), offsets_of([0, 0], first=20))   # nobody at all
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_mm_infinities_stay_in_their_group(dtype):
+    x = randn((200, 128), dtype, 5)
+    x[100:] = math.nan      # the second group's rows: in tiles and contractions next to the first group's
+    w = randn((2, 128, 64), dtype, 6).requires_grad_(True)
+    o = offsets_of([100, 100])
+    y = F.grouped_mm(x, w, o)
+    assert bool(torch.isfinite(y[:100]).all()) and bool(y[100:].isnan().all())
+    dw, = torch.autograd.grad(y, (w,), torch.ones_like(y))
+    assert bool(torch.isfinite(dw[0]).all()) and bool(dw[1].isnan().all())
+
+
+def test_grouped_mm_fp32_is_the_cmodel_chain():
+    """fp32 products are the c-model's, bit for bit, forward and backward."""
+    sizes, K, N = [70, 0, 129, 31], 100, 90
+    x, w, o = randn((230, K), torch.float32, 7).requires_grad_(True), randn((4, K, N), torch.float32, 8).requires_grad_(True), offsets_of(sizes)
+    y = F.grouped_mm(x, w, o)
+    dy = randn(y.shape, y.dtype, 9)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    at = 0
+    for g, n in enumerate(sizes):
+        xs, ws, ds = x.detach()[at:at + n].clone(), w.detach()[g].clone(), dy[at:at + n].clone()
+        if n:
+            assert torch.equal(y.detach()[at:at + n], simple.mm(xs, ws))
+            assert torch.equal(dx[at:at + n], simple.mm(ds, ws.t()))
+            assert torch.equal(dw[g], simple.mm(xs.t(), ds))
+        else:
+            assert float(dw[g].abs().sum()) == 0.0
+        at += n
+
+
+def test_grouped_mm_strides_types_and_needs(front):
+    o = offsets_of([10, 20, 3], dtype=torch.int64)
+    wide = randn((33, 128), torch.bfloat16, 1)
+    check_grouped(wide[:, ::2], randn((3, 64, 40), torch.bfloat16, 2), o)                              # x not contiguous
+    check_grouped(wide[:, :64], randn((3, 40, 128), torch.bfloat16, 2)[:, :, ::2].transpose(1, 2), o)   # nor weight
+    flat = randn((1 + 33 * 64,), torch.float16, 3)
+    check_grouped(flat[1:].view(33, 64), randn((1 + 3 * 64 * 40,), torch.float16, 4)[1:].view(3, 64, 40), o)   # odd addresses
+    x, w = randn((33, 64), torch.float32, 5), randn((3, 64, 40), torch.float32, 6)
+    full = check_grouped(x, w, o)
+    y = F.grouped_mm(x.requires_grad_(True), w, o)                                                      # only x, only weight
+    assert torch.equal(torch.autograd.grad(y, (x,), randn(y.shape, y.dtype, 11))[0], full[1])
+    y = F.grouped_mm(x.detach(), w.requires_grad_(True), o)
+    assert torch.equal(torch.autograd.grad(y, (w,), randn(y.shape, y.dtype, 11))[0], full[2])
+    y = F.grouped_mm(x, w, o)
+    y.sum().backward()                                                                                  # a broadcast gradient
+    close(x.grad[:10], (w.detach()[0].double().sum(1))[None].expand(10, 64).clone(), 64 * 64 * 2.0 ** -24)
+
+
+def test_grouped_mm_gradient_against_differences():
+    x, w, o = randn((5, 3), torch.float32, 1).requires_grad_(True), randn((2, 3, 4), torch.float32, 2).requires_grad_(True), offsets_of([2, 3])
+    v = randn((5, 4), torch.float32, 3)
+    dx, dw = torch.autograd.grad((F.grouped_mm(x, w, o) * v).sum(), (x, w))
+
+    def f(a, b):
+        return float((F.grouped_mm(a, b, o).double() * v.double()).sum())
+
+    with torch.no_grad():
+        for t, d, at in ((x, dx, (1, 2)), (x, dx, (4, 0)), (w, dw, (0, 1, 3)), (w, dw, (1, 2, 0))):
+            e = torch.zeros_like(t)
+            e[at] = 0.5
+            up, down = (f(x + e, w), f(x - e, w)) if t is x else (f(x, w + e), f(x, w - e))
+            assert abs((up - down) - float(d[at])) < 64 * 2.0 ** -22
+
+
+def test_grouped_mm_refusals(front):
+    x, w, o = randn((6, 8), torch.float32, 1), randn((2, 8, 4), torch.float32, 2), offsets_of([2, 4])
+    for bad in (lambda: F.grouped_mm(x[0], w, o), lambda: F.grouped_mm(x, w[0], o), lambda: F.grouped_mm(x[:, :7], w, o),
+                lambda: F.grouped_mm(x, w, o[:2]), lambda: F.grouped_mm(x, w[:0], o[:1]), lambda: F.grouped_mm(x, w, o[None])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        F.grouped_mm(x.half(), w, o)
+    with pytest.raises(RuntimeError):
+        y = F.grouped_mm(x.requires_grad_(True), w.requires_grad_(True), o)
+        g, = torch.autograd.grad(y.sum(), (x,), create_graph=True)
+        torch.autograd.grad(g.sum(), (w,))
+
+
+# ---- norm and clipping --------------------------------------------------------------------------------------------------------
+def norm_reference(grads, p):
+    flat = torch.cat([g.detach().double().reshape(-1) for g in grads] + [torch.zeros(1, dtype=torch.float64, device=DEV)])
+    return float(flat.abs().max()) if p == math.inf else float(flat.abs().sum()) if p == 1.0 else float(flat.square().sum().sqrt())
+
+
+def check_clip(grads, max_norm, p, out=None):
+    want = norm_reference(grads, p)
+    coef = min(1.0, max_norm / (want + 1e-6))
+    values = [g.detach().double() * coef for g in grads]
+    assert abs(float(F.grad_norm(grads, p)) - want) <= want * 2.0 ** -23 + 2.0 ** -149
+    norm = F.clip_grads_(grads, max_norm, norm_type=p, out=out)
+    assert norm.dtype == torch.float32 and norm.dim() == 0
+    assert abs(float(norm) - want) <= want * 2.0 ** -23 + 2.0 ** -149
+    for got, v in zip(grads if out is None else out, values):
+        close(got, v, v.abs() * 2.0 ** -21)    # norm, its sum with 1e-6, the quotient and the product: a rounding each
+    return norm
+
+
+SHAPES = [(1000, 77), (1,), (16384,), (16385,), (3, 5, 7), (0,), (40000,), (129,)]
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("share", [0.3, 2.0])
+def test_clip_in_place(p, dtype, share, front):
+    grads = [randn(s, dtype, i, 0.01) for i, s in enumerate(SHAPES)]
+    before = [g.clone() for g in grads]
+    check_clip(grads, norm_reference(grads, p) * share, p)
+    if share > 1.0:
+        assert all(torch.equal(a, b) for a, b in zip(grads, before))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("share", [0.3, 2.0])
+def test_clip_into_master_gradients(dtype, share, front):
+    """16-bit gradients into fp32 ones, both views of flat buffers at odd addresses, types mixed within the list."""
+    n = sum(math.prod(s) for s in SHAPES)
+    sizes = [math.prod(s) for s in SHAPES]
+    flat, master = randn((n + 1,), dtype, 1, 0.01)[1:], torch.full((n + 1,), 7.0, device=DEV)[1:]
+    grads = [t.view(s) for t, s in zip(flat.split(sizes), SHAPES)] + [randn((500,), torch.float32, 2, 0.01)]
+    outs = [t.view(s) for t, s in zip(master.split(sizes), SHAPES)] + [torch.empty(500, device=DEV)]
+    before = flat.clone()
+    check_clip(grads, norm_reference(grads, 2.0) * share, 2.0, out=outs)
+    assert torch.equal(flat, before)
+
+
+def test_clip_many_tensors(front):
+    """More tensors than one launch's table holds, and a list of nothing but empty ones."""
+    grads = [randn((1 + 37 * i % 301,), (torch.float32, torch.bfloat16, torch.float16)[i % 3], i, 0.1) for i in range(400)]
+    check_clip(grads, 1.0, 2.0)
+    assert float(F.clip_grads_([torch.zeros(0, device=DEV)] * 3, 1.0)) == 0.0
+
+
+def test_clip_large_and_small_values():
+    big = [torch.full((1000,), 3.0e38, device=DEV), torch.full((70,), -3.0e38, device=DEV)]
+    check_clip(big, 1.0e38, math.inf)
+    small = [torch.full((100000,), 1.0e-30, device=DEV)]     # squares below fp32's range
+    check_clip(small, 1.0, 2.0)
+    many = [torch.full((1 << 24,), 1.0, device=DEV), torch.full((1 << 20,), 1.0e-4, device=DEV)]
+    check_clip(many, 3.0, 1.0)
+    check_clip([torch.zeros(50, device=DEV)], 1.0, 2.0)
+    check_clip([torch.ones(50, device=DEV)], 0.0, 2.0)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+def test_clip_not_finite(p, front):
+    g = [torch.ones(100, device=DEV), torch.ones(70000, device=DEV)]
+    g[1][69999] = math.nan
+    kept = [t.clone() for t in g]
+    with pytest.raises(RuntimeError):
+        F.clip_grads_(g, 1.0, p, error_if_nonfinite=True)
+    assert all(torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0)) for a, b in zip(g, kept))   # as they were
+    assert math.isnan(float(F.clip_grads_(g, 1.0, p))) and bool(g[0].isnan().all())
+    g = [torch.ones(100, device=DEV), torch.full((3,), -math.inf, device=DEV)]
+    assert float(F.clip_grads_(g, 1.0, p)) == math.inf
+    assert float(g[0].abs().sum()) == 0.0 and bool(g[1].isnan().all())                       # inf * 0, as torch
+
+
+def test_clip_layouts_and_overlap(front):
+    conv = randn((8, 6, 3, 3), torch.float32, 1).contiguous(memory_format=torch.channels_last)
+    strided = randn((40, 30), torch.float32, 2)
+    rest = strided.clone()
+    check_clip([conv, strided[:, ::2]], 0.5, 2.0)
+    assert torch.equal(strided[:, 1::2], rest[:, 1::2])
+    t = randn((100,), torch.float32, 3)
+    for grads, out in (([t, t], None), ([t[:60], t[50:]], None), ([t[:1].expand(9)], None), ([t[:50], t[50:]], [t[50:], torch.empty(50, device=DEV)])):
+        keep = t.clone()
+        with pytest.raises(ValueError):
+            F.clip_grads_(grads, 1.0, out=out)
+        assert torch.equal(t, keep)
+    for grads, out in (([t], [t, t]), ([t], [t[:50]]), ([t], [t.half()])):
+        with pytest.raises(ValueError):
+            F.clip_grads_(grads, 1.0, out=out)
+
+
+def test_clip_grad_norm_of_parameters(front):
+    ps = [torch.nn.Parameter(randn((50, 20), torch.float32, i)) for i in range(4)]
+    for p in ps[:3]:
+        p.grad = randn(p.shape, p.dtype, 9)
+    twin = [p.grad.clone() for p in ps[:3]]
+    norm = F.clip_grad_norm_(iter(ps), 1.5)
+    want = norm_reference(twin, 2.0)
+    assert abs(float(norm) - want) <= want * 2.0 ** -23 and ps[3].grad is None
+    for p, t in zip(ps, twin):
+        v = t.double() * (1.5 / (want + 1e-6))
+        close(p.grad, v, v.abs() * 2.0 ** -21)
+
+
+# ---- streams, capture, repetition -------------------------------------------------------------------------------------------------
+def _step(ids, experts, table, w, o_rows):
+    order, offsets = F.group_rows(experts, w.shape[0])
+    h = F.embedding(ids, table, scale=2.0)
+    y = F.grouped_mm(h.index_select(0, order), w, offsets)
+    dt, dw = torch.autograd.grad(y, (table, w), torch.ones_like(y))
+    norm = F.clip_grads_([dt, dw], 0.5)
+    return [y.detach(), dt, dw, norm, order, offsets]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_and_on_other_streams(dtype):
+    """A whole step in a HIP graph, replayed on new inputs with eager work between the replays, and on a side stream: the
+    eager results, bit for bit (every sum has one order)."""
+    def inputs(seed):
+        return (torch.randint(0, 500, (6000,), generator=gen(seed), device=DEV), torch.randint(0, 9, (6000,), generator=gen(seed + 1), device=DEV))
+
+    table, w = randn((500, 64), dtype, 1).requires_grad_(True), randn((9, 64, 96), dtype, 2, 0.1).requires_grad_(True)
+    ids, experts = inputs(1)
+    eager = [t.clone() for t in _step(ids, experts, table, w, None)]
+    again = _step(ids, experts, table, w, None)
+    assert all(torch.equal(a, b) for a, b in zip(eager, again))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = _step(ids, experts, table, w, None)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(eager, other))
+    graphs = []
+    for _ in range(2):      # two graphs alive at once share nothing
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _step(ids, experts, table, w, None)
+        graphs.append((g, out))
+    for seed in (1, 5, 9, 1):
+        a, b = inputs(seed)
+        ids.copy_(a), experts.copy_(b)
+        want = [t.clone() for t in _step(ids, experts, table, w, None)]
+        for g, out in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            assert all(torch.equal(x, y) for x, y in zip(out, want)), seed
+
+
+@pytest.mark.parametrize("held", ["table", "weight", "view"])
+def test_captured_backward_beside_a_live_eager_graph(held, front):
+    """A capture whose leaves an eager graph still holds would end the process at its backward pass: refused at the forward
+    call, and fine once the eager graph is gone."""
+    table = randn((50, 16), torch.float32, 1).requires_grad_(True)
+    w, o = randn((2, 8, 16), torch.float32, 2).requires_grad_(True), offsets_of([10, 20])
+    ids = torch.randint(0, 50, (30,), generator=gen(3), device=DEV)
+
+    def step():
+        if held == "table":
+            return F.embedding(ids, table)
+        x = F.embedding(ids, table.detach())
+        return F.grouped_mm(x, w.transpose(1, 2) if held == "view" else w.view(2, 16, 8), o)
+
+    alive = step()
+    want = torch.autograd.grad(alive, (table if held == "table" else w,), torch.ones_like(alive), retain_graph=True)[0]
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    if front == "ctypes":
+        return
+    del alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step()
+        got, = torch.autograd.grad(y, (table if held == "table" else w,), torch.ones_like(y))
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+# ---- together, as a model uses them -------------------------------------------------------------------------------------------------
+class Experts(torch.nn.Module):
+    """A small language model with experts: scaled embedding, a router, grouped products, a head."""
+
+    def __init__(self, vocab=97, d=64, ff=96, groups=5, top=2):
+        super().__init__()
+        from mpemu.module_wrappers import GroupedLinear, ScaledEmbedding
+        self.groups, self.top = groups, top
+        self.embeddings = ScaledEmbedding(vocab, d, padding_idx=0, scale=8.0)
+        self.router = torch.nn.Linear(d, groups)
+        self.up, self.down = GroupedLinear(groups, d, ff), GroupedLinear(groups, ff, d)
+        self.head = torch.nn.Linear(d, vocab)
+
+    def forward(self, ids):
+        h = self.embeddings(ids).reshape(-1, self.embeddings.embedding_dim)
+        gate, choice = self.router(h).softmax(-1).topk(self.top, -1)
+        order, offsets = F.group_rows(choice, self.groups)
+        token = order.long() // self.top
+        e = self.down(torch.relu(self.up(h[token], offsets)), offsets) * gate.reshape(-1)[order.long()].unsqueeze(1)
+        return self.head(h + torch.zeros_like(h).index_add(0, token, e))
+
+    def plain(self, ids, dtype=torch.float64):
+        p = {k: v.detach().to(dtype).requires_grad_(True) for k, v in self.named_parameters()}
+        h = p["embeddings.weight"][ids.reshape(-1)] * 8.0
+        gate, choice = (h @ p["router.weight"].t() + p["router.bias"]).softmax(-1).topk(self.top, -1)
+        out = h
+        for k in range(self.top):
+            a = torch.relu((p["up.weight"][choice[:, k]] @ h.unsqueeze(2)).squeeze(2))
+            out = out + (p["down.weight"][choice[:, k]] @ a.unsqueeze(2)).squeeze(2) * gate[:, k:k + 1]
+        return out @ p["head.weight"].t() + p["head.bias"], p
+
+
+def test_model_with_experts_trains():
+    torch.manual_seed(3)
+    model = Experts().to(DEV)
+    ids = torch.randint(1, 97, (4, 50), generator=gen(1), device=DEV)
+    ids[:, 45:] = 0
+    target = torch.randint(0, 97, (200,), generator=gen(2), device=DEV)
+    torch.nn.functional.cross_entropy(model(ids), target).backward()
+    logits, p = model.plain(ids)
+    torch.nn.functional.cross_entropy(logits, target).backward()
+    for name, q in model.named_parameters():
+        want = p[name].grad
+        if name == "embeddings.weight":
+            want[0] = 0.0
+        assert float((q.grad.double() - want).norm()) <= 1e-5 * float(want.norm()), name   # fp32, a dozen layers of sums of < 200 terms
+    norm = F.clip_grad_norm_(model.parameters(), 0.1)
+    total = math.sqrt(sum(float(q.grad.double().square().sum()) for q in model.parameters()))
+    assert float(norm) > 0.1 and abs(total - 0.1) < 1e-5
+
+
+@pytest.mark.parametrize("algo", ["hybrid", "direct"])
+def test_model_with_experts_trains_emulated(algo):
+    """The same under the emulators: hooks on the new modules, gradients clipped in optimizer_step, master weights on the
+    FP16 grid, and what the experts receive on the FP8 grid."""
+    from mpemu import mpt_emu
+    torch.manual_seed(4)
+    model = Experts().to(DEV).train()
+    opt = torch.optim.SGD(model.parameters(), lr=0.1)
+    model, emu = mpt_emu.initialize(model, opt, training_algo=algo, device=DEV, list_exempt_layers=["head", "router"])
+    seen = []
+    model.up.register_forward_pre_hook(lambda m, a: seen.append((a[0].detach().clone(), a[1].clone())))
+    ids = torch.randint(1, 97, (4, 50), generator=gen(1), device=DEV)
+    target = torch.randint(0, 97, (200,), generator=gen(2), device=DEV)
+    for _ in range(2):
+        opt.zero_grad()
+        torch.nn.functional.cross_entropy(model(ids), target).backward()
+        raw = norm_reference([q.grad for q in model.parameters()], 2.0)
+        norm = emu.optimizer_step(opt, max_grad_norm=0.05)
+        assert abs(float(norm) - raw) <= raw * 2.0 ** -23
+        now = norm_reference([q.grad for q in model.parameters()], 2.0)
+        assert now <= max(raw, 0.05) and abs(now - min(raw, 0.05)) < 1e-5
+        for q in model.parameters():
+            assert bool(torch.isfinite(q).all()) and torch.equal(q.detach(), q.detach().half().float())
+    x, offsets = seen[0]
+    assert offsets.dtype == torch.int32 and int(offsets[-1]) == 400
+    assert len(x.unique()) < 600                        # 8-bit values
+    assert emu.optimizer_step(opt) is None
+
+
+def test_model_with_experts_quantised_for_inference():
+    """Post-training quantisation: one scale per expert under per-channel scaling, the table's rows likewise."""
+    from mpemu import mpt_emu, qutils
+    torch.manual_seed(5)
+    model = Experts().to(DEV).eval()
+    up, table = model.up.weight.detach().clone(), model.embeddings.weight.detach().clone()
+    model, _ = mpt_emu.quantize_model(model, dtype="e4m3", device=DEV)
+    cfg = qutils.TensorQuantConfig("e4m3", "rne", "per-channel")
+    for g in range(5):
+        one = qutils.quantize_tensor(up[g:g + 1].contiguous(), cfg, None)
+        assert torch.equal(model.up.weight[g:g + 1].detach(), one)
+    assert torch.equal(model.embeddings.weight.detach(), qutils.quantize_tensor(table, cfg, None))
+    with torch.no_grad():
+        assert bool(torch.isfinite(model(torch.randint(0, 97, (2, 3), device=DEV))).all())
+
+
+def test_abi_of_the_front():
+    assert hip.ext() is not None and hip.ext().abi_version() == hip.lib().fpemu_abi_version() == 11
