@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include <type_traits>
 
@@ -35,7 +36,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // ---- which rows a workgroup works on -----------------------------------------------------------------------------------
 struct RowTile {
   int64_t first, end;   // rows [first, end) of the tile
-  int group;            // -1: rows of no group (zeros), -2: nothing to do
+  int group;            // -1: rows of no group (zeros)
 };
 
 __device__ __forceinline__ int64_t row_at(const int32_t *offsets, int64_t g, int64_t M) {
@@ -43,55 +44,63 @@ __device__ __forceinline__ int64_t row_at(const int32_t *offsets, int64_t g, int
   return o < 0 ? 0 : o > M ? M : o;
 }
 
-// Tile number `tile` of BM rows: group after group, then the rows before the first and behind the last group.  64 groups at
-// a time, one per lane: tiles per group, a prefix sum over the wave, a ballot for the group that holds the tile.
-template <int BM> __device__ __forceinline__ RowTile find_rows(const int32_t *offsets, int64_t groups, int64_t M, uint32_t tile) {
-  const unsigned lane = threadIdx.x & 63u;
-  uint32_t before = 0;
-  for (int64_t g0 = 0; g0 < groups; g0 += 64) {
-    const int64_t g = g0 + lane;
-    int64_t lo = 0, hi = 0;
-    if (g < groups) {
-      lo = row_at(offsets, g, M);
-      hi = row_at(offsets, g + 1, M);
+// Tiles of BM rows are numbered group after group, then the rows before the first and behind the last group.  64 groups at a
+// time, one per lane: tiles per group and a prefix sum over the wave; a ballot finds the group that holds a tile.
+template <int BM> struct TileMap {
+  const int32_t *offsets;
+  int64_t groups, M;
+  uint32_t grouped, heads, tails;   // tiles of the groups, before the first, behind the last
+  int64_t head, tail;
+
+  struct Lane { int64_t lo, hi; uint32_t mine, inc; };
+  __device__ __forceinline__ Lane scan(int64_t g0) const {
+    const unsigned lane = threadIdx.x & 63u;
+    Lane l{0, 0, 0, 0};
+    if (g0 + lane < groups) {
+      l.lo = row_at(offsets, g0 + lane, M);
+      l.hi = row_at(offsets, g0 + lane + 1, M);
     }
-    const uint32_t mine = hi > lo ? (uint32_t)((hi - lo + BM - 1) / BM) : 0u;
-    uint32_t inc = mine;
+    l.inc = l.mine = l.hi > l.lo ? (uint32_t)((l.hi - l.lo + BM - 1) / BM) : 0u;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = (uint32_t)__shfl_up((int)inc, off, 64);
-      if ((int)lane >= off) inc += o;
+      const uint32_t o = (uint32_t)__shfl_up((int)l.inc, off, 64);
+      if ((int)lane >= off) l.inc += o;
     }
-    const uint32_t all = (uint32_t)__shfl((int)inc, 63, 64);
-    if (tile < before + all) {
-      const int at = __ffsll((unsigned long long)__ballot(before + inc > tile)) - 1;
-      const uint32_t start = before + (uint32_t)__shfl((int)(inc - mine), at, 64);
-      const int64_t glo = __shfl((long long)lo, at, 64), ghi = __shfl((long long)hi, at, 64);
-      RowTile r;
-      r.first = glo + (int64_t)(tile - start) * BM;
-      r.end = r.first + BM < ghi ? r.first + BM : ghi;
-      r.group = (int)(g0 + at);
-      return r;
+    return l;
+  }
+  __device__ __forceinline__ TileMap(const int32_t *o, int64_t g, int64_t m) : offsets(o), groups(g), M(m), grouped(0) {
+    for (int64_t g0 = 0; g0 < groups; g0 += 64) grouped += (uint32_t)__shfl((int)scan(g0).inc, 63, 64);
+    head = row_at(offsets, 0, M);
+    tail = row_at(offsets, groups, M);
+    heads = (uint32_t)((head + BM - 1) / BM);
+    tails = (uint32_t)((M - tail + BM - 1) / BM);
+  }
+  __device__ __forceinline__ uint32_t tiles() const { return __builtin_amdgcn_readfirstlane(grouped + heads + tails); }
+  __device__ __forceinline__ RowTile find(uint32_t tile) const {
+    RowTile r;
+    uint32_t before = 0;
+    for (int64_t g0 = 0; tile < grouped && g0 < groups; g0 += 64) {
+      const Lane l = scan(g0);
+      const uint32_t all = (uint32_t)__shfl((int)l.inc, 63, 64);
+      if (tile < before + all) {
+        const int at = __ffsll((unsigned long long)__ballot(before + l.inc > tile)) - 1;
+        const uint32_t start = before + (uint32_t)__shfl((int)(l.inc - l.mine), at, 64);
+        const int64_t lo = __shfl((long long)l.lo, at, 64), hi = __shfl((long long)l.hi, at, 64);
+        r.first = lo + (int64_t)(tile - start) * BM;
+        r.end = r.first + BM < hi ? r.first + BM : hi;
+        r.group = (int)(g0 + at);
+        return r;
+      }
+      before += all;
     }
-    before += all;
+    const uint32_t t = tile - grouped;
+    r.group = -1;
+    r.first = t < heads ? (int64_t)t * BM : tail + (int64_t)(t - heads) * BM;
+    const int64_t end = t < heads ? head : M;
+    r.end = r.first + BM < end ? r.first + BM : end;
+    return r;
   }
-  const int64_t head = row_at(offsets, 0, M), tail = row_at(offsets, groups, M);
-  uint32_t t = tile - before;
-  const uint32_t heads = (uint32_t)((head + BM - 1) / BM), tails = (uint32_t)((M - tail + BM - 1) / BM);
-  RowTile r;
-  r.group = -1;
-  if (t < heads) {
-    r.first = (int64_t)t * BM;
-    r.end = r.first + BM < head ? r.first + BM : head;
-  } else if (t - heads < tails) {
-    r.first = tail + (int64_t)(t - heads) * BM;
-    r.end = r.first + BM < M ? r.first + BM : M;
-  } else {
-    r.first = r.end = 0;
-    r.group = -2;
-  }
-  return r;
-}
+};
 
 // ---- any sizes, any alignment: 128 x 128 tiles, elements staged one by one --------------------------------------------------
 constexpr int GT = 128;
@@ -194,8 +203,9 @@ template <int DT, bool W_TRANS>
 __global__ __launch_bounds__(256) void grouped_any_kernel(typename Storage<DT>::elem *y, const typename Storage<DT>::elem *x,
                                                           const typename Storage<DT>::elem *w, const int32_t *offsets, int64_t M,
                                                           int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
-  const RowTile r = find_rows<GT>(offsets, groups, M, blockIdx.x / col_tiles);
-  if (r.group == -2) return;
+  const TileMap<GT> map(offsets, groups, M);
+  if (blockIdx.x / col_tiles >= map.tiles()) return;
+  const RowTile r = map.find(blockIdx.x / col_tiles);
   const int64_t c0 = (int64_t)(blockIdx.x % col_tiles) * GT;
   f32x16 acc[2][2] = {};
   if (r.group >= 0) {
@@ -217,18 +227,16 @@ __global__ __launch_bounds__(256) void grouped_wgrad_any_kernel(typename Storage
   tile_store<DT>(dw + (int64_t)g * P * Q, Q, p0, P, q0, Q, acc);
 }
 
-// ---- 16-bit storage in whole 16-byte vectors: 128 x 256 tiles fed by loads that go straight to LDS -------------------------
-// 4 waves, each 64 x 128 of the tile as 2 x 4 matrix tiles (128 accumulators); 32 deep in k, three LDS stages of 24 KB, so
-// two stages are in flight while one is multiplied and two workgroups share a CU: one's barrier and LDS reads hide behind
-// the other's matrix instructions.  A wave reads (64 + 128) x 32 bytes from LDS for 8 matrix instructions of 32 cycles, three
-// quarters of what LDS delivers.  An operand whose contraction is contiguous lies in LDS as rows of 64 bytes and is read 16
-// bytes a lane; one whose contraction is its slow dimension lies as it is in memory and is read through the transposing
-// LDS read (lane i of 16 gets column i of 4 k-rows).  The stages are written linearly by the loads, so the bank swizzle is
-// applied to the global address a lane fetches and undone where the fragment is read.
-constexpr int FM = 128, FN = 256, FK = 32, STAGES = 3;
-constexpr int A_BYTES = FM * FK * 2, B_BYTES = FN * FK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int OUT_LD = FN + 8;   // elements; the finished tile goes through LDS to be stored in whole rows
-static_assert(FM * OUT_LD * 2 <= STAGES * STAGE_BYTES, "the tile fits where the stages were");
+// ---- 16-bit storage in whole 16-byte vectors: tiles fed by loads that go straight to LDS ----------------------------------
+// A tile of BM rows x BN columns, 64 deep in k per stage; while one stage is multiplied the next ones are on their way.
+// A stage row of 64 k is 128 bytes, a whole cache line: with 32 deep stages every line was fetched twice (it had left the
+// 32 KB L1 before its second half was asked for), and the tiles then ran at the rate of the L2, not of the matrix cores.
+// An operand whose contraction is contiguous lies in LDS as rows of 128 bytes and is read 16 bytes a lane; one whose
+// contraction is its slow dimension lies as it is in memory and is read through the transposing LDS read (of 16 lanes, lane
+// i gets column i of 4 k-rows).  The loads write LDS linearly, so the bank swizzle is applied to the global address a lane
+// fetches and undone where the fragment is read.
+// Waves: WM x WN over the tile, WK over the four 16-deep steps of a stage (their sums are joined at the end).
+constexpr int FK = 64;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
@@ -237,15 +245,26 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_
 
 // 16 bytes per lane from base + off into LDS at `lds` + 16 * lane.  (Writing M0 needs a wait state before its use.)
 __device__ __forceinline__ void load_to_lds(uint32_t lds, const void *base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_loads() {   // all but the last N loads have arrived, all LDS reads too
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
 }
 
+template <int BM_, int BN_, int WM_, int WN_, int WK_, int STAGES_> struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WK = WK_, STAGES = STAGES_;
+  static constexpr int THREADS = WM * WN * WK * 64;
+  static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;   // matrix tiles of a wave
+  static constexpr int A_BYTES = BM * FK * 2, B_BYTES = BN * FK * 2, STAGE = A_BYTES + B_BYTES;
+  static constexpr int OUT_LD = BN + 8;   // elements; the finished tile goes through LDS to be stored in whole rows
+  static constexpr int JOIN = (WK - 1) * BM * BN * 4, OUT = BM * OUT_LD * 2;
+  static constexpr int LDS = STAGES * STAGE > OUT ? (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN) : (OUT > JOIN ? OUT : JOIN);
+};
+
 // One operand's tile: EXT entries (rows of a row operand, columns of a COL operand) x FK of the contraction.
-template <bool COL, int EXT> struct Panel {
-  static constexpr int LOADS = EXT * FK * 2 / 16 / 256;   // per thread and stage
+template <bool COL, int EXT, int THREADS> struct Panel {
+  static constexpr int LOADS = EXT * FK * 2 / 16 / THREADS;   // per thread and stage
+  static_assert(LOADS * THREADS * 16 == EXT * FK * 2, "whole vectors per thread");
   const char *base;      // uniform: the tile's first element at the stage's first k
   int64_t step;          // bytes from stage to stage
   uint32_t off[LOADS];   // per thread: byte offsets of its vectors in the tile
@@ -264,21 +283,22 @@ template <bool COL, int EXT> struct Panel {
   }
   // entry and k of the first element of this thread's vector j
   __device__ __forceinline__ static void place(int j, int &outer, int &k) {
-    const int id = j * 256 + (int)threadIdx.x;
+    const int id = j * THREADS + (int)threadIdx.x;
     if (COL) {
       constexpr int PER = EXT / 8;
       k = id / PER;
       outer = ((id % PER) ^ swizzle_col(k)) * 8;
     } else {
-      outer = id / 4;
-      k = ((id & 3) ^ ((outer >> 1) & 3)) * 8;
+      outer = id / 8;
+      k = ((id & 7) ^ (outer & 7)) * 8;
     }
   }
-  __device__ __forceinline__ static int swizzle_col(int k) { return (k & 3) * 4; }   // in vectors of 16 bytes
+  // in vectors of 16 bytes: four k-rows of a transposing read go to different banks
+  __device__ __forceinline__ static int swizzle_col(int k) { return EXT >= 128 ? (k & 3) * 4 : EXT >= 64 ? (k & 1) * 4 : 0; }
   __device__ __forceinline__ void fetch(uint32_t lds) const {
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x & ~63u) * 16u);   // the wave's first vector
 #pragma unroll
-    for (int j = 0; j < LOADS; j++) load_to_lds(to + (uint32_t)j * 4096u, base, off[j]);
+    for (int j = 0; j < LOADS; j++) load_to_lds(to + (uint32_t)(j * THREADS * 16), base, off[j]);
   }
   // the last, partial stage: `left` of the contraction, zeros behind
   __device__ __forceinline__ void fetch_tail(char *lds, int left) const {
@@ -288,7 +308,7 @@ template <bool COL, int EXT> struct Panel {
       place(j, outer, k);
       u32x4 v = {0u, 0u, 0u, 0u};
       if (k < left) v = *(const u32x4 *)(base + off[j]);
-      *(u32x4 *)(lds + (j * 256 + (int)threadIdx.x) * 16) = v;
+      *(u32x4 *)(lds + (j * THREADS + (int)threadIdx.x) * 16) = v;
     }
   }
   // matrix operand of 32 entries from `at`, 16 of k from kk: lane l has entry l % 32, k = kk + (l / 32) * 8 + 0..7
@@ -310,7 +330,7 @@ template <bool COL, int EXT> struct Panel {
       return r;
     } else {
       const int row = at + (lane & 31), c = (kk >> 3) + (lane >> 5);
-      return *(const u32x4 *)(lds + row * (FK * 2) + ((c ^ ((row >> 1) & 3)) * 16));
+      return *(const u32x4 *)(lds + row * (FK * 2) + ((c ^ (row & 7)) * 16));
     }
   }
 };
@@ -322,117 +342,206 @@ template <int DT> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// acc[i][j]: entries wa + 32 i of A (its columns) and wb + 32 j of B (its rows): a lane holds 4 neighbours along B
-template <int DT, bool A_COL, bool B_COL>
-__device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, FM> &a, Panel<B_COL, FN> &b, int full, int left, f32x16 (&acc)[2][4]) {
-  constexpr int LOADS = Panel<A_COL, FM>::LOADS + Panel<B_COL, FN>::LOADS;
-  const int wave = threadIdx.x >> 6, wa = (wave >> 1) * 64, wb = (wave & 1) * 128;
+// acc[i][j]: entries wa + 32 i of A (its columns) and wb + 32 j of B (its rows): a lane holds 4 neighbours along B.
+// idle: this wave's part of the tile has no rows (it still loads and waits with the others).
+template <int DT, class S, bool A_COL, bool B_COL>
+__device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::THREADS> &a, Panel<B_COL, S::BN, S::THREADS> &b, int full,
+                                             int left, bool idle, int wa, int wb, int wk, f32x16 (&acc)[S::TM][S::TN]) {
+  using PA = Panel<A_COL, S::BM, S::THREADS>;
+  using PB = Panel<B_COL, S::BN, S::THREADS>;
+  constexpr int AHEAD = S::STAGES - 1, LOADS = PA::LOADS + PB::LOADS;
   const uint32_t lds0 = lds_address(smem);
   const int stages = full + (left ? 1 : 0);
+  int put = 0;
   auto fetch = [&](int t) {
-    const int at = (t % STAGES) * STAGE_BYTES;
+    const int at = put * S::STAGE;
+    put = put + 1 == S::STAGES ? 0 : put + 1;
     if (t < full) {
       a.fetch(lds0 + at);
-      b.fetch(lds0 + at + A_BYTES);
+      b.fetch(lds0 + at + S::A_BYTES);
     } else if (t < stages) {
       a.fetch_tail(smem + at, left);
-      b.fetch_tail(smem + at + A_BYTES, left);
+      b.fetch_tail(smem + at + S::A_BYTES, left);
     }
     a.base += a.step;
     b.base += b.step;
   };
-  fetch(0);
-  fetch(1);
-  for (int t = 0; t < stages; t++) {
-    if (t + 1 < full) wait_loads<LOADS>();   // stage t + 1 may still be on its way
+  // Stage t is here once all loads but those of the stages behind it have arrived, for every wave.
+  auto arrive = [&](int t) {
+    if (t + AHEAD - 1 < full) wait_loads<(AHEAD - 1) * LOADS>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
-    fetch(t + 2);                            // into the stage that everybody has read
-    const char *sa = smem + (t % STAGES) * STAGE_BYTES, *sb = sa + A_BYTES;
+  };
+  constexpr int STEPS = 4 / S::WK;
+  u32x4 av[2][S::TM], bv[2][S::TN];
+  int get = 0;
+  auto read = [&](int set, int step) {
+    if (idle) return;
+    const char *sa = smem + get * S::STAGE, *sb = sa + S::A_BYTES;
+    const int kk = (step * S::WK + wk) * 16;
 #pragma unroll
-    for (int kk = 0; kk < FK; kk += 16) {
-      u32x4 av[2], bv[4];
+    for (int j = 0; j < S::TN; j++) bv[set][j] = PB::fragment(sb, wb + j * 32, kk);
 #pragma unroll
-      for (int i = 0; i < 2; i++) av[i] = Panel<A_COL, FM>::fragment(sa, wa + i * 32, kk);
+    for (int i = 0; i < S::TM; i++) av[set][i] = PA::fragment(sa, wa + i * 32, kk);
+  };
 #pragma unroll
-      for (int j = 0; j < 4; j++) bv[j] = Panel<B_COL, FN>::fragment(sb, wb + j * 32, kk);
+  for (int t = 0; t < AHEAD; t++) fetch(t);
+  arrive(0);
+  read(0, 0);
+  fetch(AHEAD);
+  for (int t = 0; t < stages; t++) {
+    // The fragments of the next step are read while the current one's are multiplied; the step that ends a stage waits for
+    // the next stage first, so the barrier and the first reads of a stage hide behind matrix instructions too.
 #pragma unroll
-      for (int i = 0; i < 2; i++)
+    for (int step = 0; step < STEPS; step++) {
+      constexpr int ODD = STEPS & 1;
+      const int set = ODD ? 0 : step & 1, next = set ^ 1;
+      if (step + 1 < STEPS) {
+        read(next, step + 1);
+      } else if (t + 1 < stages) {
+        arrive(t + 1);
+        get = get + 1 == S::STAGES ? 0 : get + 1;
+        read(next, 0);
+        fetch(t + 1 + AHEAD);
+      }
+      if (!idle) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = mfma16<DT>(bv[j], av[i], acc[i][j]);
+        for (int i = 0; i < S::TM; i++)
+#pragma unroll
+          for (int j = 0; j < S::TN; j++) acc[i][j] = mfma16<DT>(bv[set][j], av[set][i], acc[i][j]);
+      }
+      if (ODD) {
+#pragma unroll
+        for (int i = 0; i < S::TM; i++) av[0][i] = av[1][i];
+#pragma unroll
+        for (int j = 0; j < S::TN; j++) bv[0][j] = bv[1][j];
+      }
     }
   }
   wait_loads<0>();
   __builtin_amdgcn_s_barrier();   // the stages are free
+  if constexpr (S::WK > 1) {      // waves that took other k-steps hand their sums over, in order
+    float *join = (float *)smem;
+    const int lane = threadIdx.x & 63;
+    if (wk > 0) {
+#pragma unroll
+      for (int i = 0; i < S::TM; i++)
+#pragma unroll
+        for (int j = 0; j < S::TN; j++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) join[((((wk - 1) * S::TM + i) * S::TN + j) * 16 + e) * 64 + lane] = acc[i][j][e];
+    }
+    __syncthreads();
+    if (wk == 0) {
+#pragma unroll
+      for (int w = 0; w < S::WK - 1; w++)
+#pragma unroll
+        for (int i = 0; i < S::TM; i++)
+#pragma unroll
+          for (int j = 0; j < S::TN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] += join[(((w * S::TM + i) * S::TN + j) * 16 + e) * 64 + lane];
+    }
+    __syncthreads();
+  }
 }
 
-// The tile through LDS to memory in rows of 512 bytes; rows < rlim, columns < clim (a multiple of 8).
-template <int DT> __device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, const f32x16 (&acc)[2][4]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave >> 1) * 64, wb = (wave & 1) * 128;
+// The tile through LDS to memory in whole rows; rows < rlim, columns < clim (a multiple of 8).
+template <int DT, class S>
+__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, int wa, int wb, int wk,
+                                           const f32x16 (&acc)[S::TM][S::TN]) {
+  const int lane = threadIdx.x & 63;
   uint16_t *t = (uint16_t *)smem;
+  if (wk == 0) {
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+    for (int i = 0; i < S::TM; i++)
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+      for (int j = 0; j < S::TN; j++)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int row = wa + i * 32 + (lane & 31), col = wb + j * 32 + (e / 4) * 8 + (lane >> 5) * 4;
-        const uint2 v = {pack_pair16<DT>(acc[i][j][e], acc[i][j][e + 1]), pack_pair16<DT>(acc[i][j][e + 2], acc[i][j][e + 3])};
-        *(uint2 *)(t + row * OUT_LD + col) = v;
-      }
+        for (int e = 0; e < 16; e += 4) {
+          const int row = wa + i * 32 + (lane & 31), col = wb + j * 32 + (e / 4) * 8 + (lane >> 5) * 4;
+          const uint2 v = {pack_pair16<DT>(acc[i][j][e], acc[i][j][e + 1]), pack_pair16<DT>(acc[i][j][e + 2], acc[i][j][e + 3])};
+          *(uint2 *)(t + row * S::OUT_LD + col) = v;
+        }
+  }
   __syncthreads();
-  const int col = (threadIdx.x & 31) * 8;
+  constexpr int PER = S::BN / 8;
+  const int col = (threadIdx.x % PER) * 8;
   if (col < clim)
-    for (int row = threadIdx.x >> 5; row < FM && row < rlim; row += 8)
-      *(u32x4 *)(c + row * ldc + col) = *(const u32x4 *)(t + row * OUT_LD + col);
+    for (int row = threadIdx.x / PER; row < rlim; row += S::THREADS / PER)
+      *(u32x4 *)(c + row * ldc + col) = *(const u32x4 *)(t + row * S::OUT_LD + col);
 }
 
-// Tiles of one XCD follow each other: neighbours share rows of x and a group's weights in its L2.  grid: a multiple of 8.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t b) { return (b & 7u) * (gridDim.x >> 3) + (b >> 3); }
+// Workgroup b runs on XCD b % 8: each XCD gets an eighth of the tiles, one after the other, so that neighbours share rows of
+// x and a group's weights in its L2.
+constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t tiles) {
+  const uint32_t share = (tiles + 7u) / 8u, at = b >> 3;
+  const uint32_t id = (b & 7u) * share + at;
+  return at < share && id < tiles ? id : NO_TILE;
+}
 
-template <int DT, bool W_TRANS>
-__global__ __launch_bounds__(256, 2) void grouped_fast_kernel(uint16_t *y, const uint16_t *x, const uint16_t *w, const int32_t *offsets,
-                                                              int64_t M, int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
-  __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE_BYTES];
-  const uint32_t id = xcd_order(blockIdx.x);
-  const RowTile r = find_rows<FM>(offsets, groups, M, id / col_tiles);
-  if (r.group == -2) return;
-  const int64_t first = __builtin_amdgcn_readfirstlane((int)r.first), c0 = (int64_t)(id % col_tiles) * FN;
+template <class S> struct WaveAt {   // a wave's part of the tile; waves that share a SIMD (w, w + 4) differ in their rows
+  int wa, wb, wk;
+  __device__ __forceinline__ WaveAt() {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    wb = (wave % S::WN) * (S::BN / S::WN);
+    wa = (wave / S::WN % S::WM) * (S::BM / S::WM);
+    wk = wave / (S::WN * S::WM);
+  }
+};
+
+template <int DT, bool W_TRANS, class S>
+__global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, const uint16_t *x, const uint16_t *w, const int32_t *offsets,
+                                                                  int64_t M, int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
+  __shared__ __attribute__((aligned(16))) char smem[S::LDS];
+  const TileMap<S::BM> map(offsets, groups, M);
+  const uint32_t id = xcd_tile(blockIdx.x, map.tiles() * col_tiles);
+  if (id == NO_TILE) return;
+  const RowTile r = map.find(id / col_tiles);
+  const int64_t first = __builtin_amdgcn_readfirstlane((int)r.first), c0 = (int64_t)(id % col_tiles) * S::BN;
   const int group = __builtin_amdgcn_readfirstlane(r.group), rows = __builtin_amdgcn_readfirstlane((int)(r.end - r.first));
-  const int cols = (int)(N - c0 < FN ? N - c0 : FN);
-  f32x16 acc[2][4] = {};
+  const int cols = (int)(N - c0 < S::BN ? N - c0 : S::BN);
+  const WaveAt<S> at;
+  f32x16 acc[S::TM][S::TN] = {};
   if (group >= 0) {
     const uint16_t *wg = w + (int64_t)group * K * N;
-    Panel<false, FM> a;
-    Panel<!W_TRANS, FN> b;
+    Panel<false, S::BM, S::THREADS> a;
+    Panel<!W_TRANS, S::BN, S::THREADS> b;
     a.set(x + first * K, K, rows);
     b.set(W_TRANS ? wg + c0 * K : wg + c0, W_TRANS ? K : N, cols);
-    fast_product<DT, false, !W_TRANS>(smem, a, b, (int)(K / FK), (int)(K % FK), acc);
+    fast_product<DT, S, false, !W_TRANS>(smem, a, b, (int)(K / FK), (int)(K % FK), at.wa >= rows || at.wb >= cols, at.wa, at.wb, at.wk, acc);
   }
-  fast_store<DT>(smem, y + first * N + c0, N, rows, cols, acc);
+  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, at.wa, at.wb, at.wk, acc);
 }
 
-template <int DT>
-__global__ __launch_bounds__(256, 2) void grouped_wgrad_fast_kernel(uint16_t *dw, const uint16_t *a, const uint16_t *b, const int32_t *offsets,
-                                                                    int64_t M, int64_t P, int64_t Q, uint32_t ptiles, uint32_t qtiles,
-                                                                    uint32_t tiles) {
-  __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE_BYTES];
-  const uint32_t id = xcd_order(blockIdx.x);
-  if (id >= tiles) return;
+template <int DT, class S>
+__global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t *dw, const uint16_t *a, const uint16_t *b,
+                                                                        const int32_t *offsets, int64_t M, int64_t P, int64_t Q,
+                                                                        uint32_t ptiles, uint32_t qtiles, uint32_t tiles) {
+  __shared__ __attribute__((aligned(16))) char smem[S::LDS];
+  const uint32_t id = xcd_tile(blockIdx.x, tiles);
+  if (id == NO_TILE) return;
   const uint32_t g = id / (ptiles * qtiles), t = id % (ptiles * qtiles);
-  const int64_t p0 = (int64_t)(t / qtiles) * FM, q0 = (int64_t)(t % qtiles) * FN;
+  const int64_t p0 = (int64_t)(t / qtiles) * S::BM, q0 = (int64_t)(t % qtiles) * S::BN;
   const int64_t lo = row_at(offsets, g, M), hi = row_at(offsets, (int64_t)g + 1, M);
-  const int plim = (int)(P - p0 < FM ? P - p0 : FM), qlim = (int)(Q - q0 < FN ? Q - q0 : FN);
-  f32x16 acc[2][4] = {};
+  const int plim = (int)(P - p0 < S::BM ? P - p0 : S::BM), qlim = (int)(Q - q0 < S::BN ? Q - q0 : S::BN);
+  const WaveAt<S> at;
+  f32x16 acc[S::TM][S::TN] = {};
   if (hi > lo) {
-    Panel<true, FM> pa;
-    Panel<true, FN> pb;
+    Panel<true, S::BM, S::THREADS> pa;
+    Panel<true, S::BN, S::THREADS> pb;
     pa.set(a + lo * P + p0, P, plim);
     pb.set(b + lo * Q + q0, Q, qlim);
-    fast_product<DT, true, true>(smem, pa, pb, (int)((hi - lo) / FK), (int)((hi - lo) % FK), acc);
+    fast_product<DT, S, true, true>(smem, pa, pb, (int)((hi - lo) / FK), (int)((hi - lo) % FK), at.wa >= plim || at.wb >= qlim, at.wa, at.wb,
+                                    at.wk, acc);
   }
-  fast_store<DT>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, acc);
+  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, at.wa, at.wb, at.wk, acc);
 }
+
+using Large = Shape<256, 256, 2, 4, 1, 2>;
+using Medium = Shape<128, 128, 2, 2, 1, 2>;
+using Small = Shape<32, 64, 1, 1, 4, 4>;
 
 // Whole 16-byte vectors everywhere, and offsets within a tile that fit 32 bits.
 bool fast_rows(const void *p, int64_t ld) { return (uintptr_t)p % 16u == 0 && ld % 8 == 0 && ld <= 1 << 21; }
@@ -477,16 +586,22 @@ extern "C" int fpemu_grouped_gemm(void *y, const void *x, const void *w, const i
   if (rows * cols > 0x7FFFFFFFll) return fail(FPEMU_EINVAL, who, "too many tiles for one launch");
   hipStream_t s = (hipStream_t)stream;
   if (dtype != FPEMU_F32 && K > 0 && fast_rows(y, N) && fast_rows(x, K) && fast_rows(w, N)) {
-    const int64_t ct = ceil_div(N, FN), rt = ceil_div(M, FM) + groups + 2;
-    if (rt * ct < 0x7FFFFFF0ll) {
+    static const char *force = getenv("FPEMU_GROUPED_SHAPE");
+    auto shape = [&](auto tag) {
+      using S = decltype(tag);
+      const int64_t ct = ceil_div(N, S::BN), rt = ceil_div(M, S::BM) + groups + 2;
+      if (rt * ct > 0x7FFFFFF0ll) return false;
       const unsigned blocks = (unsigned)(ceil_div(rt * ct, 8) * 8);
       auto go = [&](auto kernel) {
-        kernel<<<blocks, 256, 0, s>>>((uint16_t *)y, (const uint16_t *)x, (const uint16_t *)w, offsets, M, N, K, groups, (uint32_t)ct);
+        kernel<<<blocks, S::THREADS, 0, s>>>((uint16_t *)y, (const uint16_t *)x, (const uint16_t *)w, offsets, M, N, K, groups, (uint32_t)ct);
       };
-      if (dtype == FPEMU_F16) w_trans ? go(grouped_fast_kernel<FPEMU_F16, true>) : go(grouped_fast_kernel<FPEMU_F16, false>);
-      else w_trans ? go(grouped_fast_kernel<FPEMU_BF16, true>) : go(grouped_fast_kernel<FPEMU_BF16, false>);
-      return launched(who);
-    }
+      if (dtype == FPEMU_F16) w_trans ? go(grouped_fast_kernel<FPEMU_F16, true, S>) : go(grouped_fast_kernel<FPEMU_F16, false, S>);
+      else w_trans ? go(grouped_fast_kernel<FPEMU_BF16, true, S>) : go(grouped_fast_kernel<FPEMU_BF16, false, S>);
+      return true;
+    };
+    const int f = force ? atoi(force) : -1;
+    const bool done = f == 0 ? shape(Large()) : f == 1 ? shape(Medium()) : f == 2 ? shape(Small()) : M >= 512 * groups ? shape(Large()) : M >= 48 * groups ? shape(Medium()) : shape(Small());
+    if (done) return launched(who);
   }
   const unsigned blocks = (unsigned)(rows * cols);
   if (dtype == FPEMU_F32) run_grouped<FPEMU_F32>(y, x, w, offsets, M, N, K, groups, w_trans, blocks, (uint32_t)cols, s);
@@ -505,14 +620,21 @@ extern "C" int fpemu_grouped_gemm_wgrad(void *dw, const void *a, const void *b, 
   if (pt * qt > 0x7FFFFFFFll / groups) return fail(FPEMU_EINVAL, who, "too many tiles for one launch");
   hipStream_t s = (hipStream_t)stream;
   if (dtype != FPEMU_F32 && M > 0 && fast_rows(dw, Q) && fast_rows(a, P) && fast_rows(b, Q)) {
-    const int64_t pf = ceil_div(P, FM), qf = ceil_div(Q, FN), tiles = pf * qf * groups;   // no more than the ones above
-    const unsigned blocks = (unsigned)(ceil_div(tiles, 8) * 8);
-    auto go = [&](auto kernel) {
-      kernel<<<blocks, 256, 0, s>>>((uint16_t *)dw, (const uint16_t *)a, (const uint16_t *)b, offsets, M, P, Q, (uint32_t)pf, (uint32_t)qf,
-                                    (uint32_t)tiles);
+    static const char *force = getenv("FPEMU_GROUPED_SHAPE");
+    auto shape = [&](auto tag) {
+      using S = decltype(tag);
+      const int64_t pf = ceil_div(P, S::BM), qf = ceil_div(Q, S::BN), tiles = pf * qf * groups;   // no more than the ones above
+      const unsigned blocks = (unsigned)(ceil_div(tiles, 8) * 8);
+      auto go = [&](auto kernel) {
+        kernel<<<blocks, S::THREADS, 0, s>>>((uint16_t *)dw, (const uint16_t *)a, (const uint16_t *)b, offsets, M, P, Q, (uint32_t)pf,
+                                             (uint32_t)qf, (uint32_t)tiles);
+      };
+      if (dtype == FPEMU_F16) go(grouped_wgrad_fast_kernel<FPEMU_F16, S>);
+      else go(grouped_wgrad_fast_kernel<FPEMU_BF16, S>);
     };
-    if (dtype == FPEMU_F16) go(grouped_wgrad_fast_kernel<FPEMU_F16>);
-    else go(grouped_wgrad_fast_kernel<FPEMU_BF16>);
+    const int f = force ? atoi(force) : -1;
+    if (f == 0) shape(Large());
+    else shape(Medium());
     return launched(who);
   }
   const unsigned blocks = (unsigned)(pt * qt * groups);
