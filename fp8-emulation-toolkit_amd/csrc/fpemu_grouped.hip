@@ -235,7 +235,7 @@ __global__ __launch_bounds__(256) void grouped_wgrad_any_kernel(typename Storage
 // contraction is its slow dimension lies as it is in memory and is read through the transposing LDS read (of 16 lanes, lane
 // i gets column i of 4 k-rows).  The loads write LDS linearly, so the bank swizzle is applied to the global address a lane
 // fetches and undone where the fragment is read.
-// Waves: WM x WN over the tile, WK over the four 16-deep steps of a stage (their sums are joined at the end).
+// Waves: WM x WN over the tile.
 constexpr int FK = 64;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -251,14 +251,13 @@ template <int N> __device__ __forceinline__ void wait_loads() {   // all but the
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int WK_, int STAGES_> struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WK = WK_, STAGES = STAGES_;
-  static constexpr int THREADS = WM * WN * WK * 64;
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_> struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
+  static constexpr int THREADS = WM * WN * 64;
   static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;   // matrix tiles of a wave
   static constexpr int A_BYTES = BM * FK * 2, B_BYTES = BN * FK * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int OUT_LD = BN + 8;   // elements; the finished tile goes through LDS to be stored in whole rows
-  static constexpr int JOIN = (WK - 1) * BM * BN * 4, OUT = BM * OUT_LD * 2;
-  static constexpr int LDS = STAGES * STAGE > OUT ? (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN) : (OUT > JOIN ? OUT : JOIN);
+  static constexpr int OUT = BM * OUT_LD * 2, LDS = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
 };
 
 // One operand's tile: EXT entries (rows of a row operand, columns of a COL operand) x FK of the contraction.
@@ -290,10 +289,12 @@ template <bool COL, int EXT, int THREADS> struct Panel {
       outer = ((id % PER) ^ swizzle_col(k)) * 8;
     } else {
       outer = id / 8;
-      k = ((id & 7) ^ (outer & 7)) * 8;
+      k = ((id & 7) ^ swizzle_row(outer)) * 8;
     }
   }
-  // in vectors of 16 bytes: four k-rows of a transposing read go to different banks
+  // in vectors of 16 bytes: 16 rows that are read together lie in 16 different places of 256 bytes
+  __device__ __forceinline__ static int swizzle_row(int row) { return (row >> 1) & 7; }
+  // four k-rows of a transposing read go to different banks
   __device__ __forceinline__ static int swizzle_col(int k) { return EXT >= 128 ? (k & 3) * 4 : EXT >= 64 ? (k & 1) * 4 : 0; }
   __device__ __forceinline__ void fetch(uint32_t lds) const {
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x & ~63u) * 16u);   // the wave's first vector
@@ -311,17 +312,28 @@ template <bool COL, int EXT, int THREADS> struct Panel {
       *(u32x4 *)(lds + (j * THREADS + (int)threadIdx.x) * 16) = v;
     }
   }
-  // matrix operand of 32 entries from `at`, 16 of k from kk: lane l has entry l % 32, k = kk + (l / 32) * 8 + 0..7
-  __device__ __forceinline__ static u32x4 fragment(const char *lds, int at, int kk) {
+  // Where a lane finds its fragments in the tile: a matrix operand of 32 entries, 16 of k: lane l has entry l % 32,
+  // k = (l / 32) * 8 + 0..7.  The places for the four k-steps of a stage are kept; further entries are a constant away.
+  uint32_t frag[COL ? 1 : 4];
+  __device__ __forceinline__ void set_fragments(int at) {
     const int lane = threadIdx.x & 63;
     if constexpr (COL) {
-      const int i = lane & 15, g = lane >> 4;
-      const int col = at + (g & 1) * 16 + (i & 3) * 4;
+      const int i = lane & 15, g = lane >> 4, k = (g >> 1) * 8 + (i >> 2), col = at + (g & 1) * 16 + (i & 3) * 4;
+      frag[0] = (uint32_t)(k * (EXT * 2) + (((col >> 3) ^ swizzle_col(k)) * 16) + (col & 7) * 2);
+    } else {
+      const int row = at + (lane & 31);
+#pragma unroll
+      for (int s = 0; s < 4; s++) frag[s] = (uint32_t)(row * (FK * 2) + (((s * 2 + (lane >> 5)) ^ swizzle_row(row)) * 16));
+    }
+  }
+  // the operand `tile` tiles of 32 entries further on, k-step `step` (both known at compile time), of the stage at `lds`
+  __device__ __forceinline__ u32x4 fragment(const char *lds, int tile, int step) const {
+    if constexpr (COL) {
       u32x4 r;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int k = kk + (g >> 1) * 8 + h * 4 + (i >> 2);
-        const int where = k * (EXT * 2) + (((col >> 3) ^ swizzle_col(k)) * 16) + (col & 7) * 2;
+        // entries 32 further on are 4 vectors away: an exclusive or where the swizzle may touch the same bits
+        const uint32_t where = (frag[0] ^ (uint32_t)(tile * 64)) + (uint32_t)((step * 16 + h * 4) * (EXT * 2));
         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds + where));
         const uint2 w = __builtin_bit_cast(uint2, v);
         r[2 * h] = w.x;
@@ -329,8 +341,7 @@ template <bool COL, int EXT, int THREADS> struct Panel {
       }
       return r;
     } else {
-      const int row = at + (lane & 31), c = (kk >> 3) + (lane >> 5);
-      return *(const u32x4 *)(lds + row * (FK * 2) + ((c ^ (row & 7)) * 16));
+      return *(const u32x4 *)(lds + frag[step] + (uint32_t)(tile * 32 * FK * 2));
     }
   }
 };
@@ -346,7 +357,7 @@ template <int DT> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32
 // idle: this wave's part of the tile has no rows (it still loads and waits with the others).
 template <int DT, class S, bool A_COL, bool B_COL>
 __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::THREADS> &a, Panel<B_COL, S::BN, S::THREADS> &b, int full,
-                                             int left, bool idle, int wa, int wb, int wk, f32x16 (&acc)[S::TM][S::TN]) {
+                                             int left, bool idle, f32x16 (&acc)[S::TM][S::TN]) {
   using PA = Panel<A_COL, S::BM, S::THREADS>;
   using PB = Panel<B_COL, S::BN, S::THREADS>;
   constexpr int AHEAD = S::STAGES - 1, LOADS = PA::LOADS + PB::LOADS;
@@ -372,17 +383,16 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
   };
-  constexpr int STEPS = 4 / S::WK;
+  constexpr int STEPS = FK / 16;
   u32x4 av[2][S::TM], bv[2][S::TN];
   int get = 0;
   auto read = [&](int set, int step) {
     if (idle) return;
     const char *sa = smem + get * S::STAGE, *sb = sa + S::A_BYTES;
-    const int kk = (step * S::WK + wk) * 16;
 #pragma unroll
-    for (int j = 0; j < S::TN; j++) bv[set][j] = PB::fragment(sb, wb + j * 32, kk);
+    for (int j = 0; j < S::TN; j++) bv[set][j] = b.fragment(sb, j, step);
 #pragma unroll
-    for (int i = 0; i < S::TM; i++) av[set][i] = PA::fragment(sa, wa + i * 32, kk);
+    for (int i = 0; i < S::TM; i++) av[set][i] = a.fragment(sa, i, step);
   };
 #pragma unroll
   for (int t = 0; t < AHEAD; t++) fetch(t);
@@ -394,8 +404,7 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
     // the next stage first, so the barrier and the first reads of a stage hide behind matrix instructions too.
 #pragma unroll
     for (int step = 0; step < STEPS; step++) {
-      constexpr int ODD = STEPS & 1;
-      const int set = ODD ? 0 : step & 1, next = set ^ 1;
+      const int set = step & 1, next = set ^ 1;
       if (step + 1 < STEPS) {
         read(next, step + 1);
       } else if (t + 1 < stages) {
@@ -410,60 +419,28 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
 #pragma unroll
           for (int j = 0; j < S::TN; j++) acc[i][j] = mfma16<DT>(bv[set][j], av[set][i], acc[i][j]);
       }
-      if (ODD) {
-#pragma unroll
-        for (int i = 0; i < S::TM; i++) av[0][i] = av[1][i];
-#pragma unroll
-        for (int j = 0; j < S::TN; j++) bv[0][j] = bv[1][j];
-      }
     }
   }
   wait_loads<0>();
   __builtin_amdgcn_s_barrier();   // the stages are free
-  if constexpr (S::WK > 1) {      // waves that took other k-steps hand their sums over, in order
-    float *join = (float *)smem;
-    const int lane = threadIdx.x & 63;
-    if (wk > 0) {
-#pragma unroll
-      for (int i = 0; i < S::TM; i++)
-#pragma unroll
-        for (int j = 0; j < S::TN; j++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) join[((((wk - 1) * S::TM + i) * S::TN + j) * 16 + e) * 64 + lane] = acc[i][j][e];
-    }
-    __syncthreads();
-    if (wk == 0) {
-#pragma unroll
-      for (int w = 0; w < S::WK - 1; w++)
-#pragma unroll
-        for (int i = 0; i < S::TM; i++)
-#pragma unroll
-          for (int j = 0; j < S::TN; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] += join[(((w * S::TM + i) * S::TN + j) * 16 + e) * 64 + lane];
-    }
-    __syncthreads();
-  }
 }
 
 // The tile through LDS to memory in whole rows; rows < rlim, columns < clim (a multiple of 8).
 template <int DT, class S>
-__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, int wa, int wb, int wk,
+__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, int wa, int wb,
                                            const f32x16 (&acc)[S::TM][S::TN]) {
   const int lane = threadIdx.x & 63;
   uint16_t *t = (uint16_t *)smem;
-  if (wk == 0) {
 #pragma unroll
-    for (int i = 0; i < S::TM; i++)
+  for (int i = 0; i < S::TM; i++)
 #pragma unroll
-      for (int j = 0; j < S::TN; j++)
+    for (int j = 0; j < S::TN; j++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int row = wa + i * 32 + (lane & 31), col = wb + j * 32 + (e / 4) * 8 + (lane >> 5) * 4;
-          const uint2 v = {pack_pair16<DT>(acc[i][j][e], acc[i][j][e + 1]), pack_pair16<DT>(acc[i][j][e + 2], acc[i][j][e + 3])};
-          *(uint2 *)(t + row * S::OUT_LD + col) = v;
-        }
-  }
+      for (int e = 0; e < 16; e += 4) {
+        const int row = wa + i * 32 + (lane & 31), col = wb + j * 32 + (e / 4) * 8 + (lane >> 5) * 4;
+        const uint2 v = {pack_pair16<DT>(acc[i][j][e], acc[i][j][e + 1]), pack_pair16<DT>(acc[i][j][e + 2], acc[i][j][e + 3])};
+        *(uint2 *)(t + row * S::OUT_LD + col) = v;
+      }
   __syncthreads();
   constexpr int PER = S::BN / 8;
   const int col = (threadIdx.x % PER) * 8;
@@ -481,13 +458,21 @@ __device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t tiles) {
   return at < share && id < tiles ? id : NO_TILE;
 }
 
+// Row and column tile of number id: bands of four row tiles, down the band first, so that the tiles an XCD works on at one
+// time are about as high as wide and share what they read.
+__device__ __forceinline__ void banded(uint32_t id, uint32_t row_tiles, uint32_t col_tiles, uint32_t &row, uint32_t &col) {
+  const uint32_t band = id / (4u * col_tiles), in = id - band * 4u * col_tiles;
+  const uint32_t high = row_tiles - band * 4u < 4u ? row_tiles - band * 4u : 4u;
+  row = band * 4u + in % high;
+  col = in / high;
+}
+
 template <class S> struct WaveAt {   // a wave's part of the tile; waves that share a SIMD (w, w + 4) differ in their rows
-  int wa, wb, wk;
+  int wa, wb;
   __device__ __forceinline__ WaveAt() {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     wb = (wave % S::WN) * (S::BN / S::WN);
-    wa = (wave / S::WN % S::WM) * (S::BM / S::WM);
-    wk = wave / (S::WN * S::WM);
+    wa = (wave / S::WN) * (S::BM / S::WM);
   }
 };
 
@@ -498,8 +483,10 @@ __global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, c
   const TileMap<S::BM> map(offsets, groups, M);
   const uint32_t id = xcd_tile(blockIdx.x, map.tiles() * col_tiles);
   if (id == NO_TILE) return;
-  const RowTile r = map.find(id / col_tiles);
-  const int64_t first = __builtin_amdgcn_readfirstlane((int)r.first), c0 = (int64_t)(id % col_tiles) * S::BN;
+  uint32_t row_tile, col_tile;
+  banded(id, map.tiles(), col_tiles, row_tile, col_tile);
+  const RowTile r = map.find(row_tile);
+  const int64_t first = __builtin_amdgcn_readfirstlane((int)r.first), c0 = (int64_t)col_tile * S::BN;
   const int group = __builtin_amdgcn_readfirstlane(r.group), rows = __builtin_amdgcn_readfirstlane((int)(r.end - r.first));
   const int cols = (int)(N - c0 < S::BN ? N - c0 : S::BN);
   const WaveAt<S> at;
@@ -510,9 +497,11 @@ __global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, c
     Panel<!W_TRANS, S::BN, S::THREADS> b;
     a.set(x + first * K, K, rows);
     b.set(W_TRANS ? wg + c0 * K : wg + c0, W_TRANS ? K : N, cols);
-    fast_product<DT, S, false, !W_TRANS>(smem, a, b, (int)(K / FK), (int)(K % FK), at.wa >= rows || at.wb >= cols, at.wa, at.wb, at.wk, acc);
+    a.set_fragments(at.wa);
+    b.set_fragments(at.wb);
+    fast_product<DT, S, false, !W_TRANS>(smem, a, b, (int)(K / FK), (int)(K % FK), at.wa >= rows || at.wb >= cols, acc);
   }
-  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, at.wa, at.wb, at.wk, acc);
+  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, at.wa, at.wb, acc);
 }
 
 template <int DT, class S>
@@ -522,8 +511,10 @@ __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t
   __shared__ __attribute__((aligned(16))) char smem[S::LDS];
   const uint32_t id = xcd_tile(blockIdx.x, tiles);
   if (id == NO_TILE) return;
-  const uint32_t g = id / (ptiles * qtiles), t = id % (ptiles * qtiles);
-  const int64_t p0 = (int64_t)(t / qtiles) * S::BM, q0 = (int64_t)(t % qtiles) * S::BN;
+  const uint32_t g = id / (ptiles * qtiles);
+  uint32_t pt, qt;
+  banded(id % (ptiles * qtiles), ptiles, qtiles, pt, qt);
+  const int64_t p0 = (int64_t)pt * S::BM, q0 = (int64_t)qt * S::BN;
   const int64_t lo = row_at(offsets, g, M), hi = row_at(offsets, (int64_t)g + 1, M);
   const int plim = (int)(P - p0 < S::BM ? P - p0 : S::BM), qlim = (int)(Q - q0 < S::BN ? Q - q0 : S::BN);
   const WaveAt<S> at;
@@ -533,15 +524,15 @@ __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t
     Panel<true, S::BN, S::THREADS> pb;
     pa.set(a + lo * P + p0, P, plim);
     pb.set(b + lo * Q + q0, Q, qlim);
-    fast_product<DT, S, true, true>(smem, pa, pb, (int)((hi - lo) / FK), (int)((hi - lo) % FK), at.wa >= plim || at.wb >= qlim, at.wa, at.wb,
-                                    at.wk, acc);
+    pa.set_fragments(at.wa);
+    pb.set_fragments(at.wb);
+    fast_product<DT, S, true, true>(smem, pa, pb, (int)((hi - lo) / FK), (int)((hi - lo) % FK), at.wa >= plim || at.wb >= qlim, acc);
   }
-  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, at.wa, at.wb, at.wk, acc);
+  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, at.wa, at.wb, acc);
 }
 
-using Large = Shape<256, 256, 2, 4, 1, 2>;
-using Medium = Shape<128, 128, 2, 2, 1, 2>;
-using Small = Shape<32, 64, 1, 1, 4, 4>;
+using Large = Shape<256, 256, 2, 4, 2>;
+using Medium = Shape<128, 128, 2, 2, 2>;
 
 // Whole 16-byte vectors everywhere, and offsets within a tile that fit 32 bits.
 bool fast_rows(const void *p, int64_t ld) { return (uintptr_t)p % 16u == 0 && ld % 8 == 0 && ld <= 1 << 21; }
@@ -600,7 +591,7 @@ extern "C" int fpemu_grouped_gemm(void *y, const void *x, const void *w, const i
       return true;
     };
     const int f = force ? atoi(force) : -1;
-    const bool done = f == 0 ? shape(Large()) : f == 1 ? shape(Medium()) : f == 2 ? shape(Small()) : M >= 512 * groups ? shape(Large()) : M >= 48 * groups ? shape(Medium()) : shape(Small());
+    const bool done = f == 0 ? shape(Large()) : f == 1 ? shape(Medium()) : M >= 512 * groups ? shape(Large()) : shape(Medium());
     if (done) return launched(who);
   }
   const unsigned blocks = (unsigned)(rows * cols);
