@@ -296,10 +296,8 @@ template <bool COL, int EXT, int THREADS> struct Panel {
   __device__ __forceinline__ static int swizzle_row(int row) { return (row >> 1) & 7; }
   // four k-rows of a transposing read go to different banks
   __device__ __forceinline__ static int swizzle_col(int k) { return EXT >= 128 ? (k & 3) * 4 : EXT >= 64 ? (k & 1) * 4 : 0; }
-  __device__ __forceinline__ void fetch(uint32_t lds) const {
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x & ~63u) * 16u);   // the wave's first vector
-#pragma unroll
-    for (int j = 0; j < LOADS; j++) load_to_lds(to + (uint32_t)(j * THREADS * 16), base, off[j]);
+  __device__ __forceinline__ void fetch(uint32_t wave_lds, int j) const {   // wave_lds: where the wave's first vector goes
+    load_to_lds(wave_lds + (uint32_t)(j * THREADS * 16), base, off[j]);
   }
   // the last, partial stage: `left` of the contraction, zeros behind
   __device__ __forceinline__ void fetch_tail(char *lds, int left) const {
@@ -360,22 +358,32 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
                                              int left, bool idle, f32x16 (&acc)[S::TM][S::TN]) {
   using PA = Panel<A_COL, S::BM, S::THREADS>;
   using PB = Panel<B_COL, S::BN, S::THREADS>;
-  constexpr int AHEAD = S::STAGES - 1, LOADS = PA::LOADS + PB::LOADS;
-  const uint32_t lds0 = lds_address(smem);
+  constexpr int AHEAD = S::STAGES - 1, LOADS = PA::LOADS + PB::LOADS, STEPS = FK / 16, TILES = S::TM * S::TN;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem) + (threadIdx.x & ~63u) * 16u);
   const int stages = full + (left ? 1 : 0);
-  int put = 0;
-  auto fetch = [&](int t) {
-    const int at = put * S::STAGE;
-    put = put + 1 == S::STAGES ? 0 : put + 1;
-    if (t < full) {
-      a.fetch(lds0 + at);
-      b.fetch(lds0 + at + S::A_BYTES);
-    } else if (t < stages) {
-      a.fetch_tail(smem + at, left);
-      b.fetch_tail(smem + at + S::A_BYTES, left);
-    }
+  int put = 0, get = 0;   // bytes: the stage being filled, the stage being read
+  auto load = [&](int j) {
+    if (j < PA::LOADS) a.fetch(lds0 + put, j);
+    else b.fetch(lds0 + put + S::A_BYTES, j - PA::LOADS);
+  };
+  auto filled = [&]() {
+    put = put + S::STAGE == S::STAGES * S::STAGE ? 0 : put + S::STAGE;
     a.base += a.step;
     b.base += b.step;
+  };
+  // The loads of a stage are spread over the matrix instructions of three steps (slots 0 .. 3 TILES): issued in one go they
+  // fill the memory pipeline's queue and every wave stands before it with its matrix instructions undone.
+  auto loads_at = [&](int slot) {
+#pragma unroll
+    for (int j = 0; j < LOADS; j++)
+      if (j * 3 * TILES / LOADS == slot) load(j);
+  };
+  auto tail = [&](int t) {   // stages that are not whole: the partial one, or nothing
+    if (t == full && left) {
+      a.fetch_tail(smem + put, left);
+      b.fetch_tail(smem + put + S::A_BYTES, left);
+    }
+    filled();
   };
   // Stage t is here once all loads but those of the stages behind it have arrived, for every wave.
   auto arrive = [&](int t) {
@@ -383,44 +391,71 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
   };
-  constexpr int STEPS = FK / 16;
   u32x4 av[2][S::TM], bv[2][S::TN];
-  int get = 0;
   auto read = [&](int set, int step) {
-    if (idle) return;
-    const char *sa = smem + get * S::STAGE, *sb = sa + S::A_BYTES;
+    const char *sa = smem + get, *sb = sa + S::A_BYTES;
 #pragma unroll
     for (int j = 0; j < S::TN; j++) bv[set][j] = b.fragment(sb, j, step);
 #pragma unroll
     for (int i = 0; i < S::TM; i++) av[set][i] = a.fragment(sa, i, step);
   };
-#pragma unroll
-  for (int t = 0; t < AHEAD; t++) fetch(t);
-  arrive(0);
-  read(0, 0);
-  fetch(AHEAD);
-  for (int t = 0; t < stages; t++) {
-    // The fragments of the next step are read while the current one's are multiplied; the step that ends a stage waits for
-    // the next stage first, so the barrier and the first reads of a stage hide behind matrix instructions too.
+  // One stage.  The fragments of the next step are read while the current one's are multiplied; the step that ends a stage
+  // waits for the next stage first, so the barrier and the first reads of a stage hide behind matrix instructions too.
+  auto stage = [&](auto works, int t, bool loads_now, bool loads_next) {
+    constexpr bool WORKS = decltype(works)::value;
 #pragma unroll
     for (int step = 0; step < STEPS; step++) {
       const int set = step & 1, next = set ^ 1;
-      if (step + 1 < STEPS) {
-        read(next, step + 1);
+      const bool ends = step + 1 == STEPS;
+      if (!ends) {
+        if (WORKS) read(next, step + 1);
       } else if (t + 1 < stages) {
         arrive(t + 1);
-        get = get + 1 == S::STAGES ? 0 : get + 1;
-        read(next, 0);
-        fetch(t + 1 + AHEAD);
+        get = get + S::STAGE == S::STAGES * S::STAGE ? 0 : get + S::STAGE;
+        if (WORKS) read(next, 0);
+        if (!loads_next) tail(t + 1 + AHEAD);
       }
-      if (!idle) {
+      const bool loads = ends ? loads_next : loads_now && step < 2;
+      const int slot0 = ends ? 0 : (step + 1) * TILES;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < S::TM; i++)
+      for (int i = 0; i < S::TM; i++)
 #pragma unroll
-          for (int j = 0; j < S::TN; j++) acc[i][j] = mfma16<DT>(bv[set][j], av[set][i], acc[i][j]);
-      }
+        for (int j = 0; j < S::TN; j++) {
+          if (WORKS) acc[i][j] = mfma16<DT>(bv[set][j], av[set][i], acc[i][j]);
+          if (loads) {
+            loads_at(slot0 + i * S::TN + j);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      if (loads_now && step == 1) filled();
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < AHEAD; t++) {
+    if (t < full) {
+#pragma unroll
+      for (int j = 0; j < LOADS; j++) load(j);
+      filled();
+    } else {
+      tail(t);
     }
   }
+  auto run = [&](auto works) {
+    arrive(0);
+    if (decltype(works)::value) read(0, 0);
+    if (AHEAD < full) {
+#pragma unroll
+      for (int slot = 0; slot < TILES; slot++) loads_at(slot);
+    } else {
+      tail(AHEAD);
+    }
+    int t = 0;
+    for (; t + 1 + AHEAD < full; t++) stage(works, t, true, true);
+    for (; t < stages; t++) stage(works, t, t + AHEAD < full, false);
+  };
+  if (idle) run(std::false_type());   // the same waits and barriers
+  else run(std::true_type());
   wait_loads<0>();
   __builtin_amdgcn_s_barrier();   // the stages are free
 }
