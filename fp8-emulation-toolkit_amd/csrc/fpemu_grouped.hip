@@ -9,7 +9,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
-#include <stdlib.h>
 
 #include <type_traits>
 
@@ -102,96 +101,203 @@ template <int BM> struct TileMap {
   }
 };
 
-// ---- any sizes, any alignment: 128 x 128 tiles, elements staged one by one --------------------------------------------------
-constexpr int GT = 128;
-template <int DT> struct Gen {
-  static constexpr int BK = DT == FPEMU_F32 ? 16 : 32;
-  static constexpr int LD = DT == FPEMU_F32 ? BK + 1 : BK + 8;
-};
-
-// element (r, k) of an operand: p[r * ld + k], or p[k * ld + r] where the contraction is its slow dimension (COL)
-template <int DT, bool COL>
-__device__ __forceinline__ void stage(typename Storage<DT>::elem *lds, const typename Storage<DT>::elem *p, int64_t ld, int64_t r0,
-                                      int64_t rend, int64_t k0, int64_t kend, typename Storage<DT>::elem pad) {
-  constexpr int BK = Gen<DT>::BK, LD = Gen<DT>::LD;
-  for (int i = threadIdx.x; i < GT * BK; i += 256) {
-    const int r = COL ? i % GT : i / BK, k = COL ? i / GT : i % BK;
-    const int64_t gr = r0 + r, gk = k0 + k;
-    lds[r * LD + k] = gr < rend && gk < kend ? (COL ? p[gk * ld + gr] : p[gr * ld + gk]) : pad;
-  }
+// Workgroup b runs on XCD b % 8: each XCD gets an eighth of the tiles, one after the other, so that neighbours share rows of
+// x and a group's weights in its L2.
+constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t tiles) {
+  const uint32_t share = (tiles + 7u) / 8u, at = b >> 3;
+  const uint32_t id = (b & 7u) * share + at;
+  return at < share && id < tiles ? id : NO_TILE;
 }
 
-template <int DT, bool A_COL, bool B_COL>
-__device__ __forceinline__ void tile_product(const typename Storage<DT>::elem *a, int64_t lda, int64_t ar0, int64_t arend,
-                                             const typename Storage<DT>::elem *b, int64_t ldb, int64_t br0, int64_t brend, int64_t k0,
-                                             int64_t kend, f32x16 (&acc)[2][2]) {
+// Row and column tile of number id: bands of four row tiles, down the band first, so that the tiles an XCD works on at one
+// time are about as high as wide and share what they read.
+__device__ __forceinline__ void banded(uint32_t id, uint32_t row_tiles, uint32_t col_tiles, uint32_t &row, uint32_t &col) {
+  const uint32_t band = id / (4u * col_tiles), in = id - band * 4u * col_tiles;
+  const uint32_t high = row_tiles - band * 4u < 4u ? row_tiles - band * 4u : 4u;
+  row = band * 4u + in % high;
+  col = in / high;
+}
+
+// ---- any storage, sizes and alignment: 128 x 128 tiles staged through registers ----------------------------------------------
+// fp32 is bound by its matrix instructions (64 cycles each, 512 of them a stage), so a plain double buffer feeds it: the next
+// stage's vectors are loaded into registers, the current one is multiplied, then they are written to the other LDS buffer.
+// The same kernel takes 16-bit operands whose rows are not whole 16-byte vectors: global loads need no more than element
+// alignment, and vectors that reach over an edge are put together element by element.
+// A stage is 128 bytes deep in k (64 16-bit or 32 fp32 elements).  LDS holds it as described for the tiles further down.
+constexpr int GT = 128;
+typedef uint32_t vec_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+// in vectors of 16 bytes: 16 rows that are read together lie in 16 different places of 256 bytes
+__device__ __forceinline__ int swizzle_row(int row) { return (row >> 1) & 7; }
+// four 16-bit k-rows of a transposing read, or the two fp32 k-rows of a matrix instruction, go to different banks
+template <int ES, int EXT> __device__ __forceinline__ int swizzle_col(int k) {
+  return ES == 4 ? (k & 1) * 8 : EXT >= 128 ? (k & 3) * 4 : 0;
+}
+
+// element (r, k) of an operand: p[r * ld + k], or p[k * ld + r] where the contraction is its slow dimension (COL)
+template <int DT, bool COL> struct Staged {
   using elem = typename Storage<DT>::elem;
-  constexpr int BK = Gen<DT>::BK, LD = Gen<DT>::LD;
-  __shared__ __attribute__((aligned(16))) elem as[GT * LD];
-  __shared__ __attribute__((aligned(16))) elem bs[GT * LD];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
-  elem apad = 0, bpad = 0;
-  if constexpr (DT == FPEMU_F32) apad = -0.0f;   // products of the ragged end are -0: they leave any chain as it is
-  for (int64_t k = k0; k < kend; k += BK) {
-    stage<DT, A_COL>(as, a, lda, ar0, arend, k, kend, apad);
-    stage<DT, B_COL>(bs, b, ldb, br0, brend, k, kend, bpad);
-    __syncthreads();
-    if constexpr (DT == FPEMU_F32) {
-#pragma unroll
-      for (int kk = 0; kk < BK; kk += 2) {
-        float av[2], bv[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          av[i] = as[(wr + i * 32 + (lane & 31)) * LD + kk + (lane >> 5)];
-          bv[i] = bs[(wc + i * 32 + (lane & 31)) * LD + kk + (lane >> 5)];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[i], bv[j], acc[i][j], 0, 0, 0);
-      }
+  static constexpr int ES = (int)sizeof(elem), V = 16 / ES, FK = 128 / ES, LOADS = GT * 128 / 16 / 256;
+  static constexpr int BYTES = GT * 128;
+  const elem *base;   // the tile's first element at the stage's first k
+  int64_t ld, step;
+  int lim;            // entries of the tile
+  elem pad;           // what a load behind the contraction yields
+  u32x4 v[LOADS];
+
+  __device__ __forceinline__ void set(const elem *p, int64_t ld_, int lim_, elem pad_) {
+    base = p;
+    ld = ld_;
+    lim = lim_;
+    pad = pad_;
+    step = (COL ? ld : 1) * FK;
+  }
+  __device__ __forceinline__ static void place(int j, int &outer, int &k) {
+    const int id = j * 256 + (int)threadIdx.x;
+    if (COL) {
+      constexpr int PER = GT / V;
+      k = id / PER;
+      outer = ((id % PER) ^ swizzle_col<ES, GT>(k)) * V;
     } else {
+      outer = id / 8;
+      k = ((id & 7) ^ swizzle_row(outer)) * V;
+    }
+  }
+  // the next stage, of which `left` k are there
+  __device__ __forceinline__ void load(int64_t left) {
 #pragma unroll
-      for (int kk = 0; kk < BK; kk += 16) {
-        u32x4 av[2], bv[2];
+    for (int j = 0; j < LOADS; j++) {
+      int outer, k;
+      place(j, outer, k);
+      const int r = outer < lim ? outer : lim - 1;   // entries beyond the tile's only feed results that are not stored
+      const elem *p = COL ? base + k * ld + r : base + r * ld + k;
+      const int have = COL ? (k < left ? (lim - r < V ? lim - r : V) : 0) : left - k >= V ? V : (int)(left - k);
+      if (have >= V) {
+        v[j] = *(const vec_any *)p;
+      } else {
+        elem e[V];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          av[i] = *(const u32x4 *)&as[(wr + i * 32 + (lane & 31)) * LD + kk + (lane >> 5) * 8];
-          bv[i] = *(const u32x4 *)&bs[(wc + i * 32 + (lane & 31)) * LD + kk + (lane >> 5) * 8];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            if constexpr (DT == FPEMU_BF16)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, av[i]), __builtin_bit_cast(bf16x8, bv[j]),
-                                                                  acc[i][j], 0, 0, 0);
-            else
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, av[i]), __builtin_bit_cast(f16x8, bv[j]),
-                                                                 acc[i][j], 0, 0, 0);
-          }
+        for (int i = 0; i < V; i++) e[i] = i < have ? p[i] : pad;
+        __builtin_memcpy(&v[j], e, 16);
       }
     }
+    base += step;
+  }
+  __device__ __forceinline__ void put(char *lds) const {
+#pragma unroll
+    for (int j = 0; j < LOADS; j++) *(u32x4 *)(lds + (j * 256 + (int)threadIdx.x) * 16) = v[j];
+  }
+  // 16-bit: a matrix operand of 32 entries from `at`, k-step of 16.  fp32: the operands of two matrix instructions, k-step of
+  // 4: the k of lane half h are 0 + h and 2 + h, a row's four come as one vector and pick() takes the lane's two.
+  __device__ __forceinline__ static u32x4 fragment(const char *lds, int at, int step) {
+    const int lane = threadIdx.x & 63;
+    u32x4 r = {0u, 0u, 0u, 0u};
+    if constexpr (!COL) {
+      const int row = at + (lane & 31), c = DT == FPEMU_F32 ? step : step * 2 + (lane >> 5);
+      r = *(const u32x4 *)(lds + row * 128 + ((c ^ swizzle_row(row)) * 16));
+    } else if constexpr (DT == FPEMU_F32) {
+      const int col = at + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int k = step * 4 + i * 2 + (lane >> 5);
+        r[i] = *(const uint32_t *)(lds + k * (GT * 4) + (((col >> 2) ^ swizzle_col<4, GT>(k)) * 16) + (col & 3) * 4);
+      }
+    } else {
+      const int i = lane & 15, g = lane >> 4, col = at + (g & 1) * 16 + (i & 3) * 4;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int k = step * 16 + (g >> 1) * 8 + h * 4 + (i >> 2);
+        const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(
+            lds + k * (GT * 2) + (((col >> 3) ^ swizzle_col<2, GT>(k)) * 16) + (col & 7) * 2));
+        const uint2 w = __builtin_bit_cast(uint2, t);
+        r[2 * h] = w.x;
+        r[2 * h + 1] = w.y;
+      }
+    }
+    return r;
+  }
+  __device__ __forceinline__ static float pick(u32x4 r, int i) {
+    if constexpr (COL) return u2f(r[i]);
+    else return u2f((threadIdx.x & 32u) ? r[2 * i + 1] : r[2 * i]);
+  }
+};
+
+template <int DT> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (DT == FPEMU_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// acc[i][j] of a wave (2 x 2 over the tile): rows wr + 32 i of A, columns wc + 32 j of B; k of them, ascending
+template <int DT, bool A_COL, bool B_COL>
+__device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL> &a, Staged<DT, B_COL> &b, int64_t k, f32x16 (&acc)[2][2]) {
+  using SA = Staged<DT, A_COL>;
+  using SB = Staged<DT, B_COL>;
+  constexpr int STEPS = DT == FPEMU_F32 ? SA::FK / 4 : SA::FK / 16, STAGE = SA::BYTES + SB::BYTES;
+  const int wave = threadIdx.x >> 6, wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+  char *now = smem, *then = smem + STAGE;
+  a.load(k);
+  b.load(k);
+  a.put(now);
+  b.put(now + SA::BYTES);
+  __syncthreads();
+  for (int64_t left = k; left > 0; left -= SA::FK) {
+    if (left > SA::FK) {
+      a.load(left - SA::FK);
+      b.load(left - SA::FK);
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+      u32x4 av[2], bv[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        av[i] = SA::fragment(now, wr + i * 32, s);
+        bv[i] = SB::fragment(now + SA::BYTES, wc + i * 32, s);
+      }
+      if constexpr (DT == FPEMU_F32) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(SA::pick(av[i], h), SB::pick(bv[j], h), acc[i][j], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) acc[i][j] = mfma16<DT>(av[i], bv[j], acc[i][j]);
+      }
+    }
+    if (left > SA::FK) {
+      a.put(then);
+      b.put(then + SA::BYTES);
+    }
     __syncthreads();
+    char *t = now;
+    now = then;
+    then = t;
   }
 }
 
 template <int DT>
-__device__ __forceinline__ void tile_store(typename Storage<DT>::elem *c, int64_t ldc, int64_t r0, int64_t rend, int64_t c0, int64_t cend,
-                                           const f32x16 (&acc)[2][2]) {
+__device__ __forceinline__ void any_store(typename Storage<DT>::elem *c, int64_t ldc, int rlim, int clim, const f32x16 (&acc)[2][2]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
 #pragma unroll
   for (int i = 0; i < 2; i++)
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      const int64_t col = c0 + wc + j * 32 + (lane & 31);
-      if (col >= cend) continue;
+      const int col = wc + j * 32 + (lane & 31);
+      if (col >= clim) continue;
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        const int64_t row = r0 + wr + i * 32 + (e / 4) * 8 + (lane >> 5) * 4 + (e & 3);
-        if (row >= rend) continue;
+        const int row = wr + i * 32 + (e / 4) * 8 + (lane >> 5) * 4 + (e & 3);
+        if (row >= rlim) continue;
         const float v = acc[i][j][e] + 0.0f;   // the chain's -0 is written as the c-model writes it
         if constexpr (DT == FPEMU_F32) c[row * ldc + col] = v;
         else c[row * ldc + col] = (typename Storage<DT>::elem)store_elem16<DT>(v);
@@ -199,35 +305,62 @@ __device__ __forceinline__ void tile_store(typename Storage<DT>::elem *c, int64_
     }
 }
 
+// Behind the contraction A's filler is -0 and B's +0 in fp32: products of -0, the one value that leaves any chain as it is.
+template <int DT> __device__ __forceinline__ typename Storage<DT>::elem a_pad() {
+  if constexpr (DT == FPEMU_F32) return -0.0f;
+  else return 0;
+}
+
 template <int DT, bool W_TRANS>
-__global__ __launch_bounds__(256) void grouped_any_kernel(typename Storage<DT>::elem *y, const typename Storage<DT>::elem *x,
-                                                          const typename Storage<DT>::elem *w, const int32_t *offsets, int64_t M,
-                                                          int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
+__global__ __launch_bounds__(256, 2) void grouped_any_kernel(typename Storage<DT>::elem *y, const typename Storage<DT>::elem *x,
+                                                             const typename Storage<DT>::elem *w, const int32_t *offsets, int64_t M,
+                                                             int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * 2 * GT * 128];
   const TileMap<GT> map(offsets, groups, M);
-  if (blockIdx.x / col_tiles >= map.tiles()) return;
-  const RowTile r = map.find(blockIdx.x / col_tiles);
-  const int64_t c0 = (int64_t)(blockIdx.x % col_tiles) * GT;
+  const uint32_t id = xcd_tile(blockIdx.x, map.tiles() * col_tiles);
+  if (id == NO_TILE) return;
+  uint32_t row_tile, col_tile;
+  banded(id, map.tiles(), col_tiles, row_tile, col_tile);
+  const RowTile r = map.find(row_tile);
+  const int64_t c0 = (int64_t)col_tile * GT;
+  const int rows = (int)(r.end - r.first), cols = (int)(N - c0 < GT ? N - c0 : GT);
   f32x16 acc[2][2] = {};
   if (r.group >= 0) {
     const typename Storage<DT>::elem *wg = w + (int64_t)r.group * K * N;
-    tile_product<DT, false, !W_TRANS>(x, K, r.first, r.end, wg, W_TRANS ? K : N, c0, N, 0, K, acc);
+    Staged<DT, false> a;
+    Staged<DT, !W_TRANS> b;
+    a.set(x + r.first * K, K, rows, a_pad<DT>());
+    b.set(W_TRANS ? wg + c0 * K : wg + c0, W_TRANS ? K : N, cols, 0);
+    any_product<DT, false, !W_TRANS>(smem, a, b, K, acc);
   }
-  tile_store<DT>(y, N, r.first, r.end, c0, N, acc);
+  any_store<DT>(y + r.first * N + c0, N, rows, cols, acc);
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void grouped_wgrad_any_kernel(typename Storage<DT>::elem *dw, const typename Storage<DT>::elem *a,
-                                                                const typename Storage<DT>::elem *b, const int32_t *offsets,
-                                                                int64_t M, int64_t P, int64_t Q, uint32_t ptiles, uint32_t qtiles) {
-  const uint32_t g = blockIdx.x / (ptiles * qtiles), t = blockIdx.x % (ptiles * qtiles);
-  const int64_t p0 = (int64_t)(t / qtiles) * GT, q0 = (int64_t)(t % qtiles) * GT;
+__global__ __launch_bounds__(256, 2) void grouped_wgrad_any_kernel(typename Storage<DT>::elem *dw, const typename Storage<DT>::elem *a,
+                                                                   const typename Storage<DT>::elem *b, const int32_t *offsets,
+                                                                   int64_t M, int64_t P, int64_t Q, uint32_t ptiles, uint32_t qtiles,
+                                                                   uint32_t tiles) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * 2 * GT * 128];
+  const uint32_t id = xcd_tile(blockIdx.x, tiles);
+  if (id == NO_TILE) return;
+  const uint32_t g = id / (ptiles * qtiles);
+  uint32_t pt, qt;
+  banded(id % (ptiles * qtiles), ptiles, qtiles, pt, qt);
+  const int64_t p0 = (int64_t)pt * GT, q0 = (int64_t)qt * GT;
   const int64_t lo = row_at(offsets, g, M), hi = row_at(offsets, (int64_t)g + 1, M);
+  const int plim = (int)(P - p0 < GT ? P - p0 : GT), qlim = (int)(Q - q0 < GT ? Q - q0 : GT);
   f32x16 acc[2][2] = {};
-  tile_product<DT, true, true>(a, P, p0, P, b, Q, q0, Q, lo, hi, acc);
-  tile_store<DT>(dw + (int64_t)g * P * Q, Q, p0, P, q0, Q, acc);
+  if (hi > lo) {
+    Staged<DT, true> sa, sb;
+    sa.set(a + lo * P + p0, P, plim, a_pad<DT>());
+    sb.set(b + lo * Q + q0, Q, qlim, 0);
+    any_product<DT, true, true>(smem, sa, sb, hi - lo, acc);
+  }
+  any_store<DT>(dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, acc);
 }
 
-// ---- 16-bit storage in whole 16-byte vectors: tiles fed by loads that go straight to LDS ----------------------------------
+// ---- 16-bit storage in whole 16-byte vectors: tiles fed by loads that go straight to LDS -----------------------------------
 // A tile of BM rows x BN columns, 64 deep in k per stage; while one stage is multiplied the next ones are on their way.
 // A stage row of 64 k is 128 bytes, a whole cache line: with 32 deep stages every line was fetched twice (it had left the
 // 32 KB L1 before its second half was asked for), and the tiles then ran at the rate of the L2, not of the matrix cores.
@@ -237,9 +370,6 @@ __global__ __launch_bounds__(256) void grouped_wgrad_any_kernel(typename Storage
 // fetches and undone where the fragment is read.
 // Waves: WM x WN over the tile.
 constexpr int FK = 64;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) char lds_char;
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(const lds_char *)p; }
 
@@ -286,16 +416,12 @@ template <bool COL, int EXT, int THREADS> struct Panel {
     if (COL) {
       constexpr int PER = EXT / 8;
       k = id / PER;
-      outer = ((id % PER) ^ swizzle_col(k)) * 8;
+      outer = ((id % PER) ^ swizzle_col<2, EXT>(k)) * 8;
     } else {
       outer = id / 8;
       k = ((id & 7) ^ swizzle_row(outer)) * 8;
     }
   }
-  // in vectors of 16 bytes: 16 rows that are read together lie in 16 different places of 256 bytes
-  __device__ __forceinline__ static int swizzle_row(int row) { return (row >> 1) & 7; }
-  // four k-rows of a transposing read go to different banks
-  __device__ __forceinline__ static int swizzle_col(int k) { return EXT >= 128 ? (k & 3) * 4 : EXT >= 64 ? (k & 1) * 4 : 0; }
   __device__ __forceinline__ void fetch(uint32_t wave_lds, int j) const {   // wave_lds: where the wave's first vector goes
     load_to_lds(wave_lds + (uint32_t)(j * THREADS * 16), base, off[j]);
   }
@@ -317,7 +443,7 @@ template <bool COL, int EXT, int THREADS> struct Panel {
     const int lane = threadIdx.x & 63;
     if constexpr (COL) {
       const int i = lane & 15, g = lane >> 4, k = (g >> 1) * 8 + (i >> 2), col = at + (g & 1) * 16 + (i & 3) * 4;
-      frag[0] = (uint32_t)(k * (EXT * 2) + (((col >> 3) ^ swizzle_col(k)) * 16) + (col & 7) * 2);
+      frag[0] = (uint32_t)(k * (EXT * 2) + (((col >> 3) ^ swizzle_col<2, EXT>(k)) * 16) + (col & 7) * 2);
     } else {
       const int row = at + (lane & 31);
 #pragma unroll
@@ -344,13 +470,6 @@ template <bool COL, int EXT, int THREADS> struct Panel {
   }
 };
 
-template <int DT> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (DT == FPEMU_BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
 // acc[i][j]: entries wa + 32 i of A (its columns) and wb + 32 j of B (its rows): a lane holds 4 neighbours along B.
 // idle: this wave's part of the tile has no rows (it still loads and waits with the others).
 template <int DT, class S, bool A_COL, bool B_COL>
@@ -358,7 +477,8 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
                                              int left, bool idle, f32x16 (&acc)[S::TM][S::TN]) {
   using PA = Panel<A_COL, S::BM, S::THREADS>;
   using PB = Panel<B_COL, S::BN, S::THREADS>;
-  constexpr int AHEAD = S::STAGES - 1, LOADS = PA::LOADS + PB::LOADS, STEPS = FK / 16, TILES = S::TM * S::TN;
+  constexpr int AHEAD = S::STAGES - 1, LOADS = PA::LOADS + PB::LOADS, STEPS = FK / 16, TILES = S::TM * S::TN, SPREAD = 2,
+                LATE = TILES / 2, SLOTS = SPREAD * TILES - LATE;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem) + (threadIdx.x & ~63u) * 16u);
   const int stages = full + (left ? 1 : 0);
   int put = 0, get = 0;   // bytes: the stage being filled, the stage being read
@@ -371,12 +491,13 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
     a.base += a.step;
     b.base += b.step;
   };
-  // The loads of a stage are spread over the matrix instructions of three steps (slots 0 .. 3 TILES): issued in one go they
-  // fill the memory pipeline's queue and every wave stands before it with its matrix instructions undone.
+  // The loads of a stage are spread over the matrix instructions of a step and a half (slots 0 .. SLOTS): issued in one go
+  // they fill the memory pipeline's queue and every wave stands before it with its matrix instructions undone; spread
+  // wider, the last ones arrive late (8192^3, bf16: 1119 TFLOP/s in one go, 1274 over three steps, 1346 like this).
   auto loads_at = [&](int slot) {
 #pragma unroll
     for (int j = 0; j < LOADS; j++)
-      if (j * 3 * TILES / LOADS == slot) load(j);
+      if (j * SLOTS / LOADS == slot) load(j);
   };
   auto tail = [&](int t) {   // stages that are not whole: the partial one, or nothing
     if (t == full && left) {
@@ -400,35 +521,36 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
     for (int i = 0; i < S::TM; i++) av[set][i] = a.fragment(sa, i, step);
   };
   // One stage.  The fragments of the next step are read while the current one's are multiplied; the step that ends a stage
-  // waits for the next stage first, so the barrier and the first reads of a stage hide behind matrix instructions too.
+  // waits for the next stage half way, so the barrier and the first reads of a stage hide behind matrix instructions too.
   auto stage = [&](auto works, int t, bool loads_now, bool loads_next) {
     constexpr bool WORKS = decltype(works)::value;
 #pragma unroll
     for (int step = 0; step < STEPS; step++) {
       const int set = step & 1, next = set ^ 1;
       const bool ends = step + 1 == STEPS;
-      if (!ends) {
-        if (WORKS) read(next, step + 1);
-      } else if (t + 1 < stages) {
-        arrive(t + 1);
-        get = get + S::STAGE == S::STAGES * S::STAGE ? 0 : get + S::STAGE;
-        if (WORKS) read(next, 0);
-        if (!loads_next) tail(t + 1 + AHEAD);
-      }
-      const bool loads = ends ? loads_next : loads_now && step < 2;
+      if (!ends && WORKS) read(next, step + 1);
+      const bool loads = ends ? loads_next : loads_now && step + 1 < SPREAD;
       const int slot0 = ends ? 0 : (step + 1) * TILES;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < S::TM; i++)
-#pragma unroll
-        for (int j = 0; j < S::TN; j++) {
-          if (WORKS) acc[i][j] = mfma16<DT>(bv[set][j], av[set][i], acc[i][j]);
-          if (loads) {
-            loads_at(slot0 + i * S::TN + j);
-            __builtin_amdgcn_sched_barrier(0);
+      for (int m = 0; m < TILES; m++) {
+        if (ends && m == LATE) {
+          if (t + 1 < stages) {
+            arrive(t + 1);
+            get = get + S::STAGE == S::STAGES * S::STAGE ? 0 : get + S::STAGE;
+            if (WORKS) read(next, 0);
+            if (!loads_next) tail(t + 1 + AHEAD);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
-      if (loads_now && step == 1) filled();
+        const int i = m / S::TN, j = m % S::TN;
+        if (WORKS) acc[i][j] = mfma16<DT>(bv[set][j], av[set][i], acc[i][j]);
+        if (loads) {
+          loads_at(ends ? m - LATE : slot0 - LATE + m);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (loads_now && step + 2 == SPREAD) filled();
     }
   };
 #pragma unroll
@@ -446,7 +568,7 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
     if (decltype(works)::value) read(0, 0);
     if (AHEAD < full) {
 #pragma unroll
-      for (int slot = 0; slot < TILES; slot++) loads_at(slot);
+      for (int slot = 0; slot < TILES - LATE; slot++) loads_at(slot);
     } else {
       tail(AHEAD);
     }
@@ -482,24 +604,6 @@ __device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc,
   if (col < clim)
     for (int row = threadIdx.x / PER; row < rlim; row += S::THREADS / PER)
       *(u32x4 *)(c + row * ldc + col) = *(const u32x4 *)(t + row * S::OUT_LD + col);
-}
-
-// Workgroup b runs on XCD b % 8: each XCD gets an eighth of the tiles, one after the other, so that neighbours share rows of
-// x and a group's weights in its L2.
-constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
-__device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t tiles) {
-  const uint32_t share = (tiles + 7u) / 8u, at = b >> 3;
-  const uint32_t id = (b & 7u) * share + at;
-  return at < share && id < tiles ? id : NO_TILE;
-}
-
-// Row and column tile of number id: bands of four row tiles, down the band first, so that the tiles an XCD works on at one
-// time are about as high as wide and share what they read.
-__device__ __forceinline__ void banded(uint32_t id, uint32_t row_tiles, uint32_t col_tiles, uint32_t &row, uint32_t &col) {
-  const uint32_t band = id / (4u * col_tiles), in = id - band * 4u * col_tiles;
-  const uint32_t high = row_tiles - band * 4u < 4u ? row_tiles - band * 4u : 4u;
-  row = band * 4u + in % high;
-  col = in / high;
 }
 
 template <class S> struct WaveAt {   // a wave's part of the tile; waves that share a SIMD (w, w + 4) differ in their rows
@@ -590,14 +694,57 @@ int launched(const char *who) {
   return e == hipSuccess ? FPEMU_OK : fail((int)e, who, hipGetErrorString(e));
 }
 
+// A shape's tiles cost the same whether their rows are filled or not, so the large one needs groups of some rows, and tiles
+// for every CU.  bf16, TFLOP/s with 256 x 256 / 128 x 128 tiles: 16 groups of 1024 rows, 2048 x 4096: 966 / 777; 16 of 512,
+// 1024 x 2816: 807 / 812; 8 of 256, 768 x 1024: 164 / 291; 32 of 2 rows, 2048 x 1408: 5.3 / 6.2 TB/s of weights.
+constexpr int64_t kLargeRows = 512, kLargeTiles = 512;
+bool large_tiles(int64_t rows_per_group, int64_t tiles) { return rows_per_group >= kLargeRows && tiles >= kLargeTiles; }
+
 template <int DT>
-void run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t groups,
-                 int w_trans, unsigned blocks, uint32_t cols, hipStream_t s) {
+bool run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t groups,
+                 int w_trans, hipStream_t s) {
   using elem = typename Storage<DT>::elem;
-  if (w_trans)
-    grouped_any_kernel<DT, true><<<blocks, 256, 0, s>>>((elem *)y, (const elem *)x, (const elem *)w, offsets, M, N, K, groups, cols);
-  else
-    grouped_any_kernel<DT, false><<<blocks, 256, 0, s>>>((elem *)y, (const elem *)x, (const elem *)w, offsets, M, N, K, groups, cols);
+  auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel) {
+    const int64_t cols = ceil_div(N, bn), rows = ceil_div(M, bm) + groups + 2;   // every group may end in a partial tile
+    if (rows * cols > 0x7FFFFFF0ll) return false;
+    kernel<<<(unsigned)(ceil_div(rows * cols, 8) * 8), threads, 0, s>>>((elem *)y, (const elem *)x, (const elem *)w, offsets, M, N, K, groups,
+                                                                        (uint32_t)cols);
+    return true;
+  };
+  if constexpr (DT != FPEMU_F32) {
+    if (K > 0 && fast_rows(y, N) && fast_rows(x, K) && fast_rows(w, N)) {
+      if (large_tiles(M / groups, ceil_div(M, Large::BM) * ceil_div(N, Large::BN))) {
+        if (w_trans ? go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, true, Large>)
+                    : go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, false, Large>))
+          return true;
+      }
+      return w_trans ? go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, true, Medium>)
+                     : go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, false, Medium>);
+    }
+  }
+  return w_trans ? go(GT, GT, 256, grouped_any_kernel<DT, true>) : go(GT, GT, 256, grouped_any_kernel<DT, false>);
+}
+
+template <int DT>
+bool run_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, int64_t M, int64_t P, int64_t Q, int64_t groups,
+               hipStream_t s) {
+  using elem = typename Storage<DT>::elem;
+  auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel) {
+    const int64_t pt = ceil_div(P, bm), qt = ceil_div(Q, bn);
+    if (pt * qt > 0x7FFFFFF0ll / groups) return false;
+    const int64_t tiles = pt * qt * groups;
+    kernel<<<(unsigned)(ceil_div(tiles, 8) * 8), threads, 0, s>>>((elem *)dw, (const elem *)a, (const elem *)b, offsets, M, P, Q, (uint32_t)pt,
+                                                                  (uint32_t)qt, (uint32_t)tiles);
+    return true;
+  };
+  if constexpr (DT != FPEMU_F32) {
+    if (M > 0 && fast_rows(dw, Q) && fast_rows(a, P) && fast_rows(b, Q)) {
+      if (large_tiles(M / groups, ceil_div(P, Large::BM) * ceil_div(Q, Large::BN) * groups))
+        return go(Large::BM, Large::BN, Large::THREADS, grouped_wgrad_fast_kernel<DT, Large>);
+      return go(Medium::BM, Medium::BN, Medium::THREADS, grouped_wgrad_fast_kernel<DT, Medium>);
+    }
+  }
+  return go(GT, GT, 256, grouped_wgrad_any_kernel<DT>);
 }
 
 }  // namespace
@@ -608,32 +755,11 @@ extern "C" int fpemu_grouped_gemm(void *y, const void *x, const void *w, const i
   if (const int rc = check_grouped(who, y, x, w, offsets, M, N, K, groups, dtype)) return rc;
   if (M == 0 || N == 0) return FPEMU_OK;
   if (y == nullptr || (K > 0 && (x == nullptr || w == nullptr))) return fail(FPEMU_EINVAL, who, "null buffer");
-  const int64_t cols = ceil_div(N, GT), rows = ceil_div(M, GT) + groups + 2;   // every group may end in a partial tile
-  if (rows * cols > 0x7FFFFFFFll) return fail(FPEMU_EINVAL, who, "too many tiles for one launch");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype != FPEMU_F32 && K > 0 && fast_rows(y, N) && fast_rows(x, K) && fast_rows(w, N)) {
-    static const char *force = getenv("FPEMU_GROUPED_SHAPE");
-    auto shape = [&](auto tag) {
-      using S = decltype(tag);
-      const int64_t ct = ceil_div(N, S::BN), rt = ceil_div(M, S::BM) + groups + 2;
-      if (rt * ct > 0x7FFFFFF0ll) return false;
-      const unsigned blocks = (unsigned)(ceil_div(rt * ct, 8) * 8);
-      auto go = [&](auto kernel) {
-        kernel<<<blocks, S::THREADS, 0, s>>>((uint16_t *)y, (const uint16_t *)x, (const uint16_t *)w, offsets, M, N, K, groups, (uint32_t)ct);
-      };
-      if (dtype == FPEMU_F16) w_trans ? go(grouped_fast_kernel<FPEMU_F16, true, S>) : go(grouped_fast_kernel<FPEMU_F16, false, S>);
-      else w_trans ? go(grouped_fast_kernel<FPEMU_BF16, true, S>) : go(grouped_fast_kernel<FPEMU_BF16, false, S>);
-      return true;
-    };
-    const int f = force ? atoi(force) : -1;
-    const bool done = f == 0 ? shape(Large()) : f == 1 ? shape(Medium()) : M >= 512 * groups ? shape(Large()) : shape(Medium());
-    if (done) return launched(who);
-  }
-  const unsigned blocks = (unsigned)(rows * cols);
-  if (dtype == FPEMU_F32) run_grouped<FPEMU_F32>(y, x, w, offsets, M, N, K, groups, w_trans, blocks, (uint32_t)cols, s);
-  else if (dtype == FPEMU_F16) run_grouped<FPEMU_F16>(y, x, w, offsets, M, N, K, groups, w_trans, blocks, (uint32_t)cols, s);
-  else run_grouped<FPEMU_BF16>(y, x, w, offsets, M, N, K, groups, w_trans, blocks, (uint32_t)cols, s);
-  return launched(who);
+  const bool done = dtype == FPEMU_F32   ? run_grouped<FPEMU_F32>(y, x, w, offsets, M, N, K, groups, w_trans, s)
+                    : dtype == FPEMU_F16 ? run_grouped<FPEMU_F16>(y, x, w, offsets, M, N, K, groups, w_trans, s)
+                                         : run_grouped<FPEMU_BF16>(y, x, w, offsets, M, N, K, groups, w_trans, s);
+  return done ? launched(who) : fail(FPEMU_EINVAL, who, "too many tiles for one launch");
 }
 
 extern "C" int fpemu_grouped_gemm_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, int64_t M, int64_t P, int64_t Q,
@@ -642,33 +768,9 @@ extern "C" int fpemu_grouped_gemm_wgrad(void *dw, const void *a, const void *b, 
   if (const int rc = check_grouped(who, dw, a, b, offsets, M, P, Q, groups, dtype)) return rc;
   if (P == 0 || Q == 0) return FPEMU_OK;
   if (dw == nullptr || (M > 0 && (a == nullptr || b == nullptr))) return fail(FPEMU_EINVAL, who, "null buffer");
-  const int64_t pt = ceil_div(P, GT), qt = ceil_div(Q, GT);
-  if (pt * qt > 0x7FFFFFFFll / groups) return fail(FPEMU_EINVAL, who, "too many tiles for one launch");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype != FPEMU_F32 && M > 0 && fast_rows(dw, Q) && fast_rows(a, P) && fast_rows(b, Q)) {
-    static const char *force = getenv("FPEMU_GROUPED_SHAPE");
-    auto shape = [&](auto tag) {
-      using S = decltype(tag);
-      const int64_t pf = ceil_div(P, S::BM), qf = ceil_div(Q, S::BN), tiles = pf * qf * groups;   // no more than the ones above
-      const unsigned blocks = (unsigned)(ceil_div(tiles, 8) * 8);
-      auto go = [&](auto kernel) {
-        kernel<<<blocks, S::THREADS, 0, s>>>((uint16_t *)dw, (const uint16_t *)a, (const uint16_t *)b, offsets, M, P, Q, (uint32_t)pf,
-                                             (uint32_t)qf, (uint32_t)tiles);
-      };
-      if (dtype == FPEMU_F16) go(grouped_wgrad_fast_kernel<FPEMU_F16, S>);
-      else go(grouped_wgrad_fast_kernel<FPEMU_BF16, S>);
-    };
-    const int f = force ? atoi(force) : -1;
-    if (f == 0) shape(Large());
-    else shape(Medium());
-    return launched(who);
-  }
-  const unsigned blocks = (unsigned)(pt * qt * groups);
-  if (dtype == FPEMU_F32)
-    grouped_wgrad_any_kernel<FPEMU_F32><<<blocks, 256, 0, s>>>((float *)dw, (const float *)a, (const float *)b, offsets, M, P, Q, (uint32_t)pt, (uint32_t)qt);
-  else if (dtype == FPEMU_F16)
-    grouped_wgrad_any_kernel<FPEMU_F16><<<blocks, 256, 0, s>>>((uint16_t *)dw, (const uint16_t *)a, (const uint16_t *)b, offsets, M, P, Q, (uint32_t)pt, (uint32_t)qt);
-  else
-    grouped_wgrad_any_kernel<FPEMU_BF16><<<blocks, 256, 0, s>>>((uint16_t *)dw, (const uint16_t *)a, (const uint16_t *)b, offsets, M, P, Q, (uint32_t)pt, (uint32_t)qt);
-  return launched(who);
+  const bool done = dtype == FPEMU_F32   ? run_wgrad<FPEMU_F32>(dw, a, b, offsets, M, P, Q, groups, s)
+                    : dtype == FPEMU_F16 ? run_wgrad<FPEMU_F16>(dw, a, b, offsets, M, P, Q, groups, s)
+                                         : run_wgrad<FPEMU_BF16>(dw, a, b, offsets, M, P, Q, groups, s);
+  return done ? launched(who) : fail(FPEMU_EINVAL, who, "too many tiles for one launch");
 }
