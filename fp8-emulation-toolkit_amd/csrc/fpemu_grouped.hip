@@ -119,13 +119,12 @@ __device__ __forceinline__ void banded(uint32_t id, uint32_t row_tiles, uint32_t
   col = in / high;
 }
 
-// ---- any storage, sizes and alignment: 128 x 128 tiles staged through registers ----------------------------------------------
+// ---- any storage, sizes and alignment: tiles staged through registers ----------------------------------------------------------------
 // fp32 is bound by its matrix instructions (64 cycles each, 512 of them a stage), so a plain double buffer feeds it: the next
 // stage's vectors are loaded into registers, the current one is multiplied, then they are written to the other LDS buffer.
 // The same kernel takes 16-bit operands whose rows are not whole 16-byte vectors: global loads need no more than element
 // alignment, and vectors that reach over an edge are put together element by element.
 // A stage is 128 bytes deep in k (64 16-bit or 32 fp32 elements).  LDS holds it as described for the tiles further down.
-constexpr int GT = 128;
 typedef uint32_t vec_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
@@ -134,14 +133,14 @@ typedef __attribute__((address_space(3))) char lds_char;
 __device__ __forceinline__ int swizzle_row(int row) { return (row >> 1) & 7; }
 // four 16-bit k-rows of a transposing read, or the two fp32 k-rows of a matrix instruction, go to different banks
 template <int ES, int EXT> __device__ __forceinline__ int swizzle_col(int k) {
-  return ES == 4 ? (k & 1) * 8 : EXT >= 128 ? (k & 3) * 4 : 0;
+  return ES == 4 ? (k & 1) * 8 : EXT >= 128 ? (k & 3) * 4 : (k & 1) * 4;
 }
 
 // element (r, k) of an operand: p[r * ld + k], or p[k * ld + r] where the contraction is its slow dimension (COL)
-template <int DT, bool COL> struct Staged {
+template <int DT, bool COL, int EXT> struct Staged {
   using elem = typename Storage<DT>::elem;
-  static constexpr int ES = (int)sizeof(elem), V = 16 / ES, FK = 128 / ES, LOADS = GT * 128 / 16 / 256;
-  static constexpr int BYTES = GT * 128;
+  static constexpr int ES = (int)sizeof(elem), V = 16 / ES, FK = 128 / ES, LOADS = EXT * 128 / 16 / 256;
+  static constexpr int BYTES = EXT * 128;
   const elem *base;   // the tile's first element at the stage's first k
   int64_t ld, step;
   int lim;            // entries of the tile
@@ -158,9 +157,9 @@ template <int DT, bool COL> struct Staged {
   __device__ __forceinline__ static void place(int j, int &outer, int &k) {
     const int id = j * 256 + (int)threadIdx.x;
     if (COL) {
-      constexpr int PER = GT / V;
+      constexpr int PER = EXT / V;
       k = id / PER;
-      outer = ((id % PER) ^ swizzle_col<ES, GT>(k)) * V;
+      outer = ((id % PER) ^ swizzle_col<ES, EXT>(k)) * V;
     } else {
       outer = id / 8;
       k = ((id & 7) ^ swizzle_row(outer)) * V;
@@ -203,7 +202,7 @@ template <int DT, bool COL> struct Staged {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int k = step * 4 + i * 2 + (lane >> 5);
-        r[i] = *(const uint32_t *)(lds + k * (GT * 4) + (((col >> 2) ^ swizzle_col<4, GT>(k)) * 16) + (col & 3) * 4);
+        r[i] = *(const uint32_t *)(lds + k * (EXT * 4) + (((col >> 2) ^ swizzle_col<4, EXT>(k)) * 16) + (col & 3) * 4);
       }
     } else {
       const int i = lane & 15, g = lane >> 4, col = at + (g & 1) * 16 + (i & 3) * 4;
@@ -211,7 +210,7 @@ template <int DT, bool COL> struct Staged {
       for (int h = 0; h < 2; h++) {
         const int k = step * 16 + (g >> 1) * 8 + h * 4 + (i >> 2);
         const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(
-            lds + k * (GT * 2) + (((col >> 3) ^ swizzle_col<2, GT>(k)) * 16) + (col & 7) * 2));
+            lds + k * (EXT * 2) + (((col >> 3) ^ swizzle_col<2, EXT>(k)) * 16) + (col & 7) * 2));
         const uint2 w = __builtin_bit_cast(uint2, t);
         r[2 * h] = w.x;
         r[2 * h + 1] = w.y;
@@ -232,13 +231,20 @@ template <int DT> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// acc[i][j] of a wave (2 x 2 over the tile): rows wr + 32 i of A, columns wc + 32 j of B; k of them, ascending
-template <int DT, bool A_COL, bool B_COL>
-__device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL> &a, Staged<DT, B_COL> &b, int64_t k, f32x16 (&acc)[2][2]) {
-  using SA = Staged<DT, A_COL>;
-  using SB = Staged<DT, B_COL>;
+template <int BM_, int BN_> struct AnyShape {   // 4 waves: 2 x 2 over the tile, side by side over one of 32 rows
+  static constexpr int BM = BM_, BN = BN_, WM = BM >= 64 ? 2 : 1, WN = 4 / WM, TM = BM / WM / 32, TN = BN / WN / 32;
+  __device__ __forceinline__ static int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM); }
+  __device__ __forceinline__ static int col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN); }
+};
+
+// acc[i][j] of a wave: rows S::row() + 32 i of A, columns S::col() + 32 j of B; k of them, ascending
+template <int DT, class S, bool A_COL, bool B_COL>
+__device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL, S::BM> &a, Staged<DT, B_COL, S::BN> &b, int64_t k,
+                                            f32x16 (&acc)[S::TM][S::TN]) {
+  using SA = Staged<DT, A_COL, S::BM>;
+  using SB = Staged<DT, B_COL, S::BN>;
   constexpr int STEPS = DT == FPEMU_F32 ? SA::FK / 4 : SA::FK / 16, STAGE = SA::BYTES + SB::BYTES;
-  const int wave = threadIdx.x >> 6, wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+  const int wr = S::row(), wc = S::col();
   char *now = smem, *then = smem + STAGE;
   a.load(k);
   b.load(k);
@@ -252,25 +258,24 @@ __device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL> &a, St
     }
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
-      u32x4 av[2], bv[2];
+      u32x4 av[S::TM], bv[S::TN];
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        av[i] = SA::fragment(now, wr + i * 32, s);
-        bv[i] = SB::fragment(now + SA::BYTES, wc + i * 32, s);
-      }
+      for (int i = 0; i < S::TM; i++) av[i] = SA::fragment(now, wr + i * 32, s);
+#pragma unroll
+      for (int j = 0; j < S::TN; j++) bv[j] = SB::fragment(now + SA::BYTES, wc + j * 32, s);
       if constexpr (DT == FPEMU_F32) {
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int i = 0; i < 2; i++)
+          for (int i = 0; i < S::TM; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < S::TN; j++)
               acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(SA::pick(av[i], h), SB::pick(bv[j], h), acc[i][j], 0, 0, 0);
       } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < S::TM; i++)
 #pragma unroll
-          for (int j = 0; j < 2; j++) acc[i][j] = mfma16<DT>(av[i], bv[j], acc[i][j]);
+          for (int j = 0; j < S::TN; j++) acc[i][j] = mfma16<DT>(av[i], bv[j], acc[i][j]);
       }
     }
     if (left > SA::FK) {
@@ -284,14 +289,14 @@ __device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL> &a, St
   }
 }
 
-template <int DT>
-__device__ __forceinline__ void any_store(typename Storage<DT>::elem *c, int64_t ldc, int rlim, int clim, const f32x16 (&acc)[2][2]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+template <int DT, class S>
+__device__ __forceinline__ void any_store(typename Storage<DT>::elem *c, int64_t ldc, int rlim, int clim,
+                                          const f32x16 (&acc)[S::TM][S::TN]) {
+  const int lane = threadIdx.x & 63, wr = S::row(), wc = S::col();
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int i = 0; i < S::TM; i++)
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < S::TN; j++) {
       const int col = wc + j * 32 + (lane & 31);
       if (col >= clim) continue;
 #pragma unroll
@@ -311,53 +316,54 @@ template <int DT> __device__ __forceinline__ typename Storage<DT>::elem a_pad() 
   else return 0;
 }
 
-template <int DT, bool W_TRANS>
+template <int DT, bool W_TRANS, class S>
 __global__ __launch_bounds__(256, 2) void grouped_any_kernel(typename Storage<DT>::elem *y, const typename Storage<DT>::elem *x,
                                                              const typename Storage<DT>::elem *w, const int32_t *offsets, int64_t M,
                                                              int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * 2 * GT * 128];
-  const TileMap<GT> map(offsets, groups, M);
+  __shared__ __attribute__((aligned(16))) char smem[2 * (S::BM + S::BN) * 128];
+  const TileMap<S::BM> map(offsets, groups, M);
   const uint32_t id = xcd_tile(blockIdx.x, map.tiles() * col_tiles);
   if (id == NO_TILE) return;
   uint32_t row_tile, col_tile;
   banded(id, map.tiles(), col_tiles, row_tile, col_tile);
   const RowTile r = map.find(row_tile);
-  const int64_t c0 = (int64_t)col_tile * GT;
-  const int rows = (int)(r.end - r.first), cols = (int)(N - c0 < GT ? N - c0 : GT);
-  f32x16 acc[2][2] = {};
+  const int64_t c0 = (int64_t)col_tile * S::BN;
+  const int rows = (int)(r.end - r.first), cols = (int)(N - c0 < S::BN ? N - c0 : S::BN);
+  f32x16 acc[S::TM][S::TN] = {};
   if (r.group >= 0) {
     const typename Storage<DT>::elem *wg = w + (int64_t)r.group * K * N;
-    Staged<DT, false> a;
-    Staged<DT, !W_TRANS> b;
+    Staged<DT, false, S::BM> a;
+    Staged<DT, !W_TRANS, S::BN> b;
     a.set(x + r.first * K, K, rows, a_pad<DT>());
     b.set(W_TRANS ? wg + c0 * K : wg + c0, W_TRANS ? K : N, cols, 0);
-    any_product<DT, false, !W_TRANS>(smem, a, b, K, acc);
+    any_product<DT, S, false, !W_TRANS>(smem, a, b, K, acc);
   }
-  any_store<DT>(y + r.first * N + c0, N, rows, cols, acc);
+  any_store<DT, S>(y + r.first * N + c0, N, rows, cols, acc);
 }
 
-template <int DT>
+template <int DT, class S>
 __global__ __launch_bounds__(256, 2) void grouped_wgrad_any_kernel(typename Storage<DT>::elem *dw, const typename Storage<DT>::elem *a,
                                                                    const typename Storage<DT>::elem *b, const int32_t *offsets,
                                                                    int64_t M, int64_t P, int64_t Q, uint32_t ptiles, uint32_t qtiles,
                                                                    uint32_t tiles) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * 2 * GT * 128];
+  __shared__ __attribute__((aligned(16))) char smem[2 * (S::BM + S::BN) * 128];
   const uint32_t id = xcd_tile(blockIdx.x, tiles);
   if (id == NO_TILE) return;
   const uint32_t g = id / (ptiles * qtiles);
   uint32_t pt, qt;
   banded(id % (ptiles * qtiles), ptiles, qtiles, pt, qt);
-  const int64_t p0 = (int64_t)pt * GT, q0 = (int64_t)qt * GT;
+  const int64_t p0 = (int64_t)pt * S::BM, q0 = (int64_t)qt * S::BN;
   const int64_t lo = row_at(offsets, g, M), hi = row_at(offsets, (int64_t)g + 1, M);
-  const int plim = (int)(P - p0 < GT ? P - p0 : GT), qlim = (int)(Q - q0 < GT ? Q - q0 : GT);
-  f32x16 acc[2][2] = {};
+  const int plim = (int)(P - p0 < S::BM ? P - p0 : S::BM), qlim = (int)(Q - q0 < S::BN ? Q - q0 : S::BN);
+  f32x16 acc[S::TM][S::TN] = {};
   if (hi > lo) {
-    Staged<DT, true> sa, sb;
+    Staged<DT, true, S::BM> sa;
+    Staged<DT, true, S::BN> sb;
     sa.set(a + lo * P + p0, P, plim, a_pad<DT>());
     sb.set(b + lo * Q + q0, Q, qlim, 0);
-    any_product<DT, true, true>(smem, sa, sb, hi - lo, acc);
+    any_product<DT, S, true, true>(smem, sa, sb, hi - lo, acc);
   }
-  any_store<DT>(dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, acc);
+  any_store<DT, S>(dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, acc);
 }
 
 // ---- 16-bit storage in whole 16-byte vectors: tiles fed by loads that go straight to LDS -----------------------------------
@@ -672,6 +678,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t
 
 using Large = Shape<256, 256, 2, 4, 2>;
 using Medium = Shape<128, 128, 2, 2, 2>;
+using Little = Shape<64, 64, 2, 2, 3>;
 
 // Whole 16-byte vectors everywhere, and offsets within a tile that fit 32 bits.
 bool fast_rows(const void *p, int64_t ld) { return (uintptr_t)p % 16u == 0 && ld % 8 == 0 && ld <= 1 << 21; }
@@ -700,6 +707,15 @@ int launched(const char *who) {
 constexpr int64_t kLargeRows = 512, kLargeTiles = 512;
 bool large_tiles(int64_t rows_per_group, int64_t tiles) { return rows_per_group >= kLargeRows && tiles >= kLargeTiles; }
 
+// Fewer 128 x 128 tiles than CUs: 64 x 64 ones.  us with 128 / 64: fp32, 8 groups of 256, 768 x 1000 (128 tiles): 82 / 53; 16 of
+// 256, 1024 x 1024 (256 tiles): 109 / 112; bf16, 4 of 75, 512 x 1024 (24 tiles): 9.2 / 7.8; 16 of 256 (256 tiles): 17.9 / 20.3.
+constexpr int64_t kLittleTiles = 256;
+bool little_tiles(int64_t row_tiles, int64_t col_tiles) { return row_tiles * col_tiles < kLittleTiles; }
+
+// Groups of few rows, staged through registers: tiles of 32 rows leave fewer matrix instructions to rows that are not there.
+// fp32, 32 groups, 2048 x 1408, us with 64 x 64 / 32 x 128 tiles: 2 rows a group 200 / 145, 32 rows 170 / 130, 64 rows 168 / 173.
+bool flat_tiles(int64_t rows, int64_t groups) { return rows <= 32 * groups; }
+
 template <int DT>
 bool run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t groups,
                  int w_trans, hipStream_t s) {
@@ -718,11 +734,19 @@ bool run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, 
                     : go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, false, Large>))
           return true;
       }
+      if (little_tiles(ceil_div(M, Medium::BM), ceil_div(N, Medium::BN)))
+        return w_trans ? go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, true, Little>)
+                       : go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, false, Little>);
       return w_trans ? go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, true, Medium>)
                      : go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, false, Medium>);
     }
   }
-  return w_trans ? go(GT, GT, 256, grouped_any_kernel<DT, true>) : go(GT, GT, 256, grouped_any_kernel<DT, false>);
+  auto any = [&](auto shape) {
+    using S = decltype(shape);
+    return w_trans ? go(S::BM, S::BN, 256, grouped_any_kernel<DT, true, S>) : go(S::BM, S::BN, 256, grouped_any_kernel<DT, false, S>);
+  };
+  if (flat_tiles(M, groups)) return any(AnyShape<32, 128>());
+  return little_tiles(ceil_div(M, 128), ceil_div(N, 128)) ? any(AnyShape<64, 64>()) : any(AnyShape<128, 128>());
 }
 
 template <int DT>
@@ -741,10 +765,13 @@ bool run_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, i
     if (M > 0 && fast_rows(dw, Q) && fast_rows(a, P) && fast_rows(b, Q)) {
       if (large_tiles(M / groups, ceil_div(P, Large::BM) * ceil_div(Q, Large::BN) * groups))
         return go(Large::BM, Large::BN, Large::THREADS, grouped_wgrad_fast_kernel<DT, Large>);
+      if (little_tiles(ceil_div(P, Medium::BM) * groups, ceil_div(Q, Medium::BN)))
+        return go(Little::BM, Little::BN, Little::THREADS, grouped_wgrad_fast_kernel<DT, Little>);
       return go(Medium::BM, Medium::BN, Medium::THREADS, grouped_wgrad_fast_kernel<DT, Medium>);
     }
   }
-  return go(GT, GT, 256, grouped_wgrad_any_kernel<DT>);
+  if (little_tiles(ceil_div(P, 128) * groups, ceil_div(Q, 128))) return go(64, 64, 256, grouped_wgrad_any_kernel<DT, AnyShape<64, 64>>);
+  return go(128, 128, 256, grouped_wgrad_any_kernel<DT, AnyShape<128, 128>>);
 }
 
 }  // namespace
