@@ -30,18 +30,20 @@ int launched(const char *who) {
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 // ---- rows in the order of their group -----------------------------------------------------------------------------
-// A stable counting sort by digits of the group id, least significant digit first (one pass up to 1024 keys, two up to
-// 2^20, ...).  A row outside [0, groups) has the key `groups` and so ends up behind every group.  The rank of a row
-// among the equal digits before it is found wave by wave: ballots over the digit's bits give the lanes with the same
-// digit, one LDS counter per (wave, digit) carries the count from round to round.
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64, kSortRounds = 8;
+// A stable counting sort by digits of the group id, least significant digit first (one pass up to 511 groups, two up to
+// 2^18 - 1, ...).  A row outside [0, groups) has the key `groups` and so ends up behind every group.  The rank of a row among
+// the equal digits before it is found wave by wave: ballots over the digit's bits give the lanes with the same digit, one
+// LDS counter per (wave, digit) carries the count from round to round.  The chain of rounds is what a small sort takes
+// (ballots, an LDS atomic and a shuffle each), so a workgroup is as wide as it can be: 16 waves, four rounds at most.
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortRounds = 4;
 constexpr int kSortTile = kSortThreads * kSortRounds;   // 4096 rows per workgroup
-constexpr int kMaxBits = 10;                            // digits of at most 1024 values: 32 KB of counters
+constexpr int kMaxBits = 9;                             // digits of at most 512 values: 32 KB of counters
 constexpr int kMaxBins = 1 << kMaxBits;
 constexpr unsigned kSelfSum = 32;                       // up to this many tiles a tile adds up the counts before it by itself
+constexpr int kMaxPasses = 4;
 
 struct SortPlan {
-  int bits, passes, shift[4], width[4];
+  int bits, passes, shift[kMaxPasses], width[kMaxPasses];
 };
 
 SortPlan sort_plan(uint64_t groups) {
@@ -58,6 +60,25 @@ SortPlan sort_plan(uint64_t groups) {
   return p;
 }
 
+// Memory that a sort's kernels clear beside their own work, in workgroups behind the sort's: a table's gradient is cleared
+// while its tokens are sorted (the sort keeps a few CUs busy, the stores the memory).
+typedef uint32_t vec_a2 __attribute__((ext_vector_type(4), aligned(2)));   // rows of odd widths: element-aligned only
+struct Fill {
+  char *p;
+  uint64_t bytes;          // even
+  uint64_t first, last;    // this launch's share, in pieces of kFillPiece
+};
+constexpr uint64_t kFillPiece = 128 << 10;   // of one workgroup
+
+__device__ __forceinline__ void fill_piece(const Fill &f, uint64_t piece) {
+  const uint64_t at = (f.first + piece) * kFillPiece, end = at + kFillPiece < f.bytes ? at + kFillPiece : f.bytes;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  uint64_t i = at + threadIdx.x * 16u;
+#pragma unroll 4
+  for (; i + 16 <= end; i += kSortThreads * 16u) *(vec_a2 *)(f.p + i) = zero;
+  for (; i < end; i += 2) *(uint16_t *)(f.p + i) = 0;   // the thread whose vector reaches over the end
+}
+
 __device__ __forceinline__ uint32_t key_of(const void *ids, int wide, uint64_t i, uint32_t groups) {
   if (wide) {
     const uint64_t v = ((const uint64_t *)ids)[i];
@@ -68,12 +89,13 @@ __device__ __forceinline__ uint32_t key_of(const void *ids, int wide, uint64_t i
 }
 
 // rank of each of the lane's rows among the rows of its wave with the same digit before it; cnt: the wave's counters
-__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[kSortRounds], unsigned valid, int bits, uint32_t *cnt,
+__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[kSortRounds], unsigned valid, int rounds, int bits, uint32_t *cnt,
                                            uint32_t (&rank)[kSortRounds]) {
   const unsigned lane = threadIdx.x & 63u;
   const uint64_t below = ((uint64_t)1 << lane) - 1u;
 #pragma unroll
   for (int r = 0; r < kSortRounds; r++) {
+    if (r >= rounds) break;
     const bool ok = (valid >> r) & 1u;
     uint64_t same = __ballot(ok);
     for (int b = 0; b < bits; b++) {
@@ -91,16 +113,11 @@ __device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[kSortRounds],
 
 // exclusive sum over the first `bins` entries of v (LDS), all threads of the workgroup; tmp: kSortWaves words
 __device__ __forceinline__ void exclusive_bins(uint32_t *v, int bins, uint32_t *tmp) {
-  constexpr int PER = kMaxBins / kSortThreads;   // 2
+  static_assert(kMaxBins <= kSortThreads, "a thread per digit");
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint32_t x[PER], sum = 0;
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    const int at = (int)threadIdx.x * PER + i;
-    x[i] = at < bins ? v[at] : 0u;
-    sum += x[i];
-  }
-  uint32_t inc = sum;
+  const int at = (int)threadIdx.x;
+  const uint32_t x = at < bins ? v[at] : 0u;
+  uint32_t inc = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const uint32_t o = (uint32_t)__shfl_up((int)inc, off, 64);
@@ -108,36 +125,34 @@ __device__ __forceinline__ void exclusive_bins(uint32_t *v, int bins, uint32_t *
   }
   if (lane == 63u) tmp[wave] = inc;
   __syncthreads();
-  uint32_t run = inc - sum;
+  uint32_t run = inc - x;
   for (unsigned w = 0; w < wave; w++) run += tmp[w];
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    const int at = (int)threadIdx.x * PER + i;
-    if (at < bins) v[at] = run;
-    run += x[i];
-  }
+  if (at < bins) v[at] = run;
   __syncthreads();
 }
 
-// Up to kSortTile rows: every pass inside one workgroup, rows exchanged through LDS.  keys_out: the sorted keys
-// (passes > 1 only; the offsets are searched in them); with one pass the offsets are the counters' sums.
+// Up to kSortTile rows: every pass inside one workgroup, rows exchanged through LDS.  keys_out (or NULL): the sorted keys;
+// offsets (or NULL): with one pass they are the counters' sums.
 __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const void *ids, int wide, uint32_t n, uint32_t groups,
                                                                   SortPlan plan, int32_t *order, uint32_t *keys_out,
-                                                                  int32_t *offsets) {
+                                                                  int32_t *offsets, Fill fill) {
   __shared__ uint32_t cnt[kSortWaves * kMaxBins];
   __shared__ uint32_t skey[kSortTile];
   __shared__ uint16_t spos[kSortTile];
   __shared__ uint32_t base[kMaxBins];
   __shared__ uint32_t tmp[kSortWaves];
+  if (blockIdx.x > 0) return fill_piece(fill, blockIdx.x - 1u);
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const int rounds = (int)((n + kSortThreads - 1u) / kSortThreads);
+  const uint32_t mine = wave * 64u * (uint32_t)rounds + lane;   // the wave's rows are neighbours
   uint32_t key[kSortRounds], pos[kSortRounds], digit[kSortRounds], rank[kSortRounds];
   unsigned valid = 0;
 #pragma unroll
   for (int r = 0; r < kSortRounds; r++) {
-    const uint32_t i = wave * (64u * kSortRounds) + (uint32_t)r * 64u + lane;
+    const uint32_t i = mine + (uint32_t)r * 64u;
     pos[r] = i;
     key[r] = 0;
-    if (i < n) {
+    if (r < rounds && i < n) {
       key[r] = key_of(ids, wide, i, groups);
       valid |= 1u << r;
     }
@@ -148,10 +163,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const void *id
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; r++) digit[r] = (key[r] >> plan.shift[p]) & (uint32_t)(bins - 1);
-    wave_ranks(digit, valid, plan.width[p], cnt + wave * bins, rank);
+    wave_ranks(digit, valid, rounds, plan.width[p], cnt + wave * bins, rank);
     __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += kSortThreads) {
+    if ((int)threadIdx.x < bins) {
+      const int d = (int)threadIdx.x;
       uint32_t run = 0;
+#pragma unroll
       for (int w = 0; w < kSortWaves; w++) {
         const uint32_t c = cnt[w * bins + d];
         cnt[w * bins + d] = run;
@@ -180,8 +197,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const void *id
     if (!last) {
 #pragma unroll
       for (int r = 0; r < kSortRounds; r++) {
-        const uint32_t i = wave * (64u * kSortRounds) + (uint32_t)r * 64u + lane;
-        if (i < n) {
+        const uint32_t i = mine + (uint32_t)r * 64u;
+        if ((valid >> r) & 1u) {
           key[r] = skey[i];
           pos[r] = spos[i];
         }
@@ -203,8 +220,9 @@ __device__ __forceinline__ uint32_t sort_key(const SortIn &in, uint64_t i, uint3
 }
 
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, uint32_t n, uint32_t groups, int shift, int width,
-                                                                  uint32_t tiles, uint32_t *counts) {
+                                                                  uint32_t tiles, uint32_t *counts, Fill fill) {
   __shared__ uint32_t cnt[kMaxBins];
+  if (blockIdx.x >= tiles) return fill_piece(fill, blockIdx.x - tiles);
   const int bins = 1 << width;
   for (int i = threadIdx.x; i < bins; i += kSortThreads) cnt[i] = 0;
   __syncthreads();
@@ -242,10 +260,11 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t *counts, uint32
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortIn in, uint32_t n, uint32_t groups, int shift, int width,
                                                                   uint32_t tiles, const uint32_t *counts,
                                                                   const uint32_t *totals, uint32_t *keys_out, int32_t *pos_out,
-                                                                  int32_t *offsets) {
+                                                                  int32_t *offsets, Fill fill) {
   __shared__ uint32_t cnt[kSortWaves * kMaxBins];
   __shared__ uint32_t base[kMaxBins];
   __shared__ uint32_t tmp[kSortWaves];
+  if (blockIdx.x >= tiles) return fill_piece(fill, blockIdx.x - tiles);
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const int bins = 1 << width;
   uint32_t key[kSortRounds], pos[kSortRounds], digit[kSortRounds], rank[kSortRounds];
@@ -261,47 +280,36 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortIn in, uin
     }
     digit[r] = (key[r] >> shift) & (uint32_t)(bins - 1);
   }
-  for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) cnt[i] = 0;
-  __syncthreads();
-  wave_ranks(digit, valid, width, cnt + wave * bins, rank);
-  __syncthreads();
-  // per digit: rows before this tile's (own[]), and all rows (base[], turned into the digit's start below)
-  constexpr int PER = kMaxBins / kSortThreads;
-  uint32_t own[PER];
-#pragma unroll
-  for (int j = 0; j < PER; j++) {
-    const int d = (int)threadIdx.x + j * kSortThreads;
-    own[j] = 0;
-    if (d < bins) {
-      if (totals != nullptr) {
-        own[j] = counts[(uint64_t)d * tiles + blockIdx.x];
-        base[d] = totals[d];
-      } else {
-        uint32_t all = 0, before = 0;
-        for (uint32_t t = 0; t < tiles; t++) {
-          const uint32_t c = counts[(uint64_t)d * tiles + t];
-          before += t < blockIdx.x ? c : 0u;
-          all += c;
-        }
-        own[j] = before;
-        base[d] = all;
+  // per digit (a thread each): rows of the tiles before this one, and all rows
+  const int d = (int)threadIdx.x;
+  uint32_t own = 0, all = 0;
+  if (d < bins) {
+    if (totals != nullptr) {
+      own = counts[(uint64_t)d * tiles + blockIdx.x];
+      all = totals[d];
+    } else {
+#pragma unroll 8
+      for (uint32_t t = 0; t < tiles; t++) {
+        const uint32_t c = counts[(uint64_t)d * tiles + t];
+        own += t < blockIdx.x ? c : 0u;
+        all += c;
       }
     }
+    base[d] = all;
   }
+  for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) cnt[i] = 0;
   __syncthreads();
-  exclusive_bins(base, bins, tmp);
+  wave_ranks(digit, valid, kSortRounds, width, cnt + wave * bins, rank);
+  exclusive_bins(base, bins, tmp);   // its barriers also stand between the ranks and the counters' sums
   if (offsets != nullptr && blockIdx.x == 0)
     for (uint32_t g = threadIdx.x; g <= groups; g += kSortThreads) offsets[g] = (int32_t)base[g];
+  if (d < bins) {
+    uint32_t run = base[d] + own;
 #pragma unroll
-  for (int j = 0; j < PER; j++) {
-    const int d = (int)threadIdx.x + j * kSortThreads;
-    if (d < bins) {
-      uint32_t run = base[d] + own[j];
-      for (int w = 0; w < kSortWaves; w++) {
-        const uint32_t c = cnt[w * bins + d];
-        cnt[w * bins + d] = run;
-        run += c;
-      }
+    for (int w = 0; w < kSortWaves; w++) {
+      const uint32_t c = cnt[w * bins + d];
+      cnt[w * bins + d] = run;
+      run += c;
     }
   }
   __syncthreads();
@@ -327,24 +335,20 @@ __global__ __launch_bounds__(256) void sort_offsets_kernel(const uint32_t *keys,
   offsets[g] = (int32_t)lo;
 }
 
-__global__ __launch_bounds__(256) void zero_words_kernel(int32_t *p, uint64_t n) {
-  const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-  if (i < n) p[i] = 0;
-}
+__global__ __launch_bounds__(kSortThreads) void fill_kernel(Fill fill) { fill_piece(fill, blockIdx.x); }
 
-// workspace of the sort, in words: [keys a][pos a][keys b] + counts + totals (passes alternate between a and b; the last
-// pass writes its positions to `order`)
+// workspace of the sort, in words: [sorted keys][keys a][pos a] + counts + totals (passes alternate between a and the results)
 struct SortSpace {
-  uint64_t keys_a, pos_a, keys_b, counts, totals, words;
+  uint64_t keys, keys_a, pos_a, counts, totals, words;
 };
 
-SortSpace sort_space(uint64_t n, uint64_t groups) {
+SortSpace sort_space(uint64_t n, uint64_t groups, bool with_keys) {
   const SortPlan plan = sort_plan(groups);
   const uint64_t tiles = ceil_div(n, kSortTile);
   SortSpace s{};
   uint64_t at = 0;
   auto take = [&](uint64_t words) { const uint64_t o = at; at += (words + 3) / 4 * 4; return o; };
-  if (plan.passes > 1) s.keys_b = take(n);
+  if (plan.passes > 1 || with_keys) s.keys = take(n);
   if (tiles > 1) {
     if (plan.passes > 1) {
       s.keys_a = take(n);
@@ -357,44 +361,57 @@ SortSpace sort_space(uint64_t n, uint64_t groups) {
   return s;
 }
 
-// order[n], offsets[groups + 1]; ws of sort_space().words words
-int sort_rows(const char *who, const void *ids, int wide, uint64_t n, uint64_t groups, int32_t *order, int32_t *offsets,
-              uint32_t *ws, hipStream_t stream) {
+// order[n]; offsets[groups + 1] or NULL; with_keys: the sorted keys at ws + sort_space().keys; fill: cleared on the way
+int sort_rows(const char *who, const void *ids, int wide, uint64_t n, uint64_t groups, int32_t *order, int32_t *offsets, bool with_keys,
+              uint32_t *ws, Fill fill, hipStream_t stream) {
   const SortPlan plan = sort_plan(groups);
-  const SortSpace sp = sort_space(n, groups);
+  const SortSpace sp = sort_space(n, groups, with_keys);
   const uint32_t n32 = (uint32_t)n, g32 = (uint32_t)groups;
+  const uint32_t tiles = (uint32_t)ceil_div(n, kSortTile);
+  const uint64_t pieces = ceil_div(fill.bytes, kFillPiece);
+  // the share of launch i of `of` launches that clear something
+  auto share = [&](int i, int of) {
+    fill.first = pieces * (uint64_t)i / (uint64_t)of;
+    fill.last = pieces * (uint64_t)(i + 1) / (uint64_t)of;
+    return (unsigned)(fill.last - fill.first);
+  };
   if (n == 0) {
-    zero_words_kernel<<<(unsigned)ceil_div(groups + 1, 256), 256, 0, stream>>>(offsets, groups + 1);
+    if (pieces > 0) {
+      const unsigned blocks = share(0, 1);
+      fill_kernel<<<blocks, kSortThreads, 0, stream>>>(fill);
+    }
+    if (offsets != nullptr) {
+      const Fill zero{(char *)offsets, 4 * (groups + 1), 0, 0};
+      fill_kernel<<<(unsigned)ceil_div(zero.bytes, kFillPiece), kSortThreads, 0, stream>>>(zero);
+    }
     return launched(who);
   }
-  const uint32_t tiles = (uint32_t)ceil_div(n, kSortTile);
-  const uint32_t *sorted = nullptr;
+  uint32_t *sorted = plan.passes > 1 || with_keys ? ws + sp.keys : nullptr;
   if (tiles == 1) {
-    uint32_t *keys = plan.passes > 1 ? ws + sp.keys_b : nullptr;
-    sort_small_kernel<<<1, kSortThreads, 0, stream>>>(ids, wide, n32, g32, plan, order, keys, offsets);
-    sorted = keys;
+    const unsigned more = share(0, 1);
+    sort_small_kernel<<<1 + more, kSortThreads, 0, stream>>>(ids, wide, n32, g32, plan, order, sorted, offsets, fill);
   } else {
     SortIn in{ids, nullptr, nullptr, wide};
     for (int p = 0; p < plan.passes; p++) {
-      const bool last = p + 1 == plan.passes;
-      // the last pass's keys go to b (only the offsets read them); the ones before alternate so that they end in a
-      uint32_t *keys = plan.passes == 1 ? nullptr : ws + (((plan.passes - 1 - p) & 1) ? sp.keys_a : sp.keys_b);
-      int32_t *pos = last || ((plan.passes - 1 - p) & 1) == 0 ? order : (int32_t *)(ws + sp.pos_a);
-      sort_count_kernel<<<tiles, kSortThreads, 0, stream>>>(in, n32, g32, plan.shift[p], plan.width[p], tiles, ws + sp.counts);
+      const bool other = (plan.passes - 1 - p) & 1;   // passes alternate so that the last one writes the results
+      uint32_t *keys = other ? ws + sp.keys_a : sorted;
+      int32_t *pos = other ? (int32_t *)(ws + sp.pos_a) : order;
+      unsigned more = share(2 * p, 2 * plan.passes);
+      sort_count_kernel<<<tiles + more, kSortThreads, 0, stream>>>(in, n32, g32, plan.shift[p], plan.width[p], tiles, ws + sp.counts, fill);
       const uint32_t *totals = nullptr;
       if (tiles > kSelfSum) {
         const int bins = 1 << plan.width[p];
         sort_scan_kernel<<<(unsigned)ceil_div(bins, 4), 256, 0, stream>>>(ws + sp.counts, tiles, bins, ws + sp.totals);
         totals = ws + sp.totals;
       }
-      sort_place_kernel<<<tiles, kSortThreads, 0, stream>>>(in, n32, g32, plan.shift[p], plan.width[p], tiles, ws + sp.counts,
-                                                            totals, keys, pos, plan.passes == 1 ? offsets : nullptr);
+      more = share(2 * p + 1, 2 * plan.passes);
+      sort_place_kernel<<<tiles + more, kSortThreads, 0, stream>>>(in, n32, g32, plan.shift[p], plan.width[p], tiles, ws + sp.counts, totals,
+                                                                   keys, pos, plan.passes == 1 ? offsets : nullptr, fill);
       in.keys = keys;
       in.pos = pos;
-      sorted = keys;
     }
   }
-  if (plan.passes > 1)
+  if (plan.passes > 1 && offsets != nullptr)
     sort_offsets_kernel<<<(unsigned)ceil_div(groups + 1, 256), 256, 0, stream>>>(sorted, n32, g32, offsets);
   return launched(who);
 }
@@ -409,8 +426,6 @@ int check_ids(const char *who, const void *ids, int id_bytes, uint64_t n, uint64
 }
 
 // ---- vectors of 16 bytes at any element address ----------------------------------------------------------------------
-typedef uint32_t vec_a2 __attribute__((ext_vector_type(4), aligned(2)));   // rows of odd widths: element-aligned only
-
 template <int DT> struct Elems {
   static constexpr int V = DT == FPEMU_F32 ? 4 : 8;
   using elem = typename Storage<DT>::elem;
@@ -469,100 +484,196 @@ __device__ __forceinline__ int64_t id_at(const void *ids, int wide, uint64_t i) 
   return wide ? ((const int64_t *)ids)[i] : (int64_t)((const int32_t *)ids)[i];
 }
 
-// out[t] = scale * weight[ids[t]]: 2^lg_tpr threads a row.  A row whose id is outside the table reads nothing and is NaN.
-template <int DT>
+// out[t] = scale * weight[ids[t]]: 2^lg_tpr threads a row, R rows a thread (their loads are in flight together).  A row whose
+// id is outside the table reads nothing of it and is NaN.
+template <int DT, int R>
 __global__ __launch_bounds__(256) void embedding_kernel(const void *weight, const void *ids, int wide, void *out, uint64_t n,
                                                         uint64_t vocab, uint64_t width, float scale, int lg_tpr) {
   using E = Elems<DT>;
-  const uint64_t t = (uint64_t)blockIdx.x * (256u >> lg_tpr) + (threadIdx.x >> lg_tpr);
-  if (t >= n) return;
-  const int64_t id = id_at(ids, wide, t);
-  const bool known = id >= 0 && (uint64_t)id < vocab;
-  const typename E::elem *src = (const typename E::elem *)weight + (known ? (uint64_t)id : 0u) * width;
-  typename E::elem *dst = (typename E::elem *)out + t * width;
+  const uint64_t rows = 256u >> lg_tpr;
+  const uint64_t t0 = (uint64_t)blockIdx.x * rows * R + (threadIdx.x >> lg_tpr);
+  const typename E::elem *src[R];
+  bool known[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const uint64_t t = t0 + r * rows;
+    const int64_t id = t < n ? id_at(ids, wide, t) : 0;
+    known[r] = id >= 0 && (uint64_t)id < vocab;
+    src[r] = (const typename E::elem *)weight + (known[r] ? (uint64_t)id : 0u) * width;
+  }
   const uint64_t step = (uint64_t)E::V << lg_tpr;
   for (uint64_t c = (uint64_t)(threadIdx.x & ((1u << lg_tpr) - 1u)) * E::V; c < width; c += step) {
-    float f[E::V];
-    if (known) {
-      load_cols<DT>(src, c, width, f);
+    if (c + E::V <= width) {
+      u32x4 v[R];
 #pragma unroll
-      for (int j = 0; j < E::V; j++) f[j] *= scale;
+      for (int r = 0; r < R; r++) v[r] = *(const vec_a2 *)(src[r] + c);
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const uint64_t t = t0 + r * rows;
+        if (t >= n) continue;
+        float f[E::V];
+        E::unpack(v[r], f);
+#pragma unroll
+        for (int j = 0; j < E::V; j++) f[j] = known[r] ? f[j] * scale : u2f(0x7FC00000u);
+        *(vec_a2 *)((typename E::elem *)out + t * width + c) = E::pack(f);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < E::V; j++) f[j] = u2f(0x7FC00000u);
+      for (int r = 0; r < R; r++) {
+        const uint64_t t = t0 + r * rows;
+        if (t >= n) continue;
+        for (uint64_t j = c; j < width; j++)
+          E::put((typename E::elem *)out + t * width + j, known[r] ? E::one(src[r] + j) * scale : u2f(0x7FC00000u));
+      }
     }
-    store_cols<DT>(dst, c, width, f);
   }
 }
 
-// Gradient of the table from the sorted tokens.  The sorted positions are cut into chunks of `chunk`; a chunk that lies
-// inside one entry's run is summed by embedding_chunks_kernel (a frequent token's run is long: its chunks go to many
-// workgroups), and an entry's row is the sum of its chunks' sums and of the tokens at its two ends.
-template <int DT>
-__global__ __launch_bounds__(64) void embedding_chunks_kernel(const void *dout, const void *ids, int wide, const int32_t *order,
-                                                              uint32_t n, uint64_t width, uint32_t chunk, float *sums) {
-  using E = Elems<DT>;
-  const uint32_t first = blockIdx.x * chunk;
-  if ((uint64_t)first + chunk > n) return;
-  if (id_at(ids, wide, (uint64_t)order[first]) != id_at(ids, wide, (uint64_t)order[first + chunk - 1u])) return;
-  const uint64_t c = ((uint64_t)blockIdx.y * 64u + threadIdx.x) * E::V;
-  if (c >= width) return;
-  float acc[E::V] = {};
-#pragma unroll 4
-  for (uint32_t i = 0; i < chunk; i++) {
-    float f[E::V];
-    load_cols<DT>((const typename E::elem *)dout + (uint64_t)order[first + i] * width, c, width, f);
-#pragma unroll
-    for (int j = 0; j < E::V; j++) acc[j] += f[j];
+// Gradient of the table from the sorted tokens; the table is zero when these kernels run.  The sorted positions are cut into
+// chunks.  A wave takes the runs (tokens of one entry) that begin in its chunk, to their ends, and writes their rows; a chunk
+// that an earlier run fills is summed by a wave of its own first (a frequent token's run is long: its chunks go to many
+// waves), so behind its own chunk a run is a list of chunk sums and the tokens of the chunk that it ends in.
+// 64 lanes take 16 bytes of the row each; a wave loads the rows of eight tokens before it adds the first.
+constexpr uint32_t kSub = 16;    // positions looked at together: their keys and tokens lie in the wave's lanes
+constexpr int kRows = 8;
+
+struct Tokens {
+  const void *dout;
+  const uint32_t *keys;     // sorted; entries outside the table have the key `vocab`
+  const int32_t *order;
+  uint32_t n, vocab, padding, chunk;
+  uint64_t width;
+};
+
+// One look at kSub positions from `base`: keys and tokens in the lanes, which positions are there, begin a run, count.
+struct Look {
+  uint32_t key, pos, there, starts, counts;
+  __device__ __forceinline__ Look(const Tokens &t, uint32_t base) {
+    const uint32_t lane = threadIdx.x & 63u, i = base + lane;
+    const bool here = lane < kSub && i < t.n;
+    key = here ? t.keys[i] : 0xFFFFFFFFu;
+    pos = here ? (uint32_t)t.order[i] : 0u;
+    const uint32_t before = here && i > 0 ? t.keys[i - 1] : 0xFFFFFFFFu;
+    there = (uint32_t)__ballot(here);
+    starts = (uint32_t)__ballot(here && key != before);
+    counts = (uint32_t)__ballot(here && key < t.vocab && key != t.padding);
   }
-  float *row = sums + (uint64_t)blockIdx.x * width;
+};
+
+// adds the rows of the positions in `take` of one look, in order; flush(j) runs before position j of `at` is added
+template <int DT, class F>
+__device__ __forceinline__ void add_rows(const Tokens &t, const Look &look, uint32_t take, uint64_t c, float (&acc)[Elems<DT>::V], F &&flush) {
+  using E = Elems<DT>;
 #pragma unroll
-  for (int j = 0; j < E::V; j++)
-    if (c + j < width) row[c + j] = acc[j];
+  for (uint32_t j0 = 0; j0 < kSub; j0 += kRows) {
+    if (!((take | look.starts) >> j0 & ((1u << kRows) - 1u))) continue;
+    float f[kRows][E::V];
+#pragma unroll
+    for (uint32_t u = 0; u < kRows; u++) {   // positions that are not taken load row 0 and are not added
+      const uint32_t row = (take >> (j0 + u)) & 1u ? (uint32_t)__builtin_amdgcn_readlane((int)look.pos, (int)(j0 + u)) : 0u;
+      load_cols<DT>((const typename E::elem *)t.dout + (uint64_t)row * t.width, c, t.width, f[u]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kRows; u++) {
+      flush(j0 + u);
+      if ((take >> (j0 + u)) & 1u) {
+#pragma unroll
+        for (int e = 0; e < E::V; e++) acc[e] += f[u][e];
+      }
+    }
+  }
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void embedding_rows_kernel(const void *dout, const int32_t *order, const int32_t *offsets,
-                                                             const float *sums, void *dweight, uint64_t vocab, uint64_t width,
-                                                             uint32_t chunk, float scale, int64_t padding) {
+// the lane's first column; lanes behind the row's end do column 0's work and store nothing
+template <int DT> __device__ __forceinline__ uint64_t column(uint64_t width, bool &mine) {
+  const uint64_t c = ((uint64_t)blockIdx.y * 64u + (threadIdx.x & 63u)) * Elems<DT>::V;
+  mine = c < width;
+  return mine ? c : 0;
+}
+
+template <int DT> __global__ __launch_bounds__(256) void embedding_chunks_kernel(Tokens t, float *sums) {
   using E = Elems<DT>;
-  const uint64_t v = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
-  if (v >= vocab) return;
-  const uint64_t c = ((uint64_t)blockIdx.y * 64u + (threadIdx.x & 63u)) * E::V;
-  if (c >= width) return;
-  uint32_t i = (uint32_t)offsets[v];
-  const uint32_t end = (int64_t)v == padding ? i : (uint32_t)offsets[v + 1];
+  const uint32_t chunk = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t first = (uint64_t)chunk * t.chunk;
+  if (first == 0 || first + t.chunk > t.n) return;
+  const uint32_t key = t.keys[first - 1];
+  if (key != t.keys[first + t.chunk - 1] || key >= t.vocab || key == t.padding) return;   // not inside one run
+  bool mine;
+  const uint64_t c = column<DT>(t.width, mine);
   float acc[E::V] = {};
-  while (i < end) {
-    if (i % chunk == 0 && i + chunk <= end) {
-      const float *row = sums + (uint64_t)(i / chunk) * width;
+  for (uint32_t base = 0; base < t.chunk; base += kSub) {
+    const Look look(t, (uint32_t)first + base);
+    add_rows<DT>(t, look, look.there, c, acc, [](uint32_t) {});
+  }
+  if (mine) {
+    float *row = sums + (uint64_t)chunk * t.width;
+#pragma unroll
+    for (int j = 0; j < E::V; j++)
+      if (c + j < t.width) row[c + j] = acc[j];
+  }
+}
+
+template <int DT> __global__ __launch_bounds__(256) void embedding_runs_kernel(Tokens t, const float *sums, void *dweight, float scale) {
+  using E = Elems<DT>;
+  const uint64_t first = (uint64_t)(blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * t.chunk;
+  if (first >= t.n) return;
+  bool mine;
+  const uint64_t c = column<DT>(t.width, mine);
+  float acc[E::V] = {};
+  bool open = false;      // a run of this chunk is being added up
+  uint32_t entry = 0;
+  auto close = [&]() {
+    if (open && mine) {
+      float out[E::V];
+#pragma unroll
+      for (int j = 0; j < E::V; j++) out[j] = acc[j] * scale;
+      store_cols<DT>((typename E::elem *)dweight + (uint64_t)entry * t.width, c, t.width, out);
+    }
+#pragma unroll
+    for (int j = 0; j < E::V; j++) acc[j] = 0.f;
+  };
+  for (uint32_t base = 0; base < t.chunk && first + base < t.n; base += kSub) {
+    const Look look(t, (uint32_t)(first + base));
+    // positions before the first run that begins here belong to an earlier chunk's, unless one of ours is open
+    const uint32_t ours = open ? ~0u : look.starts ? ~((look.starts & (0u - look.starts)) - 1u) : 0u;
+    add_rows<DT>(t, look, look.counts & ours, c, acc, [&](uint32_t j) {
+      if (!((look.starts >> j) & 1u)) return;
+      close();
+      open = (look.counts >> j) & 1u;
+      entry = (uint32_t)__builtin_amdgcn_readlane((int)look.key, (int)j);
+    });
+  }
+  for (uint64_t at = first + t.chunk; open && at < t.n; at += t.chunk) {   // the last run goes on
+    if (t.keys[at] != entry) break;
+    if (at + t.chunk <= t.n && t.keys[at + t.chunk - 1] == entry) {
+      const float *row = sums + at / t.chunk * t.width;
 #pragma unroll
       for (int j = 0; j < E::V; j++)
-        if (c + j < width) acc[j] += row[c + j];
-      i += chunk;
-    } else {
-      float f[E::V];
-      load_cols<DT>((const typename E::elem *)dout + (uint64_t)order[i] * width, c, width, f);
-#pragma unroll
-      for (int j = 0; j < E::V; j++) acc[j] += f[j];
-      i++;
+        if (c + j < t.width) acc[j] += row[c + j];
+      continue;
     }
+    for (uint32_t base = 0; base < t.chunk && at + base < t.n; base += kSub) {
+      const Look look(t, (uint32_t)(at + base));
+      const uint32_t same = (uint32_t)__ballot(look.key == entry) & look.there;
+      if (!same) break;
+      Look rest = look;
+      rest.starts = 0;
+      add_rows<DT>(t, rest, same, c, acc, [](uint32_t) {});
+    }
+    break;
   }
-#pragma unroll
-  for (int j = 0; j < E::V; j++) acc[j] *= scale;
-  store_cols<DT>((typename E::elem *)dweight + v * width, c, width, acc);
+  close();
 }
 
 uint32_t chunk_of(uint64_t n) {
-  uint32_t c = 32;
-  while ((uint64_t)c * 2048u < n) c *= 2u;   // at most 2048 chunk sums for one entry
+  uint32_t c = kSub;
+  while ((uint64_t)c * 1024u < n) c *= 2u;   // at most 1024 chunk sums for one entry
   return c;
 }
 
 // ---- norm and clipping of a list of gradients -----------------------------------------------------------------------------
 constexpr int kGrads = 128;              // tensors per launch (the table travels in the kernel arguments)
-constexpr uint64_t kGradChunk = 16384;   // elements of one workgroup's step
-constexpr unsigned kNormBlocks = 1024;   // workgroups (= partial sums) per launch
+constexpr unsigned kNormBlocks = 2048;   // workgroups (= partial sums) per launch
 
 struct GradTable {
   const void *in[kGrads];
@@ -571,6 +682,7 @@ struct GradTable {
   uint32_t end[kGrads];    // chunks of tensors 0 .. i
   uint8_t in_dt[kGrads], out_dt[kGrads];
   int count;
+  uint32_t chunk;          // elements of one workgroup's step
 };
 
 // tensor of chunk c (uniform), and c becomes the chunk within it
@@ -594,20 +706,42 @@ template <int ORDER> __device__ __forceinline__ double norm_add(double acc, floa
   else return norm_join<ORDER>(acc, (double)fabsf(x));
 }
 
-template <int ORDER, int DT> __device__ __forceinline__ double norm_chunk(const void *in, uint64_t n, uint32_t chunk, double acc) {
+// f(vector index) for this thread's whole vectors of `m` elements, four at a time, so that four loads are in flight
+template <int V, class F4, class F1> __device__ __forceinline__ void each_vector(uint32_t m, F4 &&four, F1 &&one) {
+  const uint32_t vecs = m / V;
+  uint32_t i = threadIdx.x;
+  for (; i + 768u < vecs; i += 1024u) four(i);
+  for (; i < vecs; i += 256u) one(i);
+}
+
+template <int ORDER, int DT> __device__ __forceinline__ double norm_chunk(const void *in, uint32_t m, double acc) {
   using E = Elems<DT>;
-  const typename E::elem *p = (const typename E::elem *)in + (uint64_t)chunk * kGradChunk;
-  const uint64_t left = n - (uint64_t)chunk * kGradChunk;
-  const uint32_t m = left < kGradChunk ? (uint32_t)left : (uint32_t)kGradChunk;
+  const typename E::elem *p = (const typename E::elem *)in;
   double a[4] = {acc, 0.0, 0.0, 0.0};
-#pragma unroll 4
-  for (uint32_t c = threadIdx.x * E::V; c < m; c += 256u * E::V) {
+  auto add = [&](u32x4 v) {
     float f[E::V];
-    load_cols<DT>(p, c, m, f);
+    E::unpack(v, f);
 #pragma unroll
     for (int j = 0; j < E::V; j++) a[j & 3] = norm_add<ORDER>(a[j & 3], f[j]);
-  }
+  };
+  each_vector<E::V>(
+      m,
+      [&](uint32_t i) {
+        u32x4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = *(const vec_a2 *)(p + (i + u * 256u) * E::V);
+#pragma unroll
+        for (int u = 0; u < 4; u++) add(v[u]);
+      },
+      [&](uint32_t i) { add(*(const vec_a2 *)(p + i * E::V)); });
+  for (uint32_t i = m / E::V * E::V + threadIdx.x; i < m; i += 256u) a[0] = norm_add<ORDER>(a[0], E::one(p + i));
   return norm_join<ORDER>(norm_join<ORDER>(a[0], a[1]), norm_join<ORDER>(a[2], a[3]));
+}
+
+// elements of chunk c of a tensor of n, and where it begins
+__device__ __forceinline__ uint32_t chunk_size(const GradTable &tab, uint64_t n, uint32_t c, uint64_t &first) {
+  first = (uint64_t)c * tab.chunk;
+  return n - first < tab.chunk ? (uint32_t)(n - first) : tab.chunk;
 }
 
 template <int ORDER> __device__ __forceinline__ double block_join(double acc, double *tmp) {
@@ -626,9 +760,11 @@ template <int ORDER> __global__ __launch_bounds__(256) void norm_kernel(GradTabl
   for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
     uint32_t c = i;
     const int t = grad_of(tab, c);
-    if (tab.in_dt[t] == FPEMU_F32) acc = norm_chunk<ORDER, FPEMU_F32>(tab.in[t], tab.n[t], c, acc);
-    else if (tab.in_dt[t] == FPEMU_F16) acc = norm_chunk<ORDER, FPEMU_F16>(tab.in[t], tab.n[t], c, acc);
-    else acc = norm_chunk<ORDER, FPEMU_BF16>(tab.in[t], tab.n[t], c, acc);
+    uint64_t first;
+    const uint32_t m = chunk_size(tab, tab.n[t], c, first);
+    if (tab.in_dt[t] == FPEMU_F32) acc = norm_chunk<ORDER, FPEMU_F32>((const float *)tab.in[t] + first, m, acc);
+    else if (tab.in_dt[t] == FPEMU_F16) acc = norm_chunk<ORDER, FPEMU_F16>((const uint16_t *)tab.in[t] + first, m, acc);
+    else acc = norm_chunk<ORDER, FPEMU_BF16>((const uint16_t *)tab.in[t] + first, m, acc);
   }
   const double all = block_join<ORDER>(acc, tmp);
   if (threadIdx.x == 0) partial[blockIdx.x] = all;
@@ -642,31 +778,33 @@ template <int ORDER> __global__ __launch_bounds__(1024) void norm_finish_kernel(
   if (threadIdx.x == 0) *sum = all;
 }
 
-template <int DI, int DO> __device__ __forceinline__ void clip_chunk(const void *in, void *out, uint64_t n, uint32_t chunk, float coef) {
+template <int DI, int DO> __device__ __forceinline__ void clip_chunk(const void *in, void *out, uint64_t first, uint32_t m, float coef) {
   using E = Elems<DI>;
   using O = Elems<DO>;
-  const typename E::elem *p = (const typename E::elem *)in + (uint64_t)chunk * kGradChunk;
-  typename O::elem *q = (typename O::elem *)out + (uint64_t)chunk * kGradChunk;
-  const uint64_t left = n - (uint64_t)chunk * kGradChunk;
-  const uint32_t m = left < kGradChunk ? (uint32_t)left : (uint32_t)kGradChunk;
-#pragma unroll 4
-  for (uint32_t c = threadIdx.x * E::V; c < m; c += 256u * E::V) {
+  const typename E::elem *p = (const typename E::elem *)in + first;
+  typename O::elem *q = (typename O::elem *)out + first;
+  auto put = [&](uint32_t i, u32x4 v) {
     float f[E::V];
-    load_cols<DI>(p, c, m, f);
+    E::unpack(v, f);
 #pragma unroll
-    for (int j = 0; j < E::V; j++) f[j] *= coef;
-    if constexpr (DI == DO) {
-      store_cols<DO>(q, c, m, f);
-    } else {   // 16-bit gradients into fp32 ones: two vectors
+    for (int h = 0; h < E::V; h += O::V) {   // 16-bit gradients into fp32 ones: two vectors
+      float g[O::V];
 #pragma unroll
-      for (int h = 0; h < E::V; h += O::V) {
-        float g[O::V];
-#pragma unroll
-        for (int j = 0; j < O::V; j++) g[j] = f[h + j];
-        if (c + h < m) store_cols<DO>(q, c + h, m, g);
-      }
+      for (int j = 0; j < O::V; j++) g[j] = f[h + j] * coef;
+      *(vec_a2 *)(q + i * E::V + h) = O::pack(g);
     }
-  }
+  };
+  each_vector<E::V>(
+      m,
+      [&](uint32_t i) {
+        u32x4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = *(const vec_a2 *)(p + (i + u * 256u) * E::V);
+#pragma unroll
+        for (int u = 0; u < 4; u++) put(i + u * 256u, v[u]);
+      },
+      [&](uint32_t i) { put(i, *(const vec_a2 *)(p + i * E::V)); });
+  for (uint32_t i = m / E::V * E::V + threadIdx.x; i < m; i += 256u) O::put(q + i, E::one(p + i) * coef);
 }
 
 // coef = min(1, max_norm / (norm + 1e-6)), a NaN norm gives a NaN coefficient.  Gradients that stay in place and keep
@@ -684,12 +822,14 @@ __global__ __launch_bounds__(256) void clip_kernel(GradTable tab, uint32_t chunk
     const void *in = tab.in[t];
     void *out = tab.out[t];
     if (coef == 1.0f && in == out) continue;
+    uint64_t first;
+    const uint32_t m = chunk_size(tab, tab.n[t], c, first);
     const int di = tab.in_dt[t], dout = tab.out_dt[t];
-    if (di == FPEMU_F32) clip_chunk<FPEMU_F32, FPEMU_F32>(in, out, tab.n[t], c, coef);
-    else if (di == FPEMU_F16 && dout == FPEMU_F16) clip_chunk<FPEMU_F16, FPEMU_F16>(in, out, tab.n[t], c, coef);
-    else if (di == FPEMU_F16) clip_chunk<FPEMU_F16, FPEMU_F32>(in, out, tab.n[t], c, coef);
-    else if (dout == FPEMU_BF16) clip_chunk<FPEMU_BF16, FPEMU_BF16>(in, out, tab.n[t], c, coef);
-    else clip_chunk<FPEMU_BF16, FPEMU_F32>(in, out, tab.n[t], c, coef);
+    if (di == FPEMU_F32) clip_chunk<FPEMU_F32, FPEMU_F32>(in, out, first, m, coef);
+    else if (di == FPEMU_F16 && dout == FPEMU_F16) clip_chunk<FPEMU_F16, FPEMU_F16>(in, out, first, m, coef);
+    else if (di == FPEMU_F16) clip_chunk<FPEMU_F16, FPEMU_F32>(in, out, first, m, coef);
+    else if (dout == FPEMU_BF16) clip_chunk<FPEMU_BF16, FPEMU_BF16>(in, out, first, m, coef);
+    else clip_chunk<FPEMU_BF16, FPEMU_F32>(in, out, first, m, coef);
   }
 }
 
@@ -704,7 +844,7 @@ int check_grads(const char *who, const fpemu_grad_t *grads, uint64_t count, int 
   for (uint64_t i = 0; i < count; i++) {
     const fpemu_grad_t &g = grads[i];
     if (g.in_dtype < FPEMU_F32 || g.in_dtype > FPEMU_BF16) return fail(FPEMU_EINVAL, who, "bad dtype id");
-    if (g.n > ((uint64_t)1 << 45)) return fail(FPEMU_EINVAL, who, "more than 2^45 elements in one tensor");
+    if (g.n > ((uint64_t)1 << 40)) return fail(FPEMU_EINVAL, who, "more than 2^40 elements in one tensor");
     if (g.n == 0) continue;
     if (g.in == nullptr) return fail(FPEMU_EINVAL, who, "null buffer");
     if ((uintptr_t)g.in % elem_size(g.in_dtype)) return fail(FPEMU_EALIGN, who, "buffer not aligned to its element size");
@@ -721,22 +861,28 @@ int check_grads(const char *who, const fpemu_grad_t *grads, uint64_t count, int 
   return FPEMU_OK;
 }
 
-// the next launch's table, from grads[at]; returns where the one after begins
+// the next launch's table, from grads[at]; returns where the one after begins.  Steps of 8192 to 65536 elements: some
+// thousand for the whole list, so that short lists use every CU and long ones look their tensors up rarely.
 uint64_t fill_table(const fpemu_grad_t *grads, uint64_t count, uint64_t at, GradTable &tab, uint64_t &chunks) {
   tab.count = 0;
-  chunks = 0;
+  uint64_t elems = 0;
   for (; at < count && tab.count < kGrads; at++) {
     if (grads[at].n == 0) continue;
-    const uint64_t c = ceil_div(grads[at].n, kGradChunk);
-    if (chunks + c > 0xFFFFFFFFull) break;
-    chunks += c;
     const int i = tab.count++;
     tab.in[i] = grads[at].in;
     tab.out[i] = grads[at].out;
     tab.n[i] = grads[at].n;
-    tab.end[i] = (uint32_t)chunks;
     tab.in_dt[i] = (uint8_t)grads[at].in_dtype;
     tab.out_dt[i] = (uint8_t)grads[at].out_dtype;
+    elems += grads[at].n;
+  }
+  tab.chunk = 8192;
+  while (tab.chunk < 65536 && elems / tab.chunk > 4096) tab.chunk *= 2;
+  while (elems / tab.chunk > 0x3FFFFFFFull) tab.chunk *= 2;
+  chunks = 0;
+  for (int i = 0; i < tab.count; i++) {
+    chunks += ceil_div(tab.n[i], tab.chunk);
+    tab.end[i] = (uint32_t)chunks;
   }
   return at;
 }
@@ -747,7 +893,7 @@ extern "C" {
 
 uint64_t fpemu_group_rows_workspace_bytes(uint64_t n, uint64_t groups) {
   if (n > 0x7FFFFFFFull || groups < 1 || groups > 0x7FFFFFFEull) return 0;
-  return 4u * sort_space(n, groups).words;
+  return 4u * sort_space(n, groups, false).words;
 }
 
 int fpemu_group_rows(const void *ids, int id_bytes, uint64_t n, uint64_t groups, int32_t *order, int32_t *offsets, void *ws,
@@ -759,7 +905,7 @@ int fpemu_group_rows(const void *ids, int id_bytes, uint64_t n, uint64_t groups,
   if (need > 0 && (ws == nullptr || ws_bytes < need)) return fail(FPEMU_EINVAL, who, "workspace too small");
   if ((uintptr_t)ws % 16u || (uintptr_t)order % 4u || (uintptr_t)offsets % 4u)
     return fail(FPEMU_EALIGN, who, "workspace (16 bytes) or output (4 bytes) not aligned");
-  return sort_rows(who, ids, id_bytes == 8, n, groups, order, offsets, (uint32_t *)ws, (hipStream_t)stream);
+  return sort_rows(who, ids, id_bytes == 8, n, groups, order, offsets, false, (uint32_t *)ws, Fill{}, (hipStream_t)stream);
 }
 
 static int check_embedding(const char *who, const void *a, const void *b, uint64_t n, uint64_t width, int dtype) {
@@ -781,18 +927,20 @@ int fpemu_embedding(const void *weight, const void *ids, int id_bytes, void *out
   const uint64_t vecs = ceil_div(width, vec_elems(dtype));
   int lg = 0;
   while (lg < 8 && ((uint64_t)1 << lg) < vecs) lg++;
-  const unsigned blocks = (unsigned)ceil_div(n, 256u >> lg);
-  const int wide = id_bytes == 8;
+  const uint64_t rows = 256u >> lg;   // of a workgroup, times 1 or 4: four only where enough workgroups are left
+  const bool four = n >= rows * 4 * 1024;
+  const unsigned blocks = (unsigned)ceil_div(n, four ? rows * 4 : rows);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == FPEMU_F32) embedding_kernel<FPEMU_F32><<<blocks, 256, 0, s>>>(weight, ids, wide, out, n, vocab, width, scale, lg);
-  else if (dtype == FPEMU_F16) embedding_kernel<FPEMU_F16><<<blocks, 256, 0, s>>>(weight, ids, wide, out, n, vocab, width, scale, lg);
-  else embedding_kernel<FPEMU_BF16><<<blocks, 256, 0, s>>>(weight, ids, wide, out, n, vocab, width, scale, lg);
+  auto go = [&](auto kernel) { kernel<<<blocks, 256, 0, s>>>(weight, ids, id_bytes == 8, out, n, vocab, width, scale, lg); };
+  if (dtype == FPEMU_F32) four ? go(embedding_kernel<FPEMU_F32, 4>) : go(embedding_kernel<FPEMU_F32, 1>);
+  else if (dtype == FPEMU_F16) four ? go(embedding_kernel<FPEMU_F16, 4>) : go(embedding_kernel<FPEMU_F16, 1>);
+  else four ? go(embedding_kernel<FPEMU_BF16, 4>) : go(embedding_kernel<FPEMU_BF16, 1>);
   return launched(who);
 }
 
-// words before the chunk sums: the sort's, the order, the offsets
+// words before the chunk sums: the sort's and the order
 static uint64_t embedding_words(uint64_t n, uint64_t vocab) {
-  const uint64_t words = sort_space(n, vocab).words + n + vocab + 1;
+  const uint64_t words = sort_space(n, vocab, true).words + n;
   return (words + 3) / 4 * 4;
 }
 
@@ -807,24 +955,28 @@ int fpemu_embedding_grad(const void *dout, const void *ids, int id_bytes, void *
   if (const int rc = check_ids(who, ids, id_bytes, n, vocab)) return rc;
   if (const int rc = check_embedding(who, dweight, dout, n, width, dtype)) return rc;
   if (width == 0) return FPEMU_OK;
-  if (ws == nullptr || ws_bytes < fpemu_embedding_grad_workspace_bytes(n, vocab, width))
+  if (n > 0 && (ws == nullptr || ws_bytes < fpemu_embedding_grad_workspace_bytes(n, vocab, width)))
     return fail(FPEMU_EINVAL, who, "workspace too small");
   if ((uintptr_t)ws % 16u) return fail(FPEMU_EALIGN, who, "workspace not aligned to 16 bytes");
-  const int wide = id_bytes == 8;
+  const uint64_t cols = ceil_div(width, 64u * vec_elems(dtype));
+  if (cols > 65535u) return fail(FPEMU_EINVAL, who, "table too wide for one launch");
+  const uint64_t bytes = vocab * width * elem_size(dtype);
+  if (ceil_div(bytes, kFillPiece) > 0x7FFFFFFFull) return fail(FPEMU_EINVAL, who, "table too large for one launch");
   hipStream_t s = (hipStream_t)stream;
   uint32_t *words = (uint32_t *)ws;
-  int32_t *order = (int32_t *)(words + sort_space(n, vocab).words), *offsets = order + n;
+  const SortSpace sp = sort_space(n, vocab, true);
+  int32_t *order = (int32_t *)(words + sp.words);
   float *sums = (float *)(words + embedding_words(n, vocab));
-  if (const int rc = sort_rows(who, ids, wide, n, vocab, order, offsets, words, s)) return rc;
+  if (const int rc = sort_rows(who, ids, id_bytes == 8, n, vocab, order, nullptr, true, words, Fill{(char *)dweight, bytes, 0, 0}, s)) return rc;
+  if (n == 0) return FPEMU_OK;
   const uint32_t chunk = chunk_of(n);
-  const unsigned cols = (unsigned)ceil_div(width, 64u * vec_elems(dtype));
-  if (cols > 65535u || vocab > 0x7FFFFFFFull) return fail(FPEMU_EINVAL, who, "table too wide for one launch");
-  const dim3 cgrid((unsigned)(n / chunk), cols), rgrid((unsigned)ceil_div(vocab, 4), cols);
+  const Tokens t{dout, words + sp.keys, order, (uint32_t)n, (uint32_t)vocab, padding >= 0 && (uint64_t)padding < vocab ? (uint32_t)padding : 0xFFFFFFFFu,
+                 chunk, width};
+  const dim3 grid((unsigned)ceil_div(ceil_div(n, chunk), 4), (unsigned)cols);
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (cgrid.x > 0)
-      embedding_chunks_kernel<DT><<<cgrid, 64, 0, s>>>(dout, ids, wide, order, (uint32_t)n, width, chunk, sums);
-    embedding_rows_kernel<DT><<<rgrid, 256, 0, s>>>(dout, order, offsets, sums, dweight, vocab, width, chunk, scale, padding);
+    if (n > chunk) embedding_chunks_kernel<DT><<<grid, 256, 0, s>>>(t, sums);
+    embedding_runs_kernel<DT><<<grid, 256, 0, s>>>(t, sums, dweight, scale);
   };
   if (dtype == FPEMU_F32) go(std::integral_constant<int, FPEMU_F32>());
   else if (dtype == FPEMU_F16) go(std::integral_constant<int, FPEMU_F16>());
