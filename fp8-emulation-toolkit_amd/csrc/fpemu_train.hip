@@ -533,7 +533,9 @@ __global__ __launch_bounds__(256) void embedding_kernel(const void *weight, cons
 // chunks.  A wave takes the runs (tokens of one entry) that begin in its chunk, to their ends, and writes their rows; a chunk
 // that an earlier run fills is summed by a wave of its own first (a frequent token's run is long: its chunks go to many
 // waves), so behind its own chunk a run is a list of chunk sums and the tokens of the chunk that it ends in.
-// 64 lanes take 16 bytes of the row each; a wave loads the rows of eight tokens before it adds the first.
+// 64 lanes take 16 bytes of the row each; a wave loads the rows of eight tokens before it adds the first.  In a row that is
+// not whole vectors the last lane's vector begins earlier and shares columns with its neighbour's, which writes the same
+// values there; only rows shorter than a vector (WHOLE false) go element by element.
 constexpr uint32_t kSub = 16;    // positions looked at together: their keys and tokens lie in the wave's lanes
 constexpr int kRows = 8;
 
@@ -560,74 +562,97 @@ struct Look {
   }
 };
 
-// adds the rows of the positions in `take` of one look, in order; flush(j) runs before position j of `at` is added
-template <int DT, class F>
-__device__ __forceinline__ void add_rows(const Tokens &t, const Look &look, uint32_t take, uint64_t c, float (&acc)[Elems<DT>::V], F &&flush) {
+// V columns of a row from c on
+template <int DT, bool WHOLE> struct Columns {
+  using E = Elems<DT>;
+  uint64_t c;      // the lane's first column
+  bool mine;       // lanes behind the row's end do column 0's work and store nothing
+  __device__ __forceinline__ explicit Columns(uint64_t width) {
+    c = ((uint64_t)blockIdx.y * 64u + (threadIdx.x & 63u)) * E::V;
+    mine = c < width;
+    if (!mine) c = 0;
+    else if (WHOLE && c + E::V > width) c = width - E::V;
+  }
+  __device__ __forceinline__ u32x4 load(const typename E::elem *row, uint64_t width) const {
+    if constexpr (WHOLE) return *(const vec_a2 *)(row + c);
+    typename E::elem e[E::V];
+#pragma unroll
+    for (int j = 0; j < E::V; j++) e[j] = c + j < width ? row[c + j] : (typename E::elem)0;
+    return __builtin_bit_cast(u32x4, e);
+  }
+  __device__ __forceinline__ void store(typename E::elem *row, uint64_t width, const float (&f)[E::V]) const {
+    if constexpr (WHOLE) *(vec_a2 *)(row + c) = E::pack(f);
+    else store_cols<DT>(row, c, width, f);
+  }
+  // fp32 sums of the same columns
+  __device__ __forceinline__ void load_sum(const float *row, uint64_t width, float (&f)[E::V]) const {
+#pragma unroll
+    for (int j = 0; j < E::V; j++) f[j] = WHOLE || c + j < width ? row[c + j] : 0.f;
+  }
+  __device__ __forceinline__ void store_sum(float *row, uint64_t width, const float (&f)[E::V]) const {
+#pragma unroll
+    for (int j = 0; j < E::V; j++)
+      if (WHOLE || c + j < width) row[c + j] = f[j];
+  }
+};
+
+// adds the rows of the positions in `take` of one look, in order; flush(j) runs before position j is added
+template <int DT, bool WHOLE, class F>
+__device__ __forceinline__ void add_rows(const Tokens &t, const Look &look, uint32_t take, const Columns<DT, WHOLE> &at,
+                                         float (&acc)[Elems<DT>::V], F &&flush) {
   using E = Elems<DT>;
 #pragma unroll
   for (uint32_t j0 = 0; j0 < kSub; j0 += kRows) {
     if (!((take | look.starts) >> j0 & ((1u << kRows) - 1u))) continue;
-    float f[kRows][E::V];
+    u32x4 v[kRows];
 #pragma unroll
     for (uint32_t u = 0; u < kRows; u++) {   // positions that are not taken load row 0 and are not added
       const uint32_t row = (take >> (j0 + u)) & 1u ? (uint32_t)__builtin_amdgcn_readlane((int)look.pos, (int)(j0 + u)) : 0u;
-      load_cols<DT>((const typename E::elem *)t.dout + (uint64_t)row * t.width, c, t.width, f[u]);
+      v[u] = at.load((const typename E::elem *)t.dout + (uint64_t)row * t.width, t.width);
     }
 #pragma unroll
     for (uint32_t u = 0; u < kRows; u++) {
       flush(j0 + u);
       if ((take >> (j0 + u)) & 1u) {
+        float f[E::V];
+        E::unpack(v[u], f);
 #pragma unroll
-        for (int e = 0; e < E::V; e++) acc[e] += f[u][e];
+        for (int e = 0; e < E::V; e++) acc[e] += f[e];
       }
     }
   }
 }
 
-// the lane's first column; lanes behind the row's end do column 0's work and store nothing
-template <int DT> __device__ __forceinline__ uint64_t column(uint64_t width, bool &mine) {
-  const uint64_t c = ((uint64_t)blockIdx.y * 64u + (threadIdx.x & 63u)) * Elems<DT>::V;
-  mine = c < width;
-  return mine ? c : 0;
-}
-
-template <int DT> __global__ __launch_bounds__(256) void embedding_chunks_kernel(Tokens t, float *sums) {
-  using E = Elems<DT>;
+template <int DT, bool WHOLE> __global__ __launch_bounds__(256) void embedding_chunks_kernel(Tokens t, float *sums) {
   const uint32_t chunk = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint64_t first = (uint64_t)chunk * t.chunk;
   if (first == 0 || first + t.chunk > t.n) return;
   const uint32_t key = t.keys[first - 1];
   if (key != t.keys[first + t.chunk - 1] || key >= t.vocab || key == t.padding) return;   // not inside one run
-  bool mine;
-  const uint64_t c = column<DT>(t.width, mine);
-  float acc[E::V] = {};
+  const Columns<DT, WHOLE> at(t.width);
+  float acc[Elems<DT>::V] = {};
   for (uint32_t base = 0; base < t.chunk; base += kSub) {
     const Look look(t, (uint32_t)first + base);
-    add_rows<DT>(t, look, look.there, c, acc, [](uint32_t) {});
+    add_rows<DT, WHOLE>(t, look, look.there, at, acc, [](uint32_t) {});
   }
-  if (mine) {
-    float *row = sums + (uint64_t)chunk * t.width;
-#pragma unroll
-    for (int j = 0; j < E::V; j++)
-      if (c + j < t.width) row[c + j] = acc[j];
-  }
+  if (at.mine) at.store_sum(sums + (uint64_t)chunk * t.width, t.width, acc);
 }
 
-template <int DT> __global__ __launch_bounds__(256) void embedding_runs_kernel(Tokens t, const float *sums, void *dweight, float scale) {
+template <int DT, bool WHOLE>
+__global__ __launch_bounds__(256) void embedding_runs_kernel(Tokens t, const float *sums, void *dweight, float scale) {
   using E = Elems<DT>;
   const uint64_t first = (uint64_t)(blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * t.chunk;
   if (first >= t.n) return;
-  bool mine;
-  const uint64_t c = column<DT>(t.width, mine);
+  const Columns<DT, WHOLE> at(t.width);
   float acc[E::V] = {};
   bool open = false;      // a run of this chunk is being added up
   uint32_t entry = 0;
   auto close = [&]() {
-    if (open && mine) {
+    if (open && at.mine) {
       float out[E::V];
 #pragma unroll
       for (int j = 0; j < E::V; j++) out[j] = acc[j] * scale;
-      store_cols<DT>((typename E::elem *)dweight + (uint64_t)entry * t.width, c, t.width, out);
+      at.store((typename E::elem *)dweight + (uint64_t)entry * t.width, t.width, out);
     }
 #pragma unroll
     for (int j = 0; j < E::V; j++) acc[j] = 0.f;
@@ -636,31 +661,41 @@ template <int DT> __global__ __launch_bounds__(256) void embedding_runs_kernel(T
     const Look look(t, (uint32_t)(first + base));
     // positions before the first run that begins here belong to an earlier chunk's, unless one of ours is open
     const uint32_t ours = open ? ~0u : look.starts ? ~((look.starts & (0u - look.starts)) - 1u) : 0u;
-    add_rows<DT>(t, look, look.counts & ours, c, acc, [&](uint32_t j) {
+    add_rows<DT, WHOLE>(t, look, look.counts & ours, at, acc, [&](uint32_t j) {
       if (!((look.starts >> j) & 1u)) return;
       close();
       open = (look.counts >> j) & 1u;
       entry = (uint32_t)__builtin_amdgcn_readlane((int)look.key, (int)j);
     });
   }
-  for (uint64_t at = first + t.chunk; open && at < t.n; at += t.chunk) {   // the last run goes on
-    if (t.keys[at] != entry) break;
-    if (at + t.chunk <= t.n && t.keys[at + t.chunk - 1] == entry) {
-      const float *row = sums + at / t.chunk * t.width;
+  // The last run goes on: 64 chunks at a time, a lane asks of each whether the run fills it; their sums, eight loads at once.
+  uint64_t next = first + t.chunk;
+  bool filled = open;
+  while (filled && next < t.n) {
+    const uint64_t mine = next + (uint64_t)(threadIdx.x & 63u) * t.chunk;
+    const uint64_t fills = __ballot(mine + t.chunk <= t.n && t.keys[mine + t.chunk - 1] == entry);   // sorted: so is all before it
+    const int count = ~fills ? __ffsll((unsigned long long)~fills) - 1 : 64;
+    const float *row = sums + next / t.chunk * t.width;
+    for (int i = 0; i < count; i += kRows) {
+      float f[kRows][E::V];
 #pragma unroll
-      for (int j = 0; j < E::V; j++)
-        if (c + j < t.width) acc[j] += row[c + j];
-      continue;
+      for (int u = 0; u < kRows; u++) at.load_sum(row + (uint64_t)(i + u < count ? i + u : i) * t.width, t.width, f[u]);
+#pragma unroll
+      for (int u = 0; u < kRows; u++)
+        if (i + u < count) {
+#pragma unroll
+          for (int e = 0; e < E::V; e++) acc[e] += f[u][e];
+        }
     }
-    for (uint32_t base = 0; base < t.chunk && at + base < t.n; base += kSub) {
-      const Look look(t, (uint32_t)(at + base));
-      const uint32_t same = (uint32_t)__ballot(look.key == entry) & look.there;
-      if (!same) break;
-      Look rest = look;
-      rest.starts = 0;
-      add_rows<DT>(t, rest, same, c, acc, [](uint32_t) {});
-    }
-    break;
+    next += (uint64_t)count * t.chunk;
+    filled = count == 64;
+  }
+  for (uint64_t end = next + t.chunk; open && next < t.n && next < end; next += kSub) {   // and the chunk that it ends in
+    Look look(t, (uint32_t)next);
+    const uint32_t same = (uint32_t)__ballot(look.key == entry) & look.there;
+    if (!same) break;
+    look.starts = 0;
+    add_rows<DT, WHOLE>(t, look, same, at, acc, [](uint32_t) {});
   }
   close();
 }
@@ -975,8 +1010,13 @@ int fpemu_embedding_grad(const void *dout, const void *ids, int id_bytes, void *
   const dim3 grid((unsigned)ceil_div(ceil_div(n, chunk), 4), (unsigned)cols);
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (n > chunk) embedding_chunks_kernel<DT><<<grid, 256, 0, s>>>(t, sums);
-    embedding_runs_kernel<DT><<<grid, 256, 0, s>>>(t, sums, dweight, scale);
+    const bool whole = width >= (uint64_t)Elems<DT>::V;
+    if (n > chunk) {
+      if (whole) embedding_chunks_kernel<DT, true><<<grid, 256, 0, s>>>(t, sums);
+      else embedding_chunks_kernel<DT, false><<<grid, 256, 0, s>>>(t, sums);
+    }
+    if (whole) embedding_runs_kernel<DT, true><<<grid, 256, 0, s>>>(t, sums, dweight, scale);
+    else embedding_runs_kernel<DT, false><<<grid, 256, 0, s>>>(t, sums, dweight, scale);
   };
   if (dtype == FPEMU_F32) go(std::integral_constant<int, FPEMU_F32>());
   else if (dtype == FPEMU_F16) go(std::integral_constant<int, FPEMU_F16>());

@@ -321,6 +321,18 @@ at::Tensor grouped_mm(const at::Tensor &x_in, const at::Tensor &weight, const at
   return grouped_impl(x, w, offsets, trans);
 }
 
+// What _gradients() of mpemu.functional checks, here for the whole list at once.
+void check_grads(const char *who, const std::vector<at::Tensor> &ts, const char *what) {
+  for (const at::Tensor &t : ts) {
+    TORCH_CHECK_TYPE(!t.is_sparse(), who, ": sparse gradients are not supported");
+    const auto k = t.scalar_type();
+    TORCH_CHECK_TYPE(k == at::kFloat || k == at::kHalf || k == at::kBFloat16, who, ": ", what,
+                     " must be a float32, float16 or bfloat16 tensor");
+    TORCH_CHECK(t.is_cuda(), who, ": tensors must live on a ROCm device (got ", t.device(), "); this build has no CPU path");
+    TORCH_CHECK_VALUE(t.device() == ts[0].device(), who, ": tensors on different devices (", ts[0].device(), ", ", t.device(), ")");
+  }
+}
+
 // the elements of a gradient as one run of memory, in whatever order: itself where it is one, else a copy
 std::vector<at::Tensor> dense_list(const std::vector<at::Tensor> &ts) {
   std::vector<at::Tensor> d;
@@ -366,6 +378,7 @@ at::Tensor norm_of(const std::vector<fpemu_grad_t> &tab, int64_t order, const at
 }
 
 at::Tensor grad_norm(const std::vector<at::Tensor> &grads, int64_t order) {
+  check_grads("grad_norm", grads, "a gradient");
   const std::vector<at::Tensor> dense = dense_list(grads);
   const OnStream on(grads[0]);
   at::Tensor sum = at::empty({1}, grads[0].options().dtype(at::kDouble));
@@ -374,9 +387,19 @@ at::Tensor grad_norm(const std::vector<at::Tensor> &grads, int64_t order) {
   return norm;
 }
 
-at::Tensor clip_grads(const std::vector<at::Tensor> &grads, const std::vector<at::Tensor> &outs, double max_norm, int64_t order,
-                      bool finite_only) {
+at::Tensor clip_grads(const std::vector<at::Tensor> &grads, const c10::optional<std::vector<at::Tensor>> &outs_or_none, double max_norm,
+                      int64_t order, bool finite_only) {
   at::NoGradGuard no_grad;
+  check_grads("clip_grads_", grads, "a gradient");
+  const std::vector<at::Tensor> &outs = outs_or_none.has_value() ? *outs_or_none : grads;
+  if (outs_or_none.has_value()) {
+    TORCH_CHECK_VALUE(outs.size() == grads.size(), "clip_grads_: ", grads.size(), " gradients but ", outs.size(), " outputs");
+    check_grads("clip_grads_", outs, "an output");
+    for (size_t i = 0; i < grads.size(); i++)
+      TORCH_CHECK_VALUE(outs[i].sizes() == grads[i].sizes() && outs[i].strides() == grads[i].strides() && outs[i].device() == grads[i].device() &&
+                            (outs[i].scalar_type() == grads[i].scalar_type() || outs[i].scalar_type() == at::kFloat),
+                        "clip_grads_: an output needs its gradient's shape, strides and device, and its type or float32");
+  }
   const std::vector<at::Tensor> dense = dense_list(grads);
   std::vector<at::Tensor> to;
   to.reserve(grads.size());
@@ -419,6 +442,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding", &embedding, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("padding"));
   m.def("grouped_mm", &grouped_mm, py::arg("x"), py::arg("weight"), py::arg("offsets"));
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("order"));
-  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("outs"), py::arg("max_norm"), py::arg("order"),
+  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("outs").none(true), py::arg("max_norm"), py::arg("order"),
         py::arg("finite_only"));
 }

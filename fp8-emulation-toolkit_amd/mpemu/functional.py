@@ -197,14 +197,16 @@ def _order(norm_type, who):
     return order
 
 
-def _gradients(grads, who):
-    grads = [grads] if torch.is_tensor(grads) else list(grads)
+def _list(grads):
+    return [grads] if torch.is_tensor(grads) else list(grads)
+
+
+def _check_gradients(grads, who, what="a gradient"):
     for g in grads:
         if torch.is_tensor(g) and g.is_sparse:
             raise TypeError("%s: sparse gradients are not supported" % who)
-        _floating(g, "a gradient", who)
+        _floating(g, what, who)
     _one_device(who, *grads)
-    return grads
 
 
 def _dense(t):
@@ -236,12 +238,13 @@ def grad_norm(grads, norm_type=2.0):
     in 64 bits, so neither large nor many elements overflow or drown it."""
     who = "grad_norm"
     order = _order(norm_type, who)
-    grads = _gradients(grads, who)
+    grads = _list(grads)
     if not grads:
         return torch.tensor(0.0)
     ext = _native()
-    if ext is not None:
+    if ext is not None and all(torch.is_tensor(g) for g in grads):
         return ext.grad_norm(grads, order)
+    _check_gradients(grads, who)
     dense = [_dense(g) for g in grads]
     total = torch.empty(1, dtype=torch.float64, device=grads[0].device)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
@@ -260,23 +263,24 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
     with every gradient as it was."""
     who = "clip_grads_"
     order = _order(norm_type, who)
-    grads = _gradients(grads, who)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("clip_grads_: max_norm must not be negative or NaN, got %r" % max_norm)
-    if out is not None:
-        out = [out] if torch.is_tensor(out) else list(out)
-        if len(out) != len(grads):
-            raise ValueError("clip_grads_: %d gradients but %d outputs" % (len(grads), len(out)))
-        for g, o in zip(grads, out):
-            _floating(o, "an output", who)
-            if o.shape != g.shape or o.stride() != g.stride() or o.device != g.device or o.dtype not in (g.dtype, torch.float32):
-                raise ValueError("clip_grads_: an output needs its gradient's shape, strides and device, and its type or float32")
+    grads = _list(grads)
+    out = None if out is None else _list(out)
+    if out is not None and len(out) != len(grads):
+        raise ValueError("clip_grads_: %d gradients but %d outputs" % (len(grads), len(out)))
     if not grads:
         return torch.tensor(0.0)
     ext = _native()
-    if ext is not None:
-        return ext.clip_grads(grads, out if out is not None else grads, max_norm, order, bool(error_if_nonfinite))
+    if ext is not None and all(torch.is_tensor(t) for t in grads + (out or [])):
+        return ext.clip_grads(grads, out, max_norm, order, bool(error_if_nonfinite))
+    _check_gradients(grads, who)
+    if out is not None:
+        _check_gradients(out, who, "an output")
+        for g, o in zip(grads, out):
+            if o.shape != g.shape or o.stride() != g.stride() or o.device != g.device or o.dtype not in (g.dtype, torch.float32):
+                raise ValueError("clip_grads_: an output needs its gradient's shape, strides and device, and its type or float32")
     dense = [_dense(g) for g in grads]
     if out is None:
         outs = dense
