@@ -120,8 +120,9 @@ __device__ __forceinline__ void banded(uint32_t id, uint32_t row_tiles, uint32_t
 }
 
 // ---- any storage, sizes and alignment: tiles staged through registers ----------------------------------------------------------------
-// fp32 is bound by its matrix instructions (64 cycles each, 512 of them a stage), so a plain double buffer feeds it: the next
-// stage's vectors are loaded into registers, the current one is multiplied, then they are written to the other LDS buffer.
+// fp32 is bound by its matrix instructions (64 cycles each), so staging through registers feeds it: the vectors of the next two
+// stages are on their way to registers while the current one is multiplied; then the next one is written to the other LDS
+// buffer.
 // The same kernel takes 16-bit operands whose rows are not whole 16-byte vectors: global loads need no more than element
 // alignment, and vectors that reach over an edge are put together element by element.
 // A stage is 128 bytes deep in k (64 16-bit or 32 fp32 elements).  LDS holds it as described for the tiles further down.
@@ -145,7 +146,7 @@ template <int DT, bool COL, int EXT> struct Staged {
   int64_t ld, step;
   int lim;            // entries of the tile
   elem pad;           // what a load behind the contraction yields
-  u32x4 v[LOADS];
+  u32x4 v[2][LOADS];  // two stages
 
   __device__ __forceinline__ void set(const elem *p, int64_t ld_, int lim_, elem pad_) {
     base = p;
@@ -165,29 +166,35 @@ template <int DT, bool COL, int EXT> struct Staged {
       k = ((id & 7) ^ swizzle_row(outer)) * V;
     }
   }
+  // every vector of a whole stage is whole
+  __device__ __forceinline__ bool plain() const { return !COL || lim >= EXT; }
   // the next stage, of which `left` k are there
-  __device__ __forceinline__ void load(int64_t left) {
+  template <bool PLAIN> __device__ __forceinline__ void load(int set, int64_t left) {
 #pragma unroll
     for (int j = 0; j < LOADS; j++) {
       int outer, k;
       place(j, outer, k);
-      const int r = outer < lim ? outer : lim - 1;   // entries beyond the tile's only feed results that are not stored
-      const elem *p = COL ? base + k * ld + r : base + r * ld + k;
-      const int have = COL ? (k < left ? (lim - r < V ? lim - r : V) : 0) : left - k >= V ? V : (int)(left - k);
-      if (have >= V) {
-        v[j] = *(const vec_any *)p;
+      const int r = PLAIN && COL ? outer : outer < lim ? outer : lim - 1;   // entries beyond the tile's only feed results that
+      const elem *p = COL ? base + k * ld + r : base + r * ld + k;          // are not stored
+      if constexpr (PLAIN) {
+        v[set][j] = *(const vec_any *)p;
       } else {
-        elem e[V];
+        const int have = COL ? (k < left ? (lim - r < V ? lim - r : V) : 0) : left - k >= V ? V : (int)(left - k);
+        if (have >= V) {
+          v[set][j] = *(const vec_any *)p;
+        } else {
+          elem e[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) e[i] = i < have ? p[i] : pad;
-        __builtin_memcpy(&v[j], e, 16);
+          for (int i = 0; i < V; i++) e[i] = i < have ? p[i] : pad;
+          __builtin_memcpy(&v[set][j], e, 16);
+        }
       }
     }
     base += step;
   }
-  __device__ __forceinline__ void put(char *lds) const {
+  __device__ __forceinline__ void put(char *lds, int set) const {
 #pragma unroll
-    for (int j = 0; j < LOADS; j++) *(u32x4 *)(lds + (j * 256 + (int)threadIdx.x) * 16) = v[j];
+    for (int j = 0; j < LOADS; j++) *(u32x4 *)(lds + (j * 256 + (int)threadIdx.x) * 16) = v[set][j];
   }
   // 16-bit: a matrix operand of 32 entries from `at`, k-step of 16.  fp32: the operands of two matrix instructions, k-step of
   // 4: the k of lane half h are 0 + h and 2 + h, a row's four come as one vector and pick() takes the lane's two.
@@ -246,16 +253,7 @@ __device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL, S::BM>
   constexpr int STEPS = DT == FPEMU_F32 ? SA::FK / 4 : SA::FK / 16, STAGE = SA::BYTES + SB::BYTES;
   const int wr = S::row(), wc = S::col();
   char *now = smem, *then = smem + STAGE;
-  a.load(k);
-  b.load(k);
-  a.put(now);
-  b.put(now + SA::BYTES);
-  __syncthreads();
-  for (int64_t left = k; left > 0; left -= SA::FK) {
-    if (left > SA::FK) {
-      a.load(left - SA::FK);
-      b.load(left - SA::FK);
-    }
+  auto multiply = [&]() {
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
       u32x4 av[S::TM], bv[S::TN];
@@ -278,14 +276,39 @@ __device__ __forceinline__ void any_product(char *smem, Staged<DT, A_COL, S::BM>
           for (int j = 0; j < S::TN; j++) acc[i][j] = mfma16<DT>(av[i], bv[j], acc[i][j]);
       }
     }
+  };
+  auto load = [&](auto plain, int set, int64_t left) {
+    a.template load<decltype(plain)::value>(set, left);
+    b.template load<decltype(plain)::value>(set, left);
+  };
+  // one stage: `set` holds the next one, the one after it is loaded into the other set
+  auto stage = [&](auto plain, int set, int64_t left) {
+    if (decltype(plain)::value || left > 2 * SA::FK) load(plain, set ^ 1, left - 2 * SA::FK);
+    multiply();
     if (left > SA::FK) {
-      a.put(then);
-      b.put(then + SA::BYTES);
+      a.put(then, set);
+      b.put(then + SA::BYTES, set);
     }
     __syncthreads();
     char *t = now;
     now = then;
     then = t;
+  };
+  load(std::false_type(), 0, k);
+  if (k > SA::FK) load(std::false_type(), 1, k - SA::FK);
+  a.put(now, 0);
+  b.put(now + SA::BYTES, 0);
+  __syncthreads();
+  int64_t left = k;
+  if (a.plain() && b.plain()) {
+    for (; left >= 4 * SA::FK; left -= 2 * SA::FK) {   // the stages two and three ahead are whole
+      stage(std::true_type(), 1, left);
+      stage(std::true_type(), 0, left - SA::FK);
+    }
+  }
+  for (; left > 0; left -= 2 * SA::FK) {
+    stage(std::false_type(), 1, left);
+    if (left > SA::FK) stage(std::false_type(), 0, left - SA::FK);
   }
 }
 

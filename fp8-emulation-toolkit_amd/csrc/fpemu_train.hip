@@ -702,7 +702,7 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(Tokens t, const flo
 
 uint32_t chunk_of(uint64_t n) {
   uint32_t c = kSub;
-  while ((uint64_t)c * 1024u < n) c *= 2u;   // at most 1024 chunk sums for one entry
+  while ((uint64_t)c * 4096u < n) c *= 2u;   // at most 4096 chunk sums for one entry
   return c;
 }
 
@@ -756,6 +756,23 @@ template <int ORDER, int DT> __device__ __forceinline__ double norm_chunk(const 
   auto add = [&](u32x4 v) {
     float f[E::V];
     E::unpack(v, f);
+    if constexpr (ORDER == FPEMU_NORM_2 && DT != FPEMU_F32) {
+      // squares of 16-bit values are exact in fp32; four of them are added there (two roundings at most, 2^-24 each)
+      // before 64 bits take over.  bf16 squares outside fp32's range go one by one.
+      float q[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const float *g = f + 4 * h;
+        q[h] = __builtin_fmaf(g[0], g[0], g[1] * g[1]) + __builtin_fmaf(g[2], g[2], g[3] * g[3]);
+      }
+      const float low = q[0] < q[1] ? q[0] : q[1], all = q[0] + q[1];
+      const bool zeros = ((v[0] | v[1] | v[2] | v[3]) & 0x7FFF7FFFu) == 0;
+      if (DT == FPEMU_F16 || zeros || (low > 0x1p-90f && all < 0x1p126f)) {
+        a[0] += (double)q[0];
+        a[1] += (double)q[1];
+        return;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < E::V; j++) a[j & 3] = norm_add<ORDER>(a[j & 3], f[j]);
   };
@@ -813,33 +830,44 @@ template <int ORDER> __global__ __launch_bounds__(1024) void norm_finish_kernel(
   if (threadIdx.x == 0) *sum = all;
 }
 
+// Every store of a wave is one run of 1 KB: 16 bytes a lane on the output's side, which is 8 on the side of 16-bit gradients
+// that become fp32 ones.
 template <int DI, int DO> __device__ __forceinline__ void clip_chunk(const void *in, void *out, uint64_t first, uint32_t m, float coef) {
   using E = Elems<DI>;
   using O = Elems<DO>;
+  typedef uint32_t half_a2 __attribute__((ext_vector_type(2), aligned(2)));
+  constexpr int V = O::V;   // elements of a lane's step
   const typename E::elem *p = (const typename E::elem *)in + first;
   typename O::elem *q = (typename O::elem *)out + first;
+  auto get = [&](uint32_t i) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if constexpr (DI == DO) {
+      v = *(const vec_a2 *)(p + i * V);
+    } else {
+      const half_a2 h = *(const half_a2 *)(p + i * V);
+      v[0] = h[0];
+      v[1] = h[1];
+    }
+    return v;
+  };
   auto put = [&](uint32_t i, u32x4 v) {
-    float f[E::V];
+    float f[E::V], g[V];
     E::unpack(v, f);
 #pragma unroll
-    for (int h = 0; h < E::V; h += O::V) {   // 16-bit gradients into fp32 ones: two vectors
-      float g[O::V];
-#pragma unroll
-      for (int j = 0; j < O::V; j++) g[j] = f[h + j] * coef;
-      *(vec_a2 *)(q + i * E::V + h) = O::pack(g);
-    }
+    for (int j = 0; j < V; j++) g[j] = f[j] * coef;
+    __builtin_nontemporal_store((u32x4)O::pack(g), (vec_a2 *)(q + i * V));
   };
-  each_vector<E::V>(
+  each_vector<V>(
       m,
       [&](uint32_t i) {
         u32x4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) v[u] = *(const vec_a2 *)(p + (i + u * 256u) * E::V);
+        for (int u = 0; u < 4; u++) v[u] = get(i + u * 256u);
 #pragma unroll
         for (int u = 0; u < 4; u++) put(i + u * 256u, v[u]);
       },
-      [&](uint32_t i) { put(i, *(const vec_a2 *)(p + i * E::V)); });
-  for (uint32_t i = m / E::V * E::V + threadIdx.x; i < m; i += 256u) O::put(q + i, E::one(p + i) * coef);
+      [&](uint32_t i) { put(i, get(i)); });
+  for (uint32_t i = m / V * V + threadIdx.x; i < m; i += 256u) O::put(q + i, E::one(p + i) * coef);
 }
 
 // coef = min(1, max_norm / (norm + 1e-6)), a NaN norm gives a NaN coefficient.  Gradients that stay in place and keep
@@ -896,8 +924,8 @@ int check_grads(const char *who, const fpemu_grad_t *grads, uint64_t count, int 
   return FPEMU_OK;
 }
 
-// the next launch's table, from grads[at]; returns where the one after begins.  Steps of 8192 to 65536 elements: some
-// thousand for the whole list, so that short lists use every CU and long ones look their tensors up rarely.
+// the next launch's table, from grads[at]; returns where the one after begins.  Steps of 8192 elements, two batches of four
+// loads a thread: 182 M bf16 gradients into fp32 ones take 185 us so, 192 with steps of 16384, 212 with 65536.
 uint64_t fill_table(const fpemu_grad_t *grads, uint64_t count, uint64_t at, GradTable &tab, uint64_t &chunks) {
   tab.count = 0;
   uint64_t elems = 0;
@@ -912,7 +940,6 @@ uint64_t fill_table(const fpemu_grad_t *grads, uint64_t count, uint64_t at, Grad
     elems += grads[at].n;
   }
   tab.chunk = 8192;
-  while (tab.chunk < 65536 && elems / tab.chunk > 4096) tab.chunk *= 2;
   while (elems / tab.chunk > 0x3FFFFFFFull) tab.chunk *= 2;
   chunks = 0;
   for (int i = 0; i < tab.count; i++) {
