@@ -101,13 +101,17 @@ template <int BM> struct TileMap {
   }
 };
 
-// Workgroup b runs on XCD b % 8: each XCD gets an eighth of the tiles, one after the other, so that neighbours share rows of
-// x and a group's weights in its L2.
-constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
+// Workgroup b runs on XCD b % 8.  In one run: each XCD gets an eighth of the tiles, one after the other, so that neighbours
+// share rows of x and a group's weights in its L2.  In turns of TURN tiles: where tiles cost what their group has rows, every
+// XCD gets its part of every group (16 groups, the largest 2.5 times the mean, weight gradient of 2048 x 4096: 362 -> 295 us).
+constexpr uint32_t NO_TILE = 0xFFFFFFFFu, TURN = 8;
 __device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t tiles) {
-  const uint32_t share = (tiles + 7u) / 8u, at = b >> 3;
-  const uint32_t id = (b & 7u) * share + at;
+  const uint32_t share = (tiles + 7u) / 8u, at = b >> 3, id = (b & 7u) * share + at;
   return at < share && id < tiles ? id : NO_TILE;
+}
+__device__ __forceinline__ uint32_t xcd_turn(uint32_t b, uint32_t tiles) {
+  const uint32_t at = b >> 3, id = (at / TURN * 8u + (b & 7u)) * TURN + at % TURN;
+  return id < tiles ? id : NO_TILE;
 }
 
 // Row and column tile of number id: bands of four row tiles, down the band first, so that the tiles an XCD works on at one
@@ -370,7 +374,7 @@ __global__ __launch_bounds__(256, 2) void grouped_wgrad_any_kernel(typename Stor
                                                                    int64_t M, int64_t P, int64_t Q, uint32_t ptiles, uint32_t qtiles,
                                                                    uint32_t tiles) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (S::BM + S::BN) * 128];
-  const uint32_t id = xcd_tile(blockIdx.x, tiles);
+  const uint32_t id = xcd_turn(blockIdx.x, tiles);
   if (id == NO_TILE) return;
   const uint32_t g = id / (ptiles * qtiles);
   uint32_t pt, qt;
@@ -415,8 +419,8 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES_> struct Shape {
   static constexpr int THREADS = WM * WN * 64;
   static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;   // matrix tiles of a wave
   static constexpr int A_BYTES = BM * FK * 2, B_BYTES = BN * FK * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int OUT_LD = BN + 8;   // elements; the finished tile goes through LDS to be stored in whole rows
-  static constexpr int OUT = BM * OUT_LD * 2, LDS = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+  static constexpr int OUT = 32 * TN * 64;   // a wave's 32 finished rows on their way to memory
+  static constexpr int LDS = STAGES * STAGE + WM * WN * OUT;
 };
 
 // One operand's tile: EXT entries (rows of a row operand, columns of a COL operand) x FK of the contraction.
@@ -607,32 +611,6 @@ __device__ __forceinline__ void fast_product(char *smem, Panel<A_COL, S::BM, S::
   };
   if (idle) run(std::false_type());   // the same waits and barriers
   else run(std::true_type());
-  wait_loads<0>();
-  __builtin_amdgcn_s_barrier();   // the stages are free
-}
-
-// The tile through LDS to memory in whole rows; rows < rlim, columns < clim (a multiple of 8).
-template <int DT, class S>
-__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, int wa, int wb,
-                                           const f32x16 (&acc)[S::TM][S::TN]) {
-  const int lane = threadIdx.x & 63;
-  uint16_t *t = (uint16_t *)smem;
-#pragma unroll
-  for (int i = 0; i < S::TM; i++)
-#pragma unroll
-    for (int j = 0; j < S::TN; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int row = wa + i * 32 + (lane & 31), col = wb + j * 32 + (e / 4) * 8 + (lane >> 5) * 4;
-        const uint2 v = {pack_pair16<DT>(acc[i][j][e], acc[i][j][e + 1]), pack_pair16<DT>(acc[i][j][e + 2], acc[i][j][e + 3])};
-        *(uint2 *)(t + row * S::OUT_LD + col) = v;
-      }
-  __syncthreads();
-  constexpr int PER = S::BN / 8;
-  const int col = (threadIdx.x % PER) * 8;
-  if (col < clim)
-    for (int row = threadIdx.x / PER; row < rlim; row += S::THREADS / PER)
-      *(u32x4 *)(c + row * ldc + col) = *(const u32x4 *)(t + row * S::OUT_LD + col);
 }
 
 template <class S> struct WaveAt {   // a wave's part of the tile; waves that share a SIMD (w, w + 4) differ in their rows
@@ -643,6 +621,36 @@ template <class S> struct WaveAt {   // a wave's part of the tile; waves that sh
     wa = (wave / S::WN) * (S::BM / S::WM);
   }
 };
+
+// A wave's part of the finished tile, 32 rows at a time through LDS of its own, to memory in rows of TN * 64 bytes; rows < rlim,
+// columns < clim (a multiple of 8) of the tile.
+template <int DT, class S>
+__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, const WaveAt<S> &at,
+                                           const f32x16 (&acc)[S::TM][S::TN]) {
+  constexpr int PER = S::TN * 4;   // vectors of a row
+  const int lane = threadIdx.x & 63;
+  char *lds = smem + S::STAGES * S::STAGE + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * S::OUT;
+  auto place = [](int row, int vec) { return row * (PER * 16) + ((vec ^ (PER == 8 ? (row >> 1) & 7 : (row >> 2) & 3)) * 16); };
+#pragma unroll
+  for (int i = 0; i < S::TM; i++) {
+#pragma unroll
+    for (int j = 0; j < S::TN; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const uint2 v = {pack_pair16<DT>(acc[i][j][e], acc[i][j][e + 1]), pack_pair16<DT>(acc[i][j][e + 2], acc[i][j][e + 3])};
+        *(uint2 *)(lds + place(lane & 31, j * 4 + e / 4) + (lane >> 5) * 8) = v;
+      }
+    asm volatile("" : : : "memory");   // one wave's LDS operations are in order: its lanes see each other's writes
+#pragma unroll
+    for (int r = 0; r < 32; r += 64 / PER) {
+      const int row = r + lane / PER, vec = lane % PER;
+      const u32x4 v = *(const u32x4 *)(lds + place(row, vec));
+      const int orow = at.wa + i * 32 + row, ocol = at.wb + vec * 8;
+      if (orow < rlim && ocol < clim) *(u32x4 *)(c + orow * ldc + ocol) = v;
+    }
+    asm volatile("" : : : "memory");
+  }
+}
 
 template <int DT, bool W_TRANS, class S>
 __global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, const uint16_t *x, const uint16_t *w, const int32_t *offsets,
@@ -669,7 +677,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, c
     b.set_fragments(at.wb);
     fast_product<DT, S, false, !W_TRANS>(smem, a, b, (int)(K / FK), (int)(K % FK), at.wa >= rows || at.wb >= cols, acc);
   }
-  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, at.wa, at.wb, acc);
+  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, at, acc);
 }
 
 template <int DT, class S>
@@ -677,7 +685,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t
                                                                         const int32_t *offsets, int64_t M, int64_t P, int64_t Q,
                                                                         uint32_t ptiles, uint32_t qtiles, uint32_t tiles) {
   __shared__ __attribute__((aligned(16))) char smem[S::LDS];
-  const uint32_t id = xcd_tile(blockIdx.x, tiles);
+  const uint32_t id = xcd_turn(blockIdx.x, tiles);
   if (id == NO_TILE) return;
   const uint32_t g = id / (ptiles * qtiles);
   uint32_t pt, qt;
@@ -696,12 +704,12 @@ __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t
     pb.set_fragments(at.wb);
     fast_product<DT, S, true, true>(smem, pa, pb, (int)((hi - lo) / FK), (int)((hi - lo) % FK), at.wa >= plim || at.wb >= qlim, acc);
   }
-  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, at.wa, at.wb, acc);
+  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, at, acc);
 }
 
 using Large = Shape<256, 256, 2, 4, 2>;
 using Medium = Shape<128, 128, 2, 2, 2>;
-using Little = Shape<64, 64, 2, 2, 3>;
+using Little = Shape<64, 64, 2, 2, 2>;
 
 // Whole 16-byte vectors everywhere, and offsets within a tile that fit 32 bits.
 bool fast_rows(const void *p, int64_t ld) { return (uintptr_t)p % 16u == 0 && ld % 8 == 0 && ld <= 1 << 21; }
@@ -732,8 +740,10 @@ bool large_tiles(int64_t rows_per_group, int64_t tiles) { return rows_per_group 
 
 // Fewer 128 x 128 tiles than CUs: 64 x 64 ones.  us with 128 / 64: fp32, 8 groups of 256, 768 x 1000 (128 tiles): 82 / 53; 16 of
 // 256, 1024 x 1024 (256 tiles): 109 / 112; bf16, 4 of 75, 512 x 1024 (24 tiles): 9.2 / 7.8; 16 of 256 (256 tiles): 17.9 / 20.3.
+// Through registers (`any`) below two tiles a CU: the longest group's tiles are what a small fp32 weight gradient waits for (8
+// groups, the largest twice the mean, 768 x 1000, 384 tiles: 92 / 58 us).
 constexpr int64_t kLittleTiles = 256;
-bool little_tiles(int64_t row_tiles, int64_t col_tiles) { return row_tiles * col_tiles < kLittleTiles; }
+bool little_tiles(int64_t row_tiles, int64_t col_tiles, bool any) { return row_tiles * col_tiles < (any ? 2 : 1) * kLittleTiles; }
 
 // Groups of few rows, staged through registers: tiles of 32 rows leave fewer matrix instructions to rows that are not there.
 // fp32, 32 groups, 2048 x 1408, us with 64 x 64 / 32 x 128 tiles: 2 rows a group 200 / 145, 32 rows 170 / 130, 64 rows 168 / 173.
@@ -757,7 +767,7 @@ bool run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, 
                     : go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, false, Large>))
           return true;
       }
-      if (little_tiles(ceil_div(M, Medium::BM), ceil_div(N, Medium::BN)))
+      if (little_tiles(ceil_div(M, Medium::BM), ceil_div(N, Medium::BN), false))
         return w_trans ? go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, true, Little>)
                        : go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, false, Little>);
       return w_trans ? go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, true, Medium>)
@@ -769,7 +779,7 @@ bool run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, 
     return w_trans ? go(S::BM, S::BN, 256, grouped_any_kernel<DT, true, S>) : go(S::BM, S::BN, 256, grouped_any_kernel<DT, false, S>);
   };
   if (flat_tiles(M, groups)) return any(AnyShape<32, 128>());
-  return little_tiles(ceil_div(M, 128), ceil_div(N, 128)) ? any(AnyShape<64, 64>()) : any(AnyShape<128, 128>());
+  return little_tiles(ceil_div(M, 128), ceil_div(N, 128), true) ? any(AnyShape<64, 64>()) : any(AnyShape<128, 128>());
 }
 
 template <int DT>
@@ -778,9 +788,9 @@ bool run_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, i
   using elem = typename Storage<DT>::elem;
   auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel) {
     const int64_t pt = ceil_div(P, bm), qt = ceil_div(Q, bn);
-    if (pt * qt > 0x7FFFFFF0ll / groups) return false;
+    if (pt * qt > 0x7FFFFF00ll / groups) return false;
     const int64_t tiles = pt * qt * groups;
-    kernel<<<(unsigned)(ceil_div(tiles, 8) * 8), threads, 0, s>>>((elem *)dw, (const elem *)a, (const elem *)b, offsets, M, P, Q, (uint32_t)pt,
+    kernel<<<(unsigned)(ceil_div(tiles, 8 * TURN) * 8 * TURN), threads, 0, s>>>((elem *)dw, (const elem *)a, (const elem *)b, offsets, M, P, Q, (uint32_t)pt,
                                                                   (uint32_t)qt, (uint32_t)tiles);
     return true;
   };
@@ -788,12 +798,12 @@ bool run_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, i
     if (M > 0 && fast_rows(dw, Q) && fast_rows(a, P) && fast_rows(b, Q)) {
       if (large_tiles(M / groups, ceil_div(P, Large::BM) * ceil_div(Q, Large::BN) * groups))
         return go(Large::BM, Large::BN, Large::THREADS, grouped_wgrad_fast_kernel<DT, Large>);
-      if (little_tiles(ceil_div(P, Medium::BM) * groups, ceil_div(Q, Medium::BN)))
+      if (little_tiles(ceil_div(P, Medium::BM) * groups, ceil_div(Q, Medium::BN), false))
         return go(Little::BM, Little::BN, Little::THREADS, grouped_wgrad_fast_kernel<DT, Little>);
       return go(Medium::BM, Medium::BN, Medium::THREADS, grouped_wgrad_fast_kernel<DT, Medium>);
     }
   }
-  if (little_tiles(ceil_div(P, 128) * groups, ceil_div(Q, 128))) return go(64, 64, 256, grouped_wgrad_any_kernel<DT, AnyShape<64, 64>>);
+  if (little_tiles(ceil_div(P, 128) * groups, ceil_div(Q, 128), true)) return go(64, 64, 256, grouped_wgrad_any_kernel<DT, AnyShape<64, 64>>);
   return go(128, 128, 256, grouped_wgrad_any_kernel<DT, AnyShape<128, 128>>);
 }
 
