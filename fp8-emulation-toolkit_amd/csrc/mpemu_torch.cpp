@@ -422,8 +422,10 @@ at::Tensor clip_grads(const std::vector<at::Tensor> &grads, const c10::optional<
   }
   check(fpemu_clip_multi(tab.data(), tab.size(), (int)order, (const double *)sum.data_ptr(), (float)max_norm,
                          (float *)norm.data_ptr(), on.stream));
-  for (size_t i = 0; i < grads.size(); i++)
+  for (size_t i = 0; i < grads.size(); i++) {
     if (!dense[i].is_same(grads[i])) grads[i].copy_(dense[i]);
+    else if (!outs[i].is_inference()) torch::autograd::impl::bump_version(outs[i]);   // written through its address
+  }
   return norm;
 }
 

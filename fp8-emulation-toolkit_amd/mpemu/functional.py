@@ -233,6 +233,23 @@ def _overlap(grads, outs):
     return False
 
 
+def _over_ranks(total, order, group):
+    """The sum (or maximum) of `total` (float64[1]) over the ranks of a process group, in place.  RCCL reduces it in stream
+    order; every other backend gets it staged through the host.  A NaN of one rank reaches all of them."""
+    import torch.distributed as dist
+    from .sharded import group_backend
+    staged = total if group_backend(group) == "nccl" else total.cpu()
+    if order == _hip.NORM_INF:   # a maximum need not carry a NaN: that travels beside it
+        pair = torch.cat([staged.nan_to_num(nan=math.inf, posinf=math.inf), staged.isnan().to(staged.dtype)])
+        dist.all_reduce(pair, op=dist.ReduceOp.MAX, group=group)
+        staged = torch.where(pair[1:] > 0, math.nan, pair[:1])
+    else:
+        dist.all_reduce(staged, op=dist.ReduceOp.SUM, group=group)
+    if staged is not total:
+        total.copy_(staged)
+    return total
+
+
 def grad_norm(grads, norm_type=2.0):
     """The norm (1, 2 or inf) of all elements of a list of tensors as one vector: float32, 0-d, on the device.  The sum runs
     in 64 bits, so neither large nor many elements overflow or drown it."""
@@ -252,7 +269,7 @@ def grad_norm(grads, norm_type=2.0):
     return norm
 
 
-def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=False):
+def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=False, group=None):
     """Scale a list of gradients by min(1, max_norm / (norm + 1e-6)), norm over all of them; returns the norm (float32, 0-d,
     on the device, before clipping).
 
@@ -260,7 +277,10 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
     gradients clipped into fp32 master gradients in one pass).  No tensor may share memory with another one's output.  A
     norm that is not finite gives what the arithmetic gives (NaN, or zeros and NaN), as
     torch.nn.utils.clip_grad_norm_ does; error_if_nonfinite=True reads the norm on the host first and raises instead,
-    with every gradient as it was."""
+    with every gradient as it was.
+
+    group: a torch.distributed process group over whose ranks the gradients are sharded: the norm is that of all ranks'
+    gradients (one all-reduce of one word), every rank's list on one device of its own, an empty one included."""
     who = "clip_grads_"
     order = _order(norm_type, who)
     max_norm = float(max_norm)
@@ -270,10 +290,10 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
     out = None if out is None else _list(out)
     if out is not None and len(out) != len(grads):
         raise ValueError("clip_grads_: %d gradients but %d outputs" % (len(grads), len(out)))
-    if not grads:
+    if not grads and group is None:
         return torch.tensor(0.0)
     ext = _native()
-    if ext is not None and all(torch.is_tensor(t) for t in grads + (out or [])):
+    if ext is not None and group is None and all(torch.is_tensor(t) for t in grads + (out or [])):
         return ext.clip_grads(grads, out, max_norm, order, bool(error_if_nonfinite))
     _check_gradients(grads, who)
     if out is not None:
@@ -291,22 +311,27 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
                 raise ValueError("clip_grads_: out needs gradients that fill their memory without gaps")
     if any(0 in g.stride() and g.numel() > 1 and d.data_ptr() != g.data_ptr() for g, d in zip(grads, dense)) or _overlap(dense, outs):
         raise ValueError("clip_grads_: a gradient or output shares memory with another output (or with itself)")
-    total = torch.empty(1, dtype=torch.float64, device=grads[0].device)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _hip.grad_norm_multi_(dense, order, total, norm)
-    if error_if_nonfinite and not bool(torch.isfinite(norm)):
-        raise RuntimeError("clip_grads_: the norm of the gradients is %s" % norm.item())
-    _hip.clip_multi_(dense, outs, order, total, max_norm)
-    if out is None:
-        for d, g in zip(dense, grads):
-            if d.data_ptr() != g.data_ptr():
-                g.detach().copy_(d)
+    device = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    total = torch.empty(1, dtype=torch.float64, device=device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    _hip.grad_norm_multi_(dense, order, total)
+    if group is not None:
+        _over_ranks(total, order, group)
+    if error_if_nonfinite and not bool(torch.isfinite(total)):
+        raise RuntimeError("clip_grads_: the norm of the gradients is %s" % total.item())
+    _hip.clip_multi_(dense, outs, order, total, max_norm, norm)
+    for d, g, o in zip(dense, grads, grads if out is None else out):
+        if out is None and d.data_ptr() != g.data_ptr():
+            g.detach().copy_(d)
+        elif not o.is_inference():
+            torch.autograd.graph.increment_version(o)   # written through its address
     return norm
 
 
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, group=None):
     """torch.nn.utils.clip_grad_norm_ on these kernels: clips the .grad of the parameters that have one, in place, and
     returns the norm before clipping.  Two passes over the gradients (one where nothing has to be clipped), a few launches
-    for the whole list, no host synchronisation."""
+    for the whole list, no host synchronisation.  The gradients are on one device; group: as clip_grads_."""
     params = [parameters] if torch.is_tensor(parameters) else parameters
-    return clip_grads_([p.grad for p in params if p.grad is not None], max_norm, norm_type, error_if_nonfinite=error_if_nonfinite)
+    return clip_grads_([p.grad for p in params if p.grad is not None], max_norm, norm_type, error_if_nonfinite=error_if_nonfinite,
+                       group=group)

@@ -125,7 +125,7 @@ def test_modules_and_their_hooks_configure():
 
     model = Model().train()
     assert "scale=2.0" in repr(model.emb) and "num_groups=3" in repr(model.experts)
-    assert float(model.emb.weight[1].abs().sum()) == 0.0          # nn.Embedding's own rule for the padding entry
+    assert float(model.emb.weight.detach()[1].abs().sum()) == 0.0          # nn.Embedding's own rule for the padding entry
     emu = HybridEmulator(model, None, device="cpu")
     emu.prepare_model(model, None, None)
     d = emu.model_qconfig_dict
@@ -136,3 +136,27 @@ def test_modules_and_their_hooks_configure():
     emu.prepare_model(emu.model, None, None)
     assert emu.model_qconfig_dict["experts"].wt_qconfig is not None
     assert emu.model_qconfig_dict["product"].wt_qconfig is None
+
+
+def _ranks(rank, world, path, values, out):
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method="file://" + path, rank=rank, world_size=world)
+    got = []
+    for order, per_rank in values:
+        total = torch.tensor([per_rank[rank]], dtype=torch.float64)
+        got.append(float(F._over_ranks(total, order, dist.group.WORLD)))
+    torch.save(got, "%s.%d" % (out, rank))
+    dist.destroy_process_group()
+
+
+def test_norm_over_two_ranks(tmp_path):
+    """The word that ranks exchange: sums add up, maxima win, a NaN or infinity of one rank reaches the other."""
+    import math
+    inf, nan = math.inf, math.nan
+    values = [(b.NORM_2, (2.0, 3.5)), (b.NORM_1, (0.0, 1.25)), (b.NORM_INF, (2.0, 3.5)), (b.NORM_INF, (7.0, 0.0)),
+              (b.NORM_INF, (nan, 3.0)), (b.NORM_INF, (inf, nan)), (b.NORM_INF, (inf, 1.0)), (b.NORM_2, (nan, 1.0))]
+    torch.multiprocessing.spawn(_ranks, args=(2, str(tmp_path / "store"), values, str(tmp_path / "out")), nprocs=2)
+    want = [5.5, 1.25, 3.5, 7.0, nan, nan, inf, nan]
+    for rank in range(2):
+        got = torch.load(str(tmp_path / "out") + ".%d" % rank)
+        assert all(g == w or (math.isnan(g) and math.isnan(w)) for g, w in zip(got, want)), got

@@ -223,6 +223,22 @@ def test_grouped_mm(dtype, linear, sizes, K, N):
     check_grouped(x, w, offsets_of(sizes))
 
 
+RAGGED = [900, 0, 333, 129, 127, 600, 8, 3]
+
+
+@pytest.mark.parametrize("linear", [False, True])
+@pytest.mark.parametrize("dtype,sizes,K,N", [(t, RAGGED, 72, 2056) for t in TYPES]             # tiles of 128 x 128, in whole
+                         + [(t, RAGGED, 77, 4109) for t in TYPES]                              # vectors or not,
+                         + [(t, [1500, 300, 257, 0, 1200, 600, 1000, 100], 2056, 8264) for t in TYPES[1:]])   # and of 256 x 256
+def test_grouped_mm_large(dtype, linear, sizes, K, N):
+    M, G = sum(sizes), len(sizes)
+    x = randn((M + 300, K), dtype, 1)
+    x[M:] = math.nan
+    w = randn((G, N, K), dtype, 2).transpose(1, 2) if linear else randn((G, K, N), dtype, 2)
+    y, dx, dw = check_grouped(x, w, offsets_of(sizes))
+    assert float(y[M:].abs().sum()) == 0.0 and float(dx[M:].abs().sum()) == 0.0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_grouped_mm_rows_of_no_group(dtype):
     """Rows before the first and behind the last group hold infinities and NaN: they reach nothing, and come out zero."""
@@ -408,6 +424,35 @@ def test_clip_layouts_and_overlap(front):
     for grads, out in (([t], [t, t]), ([t], [t[:50]]), ([t], [t.half()])):
         with pytest.raises(ValueError):
             F.clip_grads_(grads, 1.0, out=out)
+
+
+def test_clip_moves_the_version(front):
+    """A gradient that autograd still needs must not change unseen."""
+    a = randn((10,), torch.float32, 1).requires_grad_(True)
+    g = randn((10,), torch.float32, 2)
+    kept, out = (a * g).sum(), torch.empty(10, device=DEV)
+    F.clip_grads_([g], 0.1, out=[out])
+    before = out._version
+    F.clip_grads_([randn((10,), torch.float32, 2)], 0.1, out=[out])
+    assert out._version > before
+    F.clip_grads_([g], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        kept.backward()
+
+
+def test_clip_over_a_group_of_one(front, tmp_path):
+    """The sharded form through a process group: gloo stages the one word through the host."""
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method="file://" + str(tmp_path / "store"), rank=0, world_size=1)
+    try:
+        for p in (1.0, 2.0, math.inf):
+            g = [randn((1000,), torch.bfloat16, 1), randn((77,), torch.float32, 2)]
+            twin = [t.clone() for t in g]
+            a, b = F.clip_grads_(g, 0.5, p, group=dist.group.WORLD), F.clip_grads_(twin, 0.5, p)
+            assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(g, twin))
+        assert float(F.clip_grads_([], 1.0, group=dist.group.WORLD)) == 0.0
+    finally:
+        dist.destroy_process_group()
 
 
 def test_clip_grad_norm_of_parameters(front):
