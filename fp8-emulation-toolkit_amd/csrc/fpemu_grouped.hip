@@ -733,9 +733,10 @@ int launched(const char *who) {
 }
 
 // A shape's tiles cost the same whether their rows are filled or not, so the large one needs groups of some rows, and tiles
-// for every CU.  bf16, TFLOP/s with 256 x 256 / 128 x 128 tiles: 16 groups of 1024 rows, 2048 x 4096: 966 / 777; 16 of 512,
-// 1024 x 2816: 807 / 812; 8 of 256, 768 x 1024: 164 / 291; 32 of 2 rows, 2048 x 1408: 5.3 / 6.2 TB/s of weights.
-constexpr int64_t kLargeRows = 512, kLargeTiles = 512;
+// for half of the CUs.  bf16, us with 256 x 256 / 128 x 128 tiles, operands from memory: 16 groups of about 1024 rows, 2048 x
+// 4096: 324 / 385; of about 512, 1024 x 2816 (352 large tiles): 68 / 83, 2816 x 1024 (128): 86 / 98; 8 of 256, 768 x 1024
+// (32): 20 / 11; 32 of 2 rows, 2048 x 1408: 5.3 / 6.2 TB/s of weights.
+constexpr int64_t kLargeRows = 256, kLargeTiles = 128;
 bool large_tiles(int64_t rows_per_group, int64_t tiles) { return rows_per_group >= kLargeRows && tiles >= kLargeTiles; }
 
 // Fewer 128 x 128 tiles than CUs: 64 x 64 ones.  us with 128 / 64: fp32, 8 groups of 256, 768 x 1000 (128 tiles): 82 / 53; 16 of
