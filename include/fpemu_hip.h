@@ -367,7 +367,7 @@ int fpemu_embedding_grad(const void *dout, const void *ids, int id_bytes, void *
 /* Matrix products by group: y[i][:] = x[i][:] @ W_g for offsets[g] <= i < offsets[g + 1]; x [M][K], y [M][N].
  *   w_trans = 0 : w [groups][K][N], W_g = w[g];   w_trans = 1 : w [groups][N][K], W_g = w[g] transposed (the layout of a
  *   linear layer's weight).  offsets: groups + 1 device words, not decreasing, within [0, M]; rows outside every group
- *   are zero in y.  The gradient of x is the same call on dy with the other w_trans.  16-bit types multiply on the matrix
+ *   are zero in y.  Every workgroup looks its tile up in the offsets: meant for up to some thousand groups.  The gradient of x is the same call on dy with the other w_trans.  16-bit types multiply on the matrix
  *   cores with fp32 sums; fp32 runs the k-ascending fmaf chain of fpemu_gemm_f32 (variant 1), bit for bit. */
 int fpemu_grouped_gemm(void *y, const void *x, const void *w, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
                        int64_t groups, int dtype, int w_trans, void *stream);
@@ -384,7 +384,8 @@ int fpemu_grouped_gemm_wgrad(void *dw, const void *a, const void *b, const int32
  *                           fpemu_grad_norm_workspace_bytes(count) bytes, 8-byte aligned.
  *   fpemu_clip_multi      : out = in * min(1, max_norm / (norm + 1e-6)), the norm taken from *sum on the device (ranks
  *                           that hold shards add their sums up in between); norm (or NULL) receives it.
- * The tables are host memory, read before the call returns. */
+ * The tables are host memory, read before the call returns.  Outputs must not overlap each other or another entry's
+ * gradient. */
 enum { FPEMU_NORM_INF = 0, FPEMU_NORM_1 = 1, FPEMU_NORM_2 = 2 };
 typedef struct fpemu_grad {
   const void *in;
