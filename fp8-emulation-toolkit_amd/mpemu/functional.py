@@ -317,8 +317,10 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
     _hip.grad_norm_multi_(dense, order, total)
     if group is not None:
         _over_ranks(total, order, group)
-    if error_if_nonfinite and not bool(torch.isfinite(total)):
-        raise RuntimeError("clip_grads_: the norm of the gradients is %s" % total.item())
+    if error_if_nonfinite:
+        value = (total.sqrt() if order == _hip.NORM_2 else total).float().item()   # the norm as it is returned
+        if not math.isfinite(value):
+            raise RuntimeError("clip_grads_: the norm of the gradients is %s" % value)
     _hip.clip_multi_(dense, outs, order, total, max_norm, norm)
     for d, g, o in zip(dense, grads, grads if out is None else out):
         if out is None and d.data_ptr() != g.data_ptr():

@@ -455,6 +455,28 @@ def test_clip_over_a_group_of_one(front, tmp_path):
         dist.destroy_process_group()
 
 
+@pytest.mark.parametrize("sharded", [False, True])
+def test_clip_refuses_a_norm_beyond_float32(front, sharded, tmp_path):
+    """Four times 3e38: the 64-bit sum is finite, the norm (6e38) is not a float32; 4e19: the sum of squares is not one, the norm is."""
+    import torch.distributed as dist
+    group = None
+    if sharded:
+        dist.init_process_group("gloo", init_method="file://" + str(tmp_path / "store"), rank=0, world_size=1)
+        group = dist.group.WORLD
+    try:
+        g = torch.full((4,), 3e38, device=DEV)
+        with pytest.raises(RuntimeError, match="norm of the gradients is inf"):
+            F.clip_grads_([g], 1.0, error_if_nonfinite=True, group=group)
+        assert torch.equal(g, torch.full((4,), 3e38, device=DEV))
+        g = torch.full((4,), 4e19, device=DEV)
+        norm = F.clip_grads_([g], 1.0, error_if_nonfinite=True, group=group)
+        assert abs(float(norm) - 8e19) <= 8e19 * 2.0 ** -22
+        close(g, torch.full((4,), 0.5, dtype=torch.float64, device=DEV), 0.5 * 2.0 ** -21)
+    finally:
+        if sharded:
+            dist.destroy_process_group()
+
+
 def test_clip_grad_norm_of_parameters(front):
     ps = [torch.nn.Parameter(randn((50, 20), torch.float32, i)) for i in range(4)]
     for p in ps[:3]:
