@@ -63,12 +63,13 @@ SortPlan sort_plan(uint64_t groups) {
 }
 
 // Memory that a sort's kernels clear beside their own work, in workgroups behind the sort's: a table's gradient is cleared
-// while its tokens are sorted (the sort keeps a few CUs busy, the stores the memory).
+// while its tokens are sorted (the sort keeps a few CUs busy, the stores the memory).  `stream`: past the caches.
 typedef uint32_t vec_a2 __attribute__((ext_vector_type(4), aligned(2)));   // rows of odd widths: element-aligned only
 struct Fill {
   char *p;
   uint64_t bytes;          // even
   uint64_t first, last;    // this launch's share, in pieces of kFillPiece
+  bool stream;
 };
 constexpr uint64_t kFillPiece = 128 << 10;   // of one workgroup
 
@@ -76,8 +77,13 @@ __device__ __forceinline__ void fill_piece(const Fill &f, uint64_t piece) {
   const uint64_t at = (f.first + piece) * kFillPiece, end = at + kFillPiece < f.bytes ? at + kFillPiece : f.bytes;
   const u32x4 zero = {0u, 0u, 0u, 0u};
   uint64_t i = at + threadIdx.x * 16u;
+  if (f.stream) {
 #pragma unroll 4
-  for (; i + 16 <= end; i += kSortThreads * 16u) *(vec_a2 *)(f.p + i) = zero;
+    for (; i + 16 <= end; i += kSortThreads * 16u) __builtin_nontemporal_store(zero, (vec_a2 *)(f.p + i));
+  } else {
+#pragma unroll 4
+    for (; i + 16 <= end; i += kSortThreads * 16u) *(vec_a2 *)(f.p + i) = zero;
+  }
   for (; i < end; i += 2) *(uint16_t *)(f.p + i) = 0;   // the thread whose vector reaches over the end
 }
 
@@ -383,7 +389,7 @@ int sort_rows(const char *who, const void *ids, int wide, uint64_t n, uint64_t g
       fill_kernel<<<blocks, kSortThreads, 0, stream>>>(fill);
     }
     if (offsets != nullptr) {
-      const Fill zero{(char *)offsets, 4 * (groups + 1), 0, 0};
+      const Fill zero{(char *)offsets, 4 * (groups + 1), 0, 0, false};
       fill_kernel<<<(unsigned)ceil_div(zero.bytes, kFillPiece), kSortThreads, 0, stream>>>(zero);
     }
     return launched(who);
@@ -539,9 +545,9 @@ __global__ __launch_bounds__(256) void embedding_kernel(const void *weight, cons
 // 64 lanes take 16 bytes of the row each; a wave loads the rows of eight tokens before it adds the first.  In a row that is
 // not whole vectors the last lane's vector begins earlier and shares columns with its neighbour's, which writes the same
 // values there; only rows shorter than a vector (WHOLE false) go element by element.
-// Bound by rows read at random and by the waves with the longest runs.  Measured: 32768 tokens, entry v about as often as
-// 1 / (v + 1), 131072 x 2048 bf16: chunks 23 us, runs 56 us, behind a sort of 86 us that clears 537 MB meanwhile (6.2 TB/s); 1024
-// tokens, 30522 x 768 fp32: 4.3 and 4.7 us, behind 14 us for sort and clearing.
+// Bound by rows read at random, 4 KB at a time, with the cleared table on its way out.  Measured: 32768 tokens, entry v about as often as
+// 1 / (v + 1), 131072 x 2048 bf16: chunks 15 us, runs 37 us, behind a sort of 94 us that clears 537 MB meanwhile (5.7 TB/s); 1024
+// tokens, 30522 x 768 fp32: 3.7 and 6.1 us, behind 14 us for sort and clearing.
 constexpr uint32_t kSub = 16;    // positions looked at together: their keys and tokens lie in the wave's lanes
 constexpr int kRows = 8;
 
@@ -550,7 +556,19 @@ struct Tokens {
   const uint32_t *keys;     // sorted; entries outside the table have the key `vocab`
   const int32_t *order;
   uint32_t n, vocab, padding, chunk;
+  uint32_t cols;            // waves side by side over a row
   uint64_t width;
+  bool stream;              // rows are read past the caches
+};
+
+// A wave's chunk and its part of the row: the waves of one row lie side by side, so that they ask for its memory together.
+struct WaveChunk {
+  uint32_t chunk, col;
+  __device__ __forceinline__ explicit WaveChunk(uint32_t cols) {
+    const uint32_t wave = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    chunk = wave / cols;
+    col = wave - chunk * cols;
+  }
 };
 
 // One look at kSub positions from `base`: keys and tokens in the lanes, which positions are there, begin a run, count.
@@ -573,13 +591,14 @@ template <int DT, bool WHOLE> struct Columns {
   using E = Elems<DT>;
   uint64_t c;      // the lane's first column
   bool mine;       // lanes behind the row's end do column 0's work and store nothing
-  __device__ __forceinline__ explicit Columns(uint64_t width) {
-    c = ((uint64_t)blockIdx.y * 64u + (threadIdx.x & 63u)) * E::V;
+  __device__ __forceinline__ Columns(uint32_t col, uint64_t width) {
+    c = ((uint64_t)col * 64u + (threadIdx.x & 63u)) * E::V;
     mine = c < width;
     if (!mine) c = 0;
     else if (WHOLE && c + E::V > width) c = width - E::V;
   }
-  __device__ __forceinline__ u32x4 load(const typename E::elem *row, uint64_t width) const {
+  template <bool STREAM> __device__ __forceinline__ u32x4 load(const typename E::elem *row, uint64_t width) const {
+    if constexpr (WHOLE && STREAM) return __builtin_nontemporal_load((const vec_a2 *)(row + c));
     if constexpr (WHOLE) return *(const vec_a2 *)(row + c);
     typename E::elem e[E::V];
 #pragma unroll
@@ -611,11 +630,15 @@ __device__ __forceinline__ void add_rows(const Tokens &t, const Look &look, uint
   for (uint32_t j0 = 0; j0 < kSub; j0 += kRows) {
     if (!((take | look.starts) >> j0 & ((1u << kRows) - 1u))) continue;
     u32x4 v[kRows];
+    auto load_rows = [&](auto stream) {
 #pragma unroll
-    for (uint32_t u = 0; u < kRows; u++) {   // positions that are not taken load row 0 and are not added
-      const uint32_t row = (take >> (j0 + u)) & 1u ? (uint32_t)__builtin_amdgcn_readlane((int)look.pos, (int)(j0 + u)) : 0u;
-      v[u] = at.load((const typename E::elem *)t.dout + (uint64_t)row * t.width, t.width);
-    }
+      for (uint32_t u = 0; u < kRows; u++) {   // positions that are not taken load row 0 and are not added
+        const uint32_t row = (take >> (j0 + u)) & 1u ? (uint32_t)__builtin_amdgcn_readlane((int)look.pos, (int)(j0 + u)) : 0u;
+        v[u] = at.template load<decltype(stream)::value>((const typename E::elem *)t.dout + (uint64_t)row * t.width, t.width);
+      }
+    };
+    if (WHOLE && t.stream) load_rows(std::true_type());
+    else load_rows(std::false_type());
 #pragma unroll
     for (uint32_t u = 0; u < kRows; u++) {
       flush(j0 + u);
@@ -630,26 +653,27 @@ __device__ __forceinline__ void add_rows(const Tokens &t, const Look &look, uint
 }
 
 template <int DT, bool WHOLE> __global__ __launch_bounds__(256) void embedding_chunks_kernel(Tokens t, float *sums) {
-  const uint32_t chunk = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint64_t first = (uint64_t)chunk * t.chunk;
+  const WaveChunk wave(t.cols);
+  const uint64_t first = (uint64_t)wave.chunk * t.chunk;
   if (first == 0 || first + t.chunk > t.n) return;
   const uint32_t key = t.keys[first - 1];
   if (key != t.keys[first + t.chunk - 1] || key >= t.vocab || key == t.padding) return;   // not inside one run
-  const Columns<DT, WHOLE> at(t.width);
+  const Columns<DT, WHOLE> at(wave.col, t.width);
   float acc[Elems<DT>::V] = {};
   for (uint32_t base = 0; base < t.chunk; base += kSub) {
     const Look look(t, (uint32_t)first + base);
     add_rows<DT, WHOLE>(t, look, look.there, at, acc, [](uint32_t) {});
   }
-  if (at.mine) at.store_sum(sums + (uint64_t)chunk * t.width, t.width, acc);
+  if (at.mine) at.store_sum(sums + (uint64_t)wave.chunk * t.width, t.width, acc);
 }
 
 template <int DT, bool WHOLE>
 __global__ __launch_bounds__(256) void embedding_runs_kernel(Tokens t, const float *sums, void *dweight, float scale) {
   using E = Elems<DT>;
-  const uint64_t first = (uint64_t)(blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * t.chunk;
+  const WaveChunk wave(t.cols);
+  const uint64_t first = (uint64_t)wave.chunk * t.chunk;
   if (first >= t.n) return;
-  const Columns<DT, WHOLE> at(t.width);
+  const Columns<DT, WHOLE> at(wave.col, t.width);
   float acc[E::V] = {};
   bool open = false;      // a run of this chunk is being added up
   uint32_t entry = 0;
@@ -705,6 +729,14 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(Tokens t, const flo
   }
   close();
 }
+
+// The table's gradient and the tokens' rows go through the 256 MB cache before the memory where the next reader can find them
+// there, past it where they are more: then the rows do not wait for cleared lines to be written back, nor that reader.  us
+// through / past the cache, an elementwise pass over the gradient included, by MB of table and rows: 106 69 / 75, 135 86 / 91,
+// 168 110 / 110, 208 158 / 146, 250 128 / 119, 266 201 / 194, 671 448 / 434 (and 164 / 142 without that pass, which alone loses
+// from streaming up to 266 MB of table with few rows: 46 / 59).
+constexpr uint64_t kStreamBytes = 192ull << 20;
+bool streams(uint64_t bytes) { return bytes > kStreamBytes; }
 
 uint32_t chunk_of(uint64_t n) {
   uint32_t c = kSub;
@@ -1034,16 +1066,17 @@ int fpemu_embedding_grad(const void *dout, const void *ids, int id_bytes, void *
   const uint64_t bytes = vocab * width * elem_size(dtype);
   if (ceil_div(bytes, kFillPiece) > 0x7FFFFFFFull) return fail(FPEMU_EINVAL, who, "table too large for one launch");
   hipStream_t s = (hipStream_t)stream;
+  const bool past = streams(bytes + n * width * elem_size(dtype));
   uint32_t *words = (uint32_t *)ws;
   const SortSpace sp = sort_space(n, vocab, true);
   int32_t *order = (int32_t *)(words + sp.words);
   float *sums = (float *)(words + embedding_words(n, vocab));
-  if (const int rc = sort_rows(who, ids, id_bytes == 8, n, vocab, order, nullptr, true, words, Fill{(char *)dweight, bytes, 0, 0}, s)) return rc;
+  if (const int rc = sort_rows(who, ids, id_bytes == 8, n, vocab, order, nullptr, true, words, Fill{(char *)dweight, bytes, 0, 0, past}, s)) return rc;
   if (n == 0) return FPEMU_OK;
   const uint32_t chunk = chunk_of(n);
   const Tokens t{dout, words + sp.keys, order, (uint32_t)n, (uint32_t)vocab, padding >= 0 && (uint64_t)padding < vocab ? (uint32_t)padding : 0xFFFFFFFFu,
-                 chunk, width};
-  const dim3 grid((unsigned)ceil_div(ceil_div(n, chunk), 4), (unsigned)cols);
+                 chunk, (uint32_t)cols, width, past};
+  const unsigned grid = (unsigned)ceil_div(ceil_div(n, chunk) * cols, 4);   // at most 4096 chunks, 65535 parts of a row
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const bool whole = width >= (uint64_t)Elems<DT>::V;

@@ -118,6 +118,14 @@ def test_embedding(dtype, tokens, vocab, width):
     check_embedding(ids, randn((vocab, width), dtype, 1), 27.75, None)
 
 
+@pytest.mark.parametrize("dtype,vocab,width", [(torch.float16, 100003, 1030), (torch.float32, 50001, 1027), (torch.bfloat16, 101, 1025)])
+def test_embedding_larger_than_the_cache(dtype, vocab, width):
+    """Table and rows of more than 192 MB: cleared and read past the caches; rows that begin at any element."""
+    tokens = 100001 if vocab < 1000 else 3001
+    ids = (torch.rand(tokens, generator=gen(7), device=DEV) ** 3 * vocab).long()   # the first entries often
+    check_embedding(ids, randn((vocab, width), dtype, 1), 0.75, vocab - 1)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_embedding_frequent_entries(dtype):
     """Runs that fill chunks, end inside one, begin inside one, and one entry with nearly everything."""
