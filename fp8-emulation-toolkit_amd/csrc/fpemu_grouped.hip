@@ -406,8 +406,8 @@ __global__ __launch_bounds__(256, 2) void grouped_wgrad_any_kernel(typename Stor
 // Waves: WM x WN over the tile.
 // Bound by the matrix cores (by the clock they hold on data that is not zero) where K is long, by a tile's start and end (about
 // 10 us of a 256 x 256 tile) where it is not, by the weights' bytes for few rows.  Measured: 8192^3 bf16 1350 to 1400 TFLOP/s;
-// 16381 rows, 16 uneven groups, 2048 x 4096 fp16 300 us (916); 8197 rows, 16 groups, 1024 x 2816 bf16, y / dx / dW 78 / 72 / 66
-// us; 64 rows, 32 groups, 2048 x 1408 38 us with the weights from memory (4.9 TB/s), 29 us with them in the cache.
+// 16381 rows, 16 uneven groups, 2048 x 4096 fp16 296 us (928); 8197 rows, 16 groups, 1024 x 2816 bf16, y, dx and dW 199 us
+// (712); 64 rows, 32 groups, 2048 x 1408 36 to 39 us with the weights from memory (4.9 TB/s), 25 us with them in the cache.
 constexpr int FK = 64;
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(const lds_char *)p; }
@@ -629,9 +629,9 @@ template <class S> struct WaveAt {   // a wave's part of the tile; waves that sh
 };
 
 // A wave's part of the finished tile, 32 rows at a time through LDS of its own, to memory in rows of TN * 64 bytes; rows < rlim,
-// columns < clim (a multiple of 8) of the tile.
+// columns < clim (a multiple of 8) of the tile.  stream: past the caches.
 template <int DT, class S>
-__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, const WaveAt<S> &at,
+__device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc, int rlim, int clim, bool stream, const WaveAt<S> &at,
                                            const f32x16 (&acc)[S::TM][S::TN]) {
   constexpr int PER = S::TN * 4;   // vectors of a row
   const int lane = threadIdx.x & 63;
@@ -652,7 +652,16 @@ __device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc,
       const int row = r + lane / PER, vec = lane % PER;
       const u32x4 v = *(const u32x4 *)(lds + place(row, vec));
       const int orow = at.wa + i * 32 + row, ocol = at.wb + vec * 8;
-      if (orow < rlim && ocol < clim) *(u32x4 *)(c + orow * ldc + ocol) = v;
+      if (orow < rlim && ocol < clim) {
+        u32x4 *to = (u32x4 *)(c + orow * ldc + ocol);
+        if (stream) {   // fenced off: the compiler would make one ordinary store of the two
+          asm volatile("" : : : "memory");
+          __builtin_nontemporal_store(v, to);
+          asm volatile("" : : : "memory");
+        } else {
+          *to = v;
+        }
+      }
     }
     asm volatile("" : : : "memory");
   }
@@ -660,7 +669,7 @@ __device__ __forceinline__ void fast_store(char *smem, uint16_t *c, int64_t ldc,
 
 template <int DT, bool W_TRANS, class S>
 __global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, const uint16_t *x, const uint16_t *w, const int32_t *offsets,
-                                                                  int64_t M, int64_t N, int64_t K, int64_t groups, uint32_t col_tiles) {
+                                                                  int64_t M, int64_t N, int64_t K, int64_t groups, uint32_t col_tiles, bool stream) {
   __shared__ __attribute__((aligned(16))) char smem[S::LDS];
   const TileMap<S::BM> map(offsets, groups, M);
   const uint32_t id = xcd_tile(blockIdx.x, map.tiles() * col_tiles);
@@ -683,13 +692,13 @@ __global__ __launch_bounds__(S::THREADS) void grouped_fast_kernel(uint16_t *y, c
     b.set_fragments(at.wb);
     fast_product<DT, S, false, !W_TRANS>(smem, a, b, (int)(K / FK), (int)(K % FK), at.wa >= rows || at.wb >= cols, acc);
   }
-  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, at, acc);
+  fast_store<DT, S>(smem, y + first * N + c0, N, rows, cols, stream, at, acc);
 }
 
 template <int DT, class S>
 __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t *dw, const uint16_t *a, const uint16_t *b,
                                                                         const int32_t *offsets, int64_t M, int64_t P, int64_t Q,
-                                                                        uint32_t ptiles, uint32_t qtiles, uint32_t tiles) {
+                                                                        uint32_t ptiles, uint32_t qtiles, uint32_t tiles, bool stream) {
   __shared__ __attribute__((aligned(16))) char smem[S::LDS];
   const uint32_t id = xcd_turn(blockIdx.x, tiles);
   if (id == NO_TILE) return;
@@ -710,7 +719,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_wgrad_fast_kernel(uint16_t
     pb.set_fragments(at.wb);
     fast_product<DT, S, true, true>(smem, pa, pb, (int)((hi - lo) / FK), (int)((hi - lo) % FK), at.wa >= plim || at.wb >= qlim, acc);
   }
-  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, at, acc);
+  fast_store<DT, S>(smem, dw + (int64_t)g * P * Q + p0 * Q + q0, Q, plim, qlim, stream, at, acc);
 }
 
 using Large = Shape<256, 256, 2, 4, 2>;
@@ -752,6 +761,13 @@ bool large_tiles(int64_t rows_per_group, int64_t tiles) { return rows_per_group 
 constexpr int64_t kLittleTiles = 256;
 bool little_tiles(int64_t row_tiles, int64_t col_tiles, bool any) { return row_tiles * col_tiles < (any ? 2 : 1) * kLittleTiles; }
 
+// Results of more than 64 MB (16-bit, whole vectors) are stored past the caches, which keep the operands instead.  bf16, us in
+// the cache / past it, and with an elementwise pass over the result behind: y of 23 MB 35 / 34, 43 / 46; 46 MB 69 / 69, 82 / 85;
+// 134 MB 306 / 300, 347 / 339; dW of 46 MB 47 / 41, 66 / 68; 92 MB 80 / 63, 118 / 119; 185 MB 52 / 41, 154 / 141; 268 MB
+// 292 / 275, 426 / 406.
+constexpr int64_t kStreamBytes = 64ll << 20;
+bool streams(int64_t bytes) { return bytes > kStreamBytes; }
+
 // Groups of few rows, staged through registers: tiles of 32 rows leave fewer matrix instructions to rows that are not there.
 // fp32, 32 groups, 2048 x 1408, us with 64 x 64 / 32 x 128 tiles: 2 rows a group 200 / 145, 32 rows 170 / 130, 64 rows 168 / 173.
 bool flat_tiles(int64_t rows, int64_t groups) { return rows <= 32 * groups; }
@@ -760,25 +776,26 @@ template <int DT>
 bool run_grouped(void *y, const void *x, const void *w, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t groups,
                  int w_trans, hipStream_t s) {
   using elem = typename Storage<DT>::elem;
-  auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel) {
+  auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel, auto... more) {
     const int64_t cols = ceil_div(N, bn), rows = ceil_div(M, bm) + groups + 2;   // every group may end in a partial tile
     if (rows * cols > 0x7FFFFFF0ll) return false;
     kernel<<<(unsigned)(ceil_div(rows * cols, 8) * 8), threads, 0, s>>>((elem *)y, (const elem *)x, (const elem *)w, offsets, M, N, K, groups,
-                                                                        (uint32_t)cols);
+                                                                        (uint32_t)cols, more...);
     return true;
   };
   if constexpr (DT != FPEMU_F32) {
     if (K > 0 && fast_rows(y, N) && fast_rows(x, K) && fast_rows(w, N)) {
+      const bool stream = streams(2 * M * N);
       if (large_tiles(M / groups, ceil_div(M, Large::BM) * ceil_div(N, Large::BN))) {
-        if (w_trans ? go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, true, Large>)
-                    : go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, false, Large>))
+        if (w_trans ? go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, true, Large>, stream)
+                    : go(Large::BM, Large::BN, Large::THREADS, grouped_fast_kernel<DT, false, Large>, stream))
           return true;
       }
       if (little_tiles(ceil_div(M, Medium::BM), ceil_div(N, Medium::BN), false))
-        return w_trans ? go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, true, Little>)
-                       : go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, false, Little>);
-      return w_trans ? go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, true, Medium>)
-                     : go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, false, Medium>);
+        return w_trans ? go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, true, Little>, stream)
+                       : go(Little::BM, Little::BN, Little::THREADS, grouped_fast_kernel<DT, false, Little>, stream);
+      return w_trans ? go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, true, Medium>, stream)
+                     : go(Medium::BM, Medium::BN, Medium::THREADS, grouped_fast_kernel<DT, false, Medium>, stream);
     }
   }
   auto any = [&](auto shape) {
@@ -793,21 +810,22 @@ template <int DT>
 bool run_wgrad(void *dw, const void *a, const void *b, const int32_t *offsets, int64_t M, int64_t P, int64_t Q, int64_t groups,
                hipStream_t s) {
   using elem = typename Storage<DT>::elem;
-  auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel) {
+  auto go = [&](int64_t bm, int64_t bn, int threads, auto kernel, auto... more) {
     const int64_t pt = ceil_div(P, bm), qt = ceil_div(Q, bn);
     if (pt * qt > 0x7FFFFF00ll / groups) return false;
     const int64_t tiles = pt * qt * groups;
     kernel<<<(unsigned)(ceil_div(tiles, 8 * TURN) * 8 * TURN), threads, 0, s>>>((elem *)dw, (const elem *)a, (const elem *)b, offsets, M, P, Q, (uint32_t)pt,
-                                                                  (uint32_t)qt, (uint32_t)tiles);
+                                                                  (uint32_t)qt, (uint32_t)tiles, more...);
     return true;
   };
   if constexpr (DT != FPEMU_F32) {
     if (M > 0 && fast_rows(dw, Q) && fast_rows(a, P) && fast_rows(b, Q)) {
+      const bool stream = streams(2 * P * Q * groups);
       if (large_tiles(M / groups, ceil_div(P, Large::BM) * ceil_div(Q, Large::BN) * groups))
-        return go(Large::BM, Large::BN, Large::THREADS, grouped_wgrad_fast_kernel<DT, Large>);
+        return go(Large::BM, Large::BN, Large::THREADS, grouped_wgrad_fast_kernel<DT, Large>, stream);
       if (little_tiles(ceil_div(P, Medium::BM) * groups, ceil_div(Q, Medium::BN), false))
-        return go(Little::BM, Little::BN, Little::THREADS, grouped_wgrad_fast_kernel<DT, Little>);
-      return go(Medium::BM, Medium::BN, Medium::THREADS, grouped_wgrad_fast_kernel<DT, Medium>);
+        return go(Little::BM, Little::BN, Little::THREADS, grouped_wgrad_fast_kernel<DT, Little>, stream);
+      return go(Medium::BM, Medium::BN, Medium::THREADS, grouped_wgrad_fast_kernel<DT, Medium>, stream);
     }
   }
   if (little_tiles(ceil_div(P, 128) * groups, ceil_div(Q, 128), true)) return go(64, 64, 256, grouped_wgrad_any_kernel<DT, AnyShape<64, 64>>);

@@ -247,6 +247,13 @@ def test_grouped_mm_large(dtype, linear, sizes, K, N):
     assert float(y[M:].abs().sum()) == 0.0 and float(dx[M:].abs().sum()) == 0.0
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("sizes,K,N", [([2, 0, 5, 1] * 8, 1032, 1160),      # a weight gradient of 76 MB, few rows a group
+                                       ([9000], 64, 4104)])                 # y of 74 MB, one group
+def test_grouped_mm_results_past_the_caches(dtype, sizes, K, N):
+    check_grouped(randn((sum(sizes), K), dtype, 1), randn((len(sizes), K, N), dtype, 2), offsets_of(sizes))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_grouped_mm_rows_of_no_group(dtype):
     """Rows before the first and behind the last group hold infinities and NaN: they reach nothing, and come out zero."""
