@@ -184,6 +184,14 @@ void once_only(const char *who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, ": differentiable once (create_graph is not supported)");
 }
 
+// Nor do they carry forward-mode derivatives: a dual tensor's result would come out without its tangent, whatever the grad
+// mode and requires_grad say.  Refused before the kernels read its address, in the backward pass too.
+void reverse_only(const char *who, at::ArrayRef<at::Tensor> ts) {
+  for (const at::Tensor &t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), who,
+                                ": forward-mode derivatives are not supported (a dual tensor came in)");
+}
+
 // A leaf that an eager autograd graph still holds has its accumulation node on the eager stream.  A backward pass captured
 // into a HIP graph would make the capture wait for that stream, which ends the process when the capture ends: such a
 // forward is refused.  Looked for while a capture runs only: every accumulation node behind the inputs.
@@ -246,6 +254,7 @@ struct EmbeddingOp : public torch::autograd::Function<EmbeddingOp> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     once_only("embedding");
+    reverse_only("embedding", grads[0]);
     const at::Tensor ids = ctx->get_saved_variables()[0];
     const at::Tensor dout = grads[0].contiguous();
     const OnStream on(dout);
@@ -261,6 +270,7 @@ struct EmbeddingOp : public torch::autograd::Function<EmbeddingOp> {
 };
 
 at::Tensor embedding(const at::Tensor &ids_in, const at::Tensor &weight, double scale, int64_t padding) {
+  reverse_only("embedding", weight);
   const at::Tensor ids = ids_in.contiguous();
   if (needs_graph(weight)) {
     { const OnStream on(weight); refuse_live_leaves("embedding", {weight}, on.stream); }
@@ -287,6 +297,7 @@ struct GroupedOp : public torch::autograd::Function<GroupedOp> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     once_only("grouped_mm");
+    reverse_only("grouped_mm", grads[0]);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
     const bool trans = ctx->saved_data["trans"].toBool();
@@ -305,6 +316,7 @@ struct GroupedOp : public torch::autograd::Function<GroupedOp> {
 };
 
 at::Tensor grouped_mm(const at::Tensor &x_in, const at::Tensor &weight, const at::Tensor &offsets) {
+  reverse_only("grouped_mm", {x_in, weight});
   // contiguous() and transpose() are differentiable steps outside the node: its operands are what the kernels read
   const at::Tensor x = x_in.contiguous();
   at::Tensor w = weight;
@@ -323,6 +335,7 @@ at::Tensor grouped_mm(const at::Tensor &x_in, const at::Tensor &weight, const at
 
 // What _gradients() of mpemu.functional checks, here for the whole list at once.
 void check_grads(const char *who, const std::vector<at::Tensor> &ts, const char *what) {
+  reverse_only(who, ts);
   for (const at::Tensor &t : ts) {
     TORCH_CHECK_TYPE(!t.is_sparse(), who, ": sparse gradients are not supported");
     const auto k = t.scalar_type();

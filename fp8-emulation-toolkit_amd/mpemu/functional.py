@@ -9,7 +9,8 @@ Every operator runs in hand-written gfx950 kernels (libfpemu_hip.so) on torch's 
 device, float32 / float16 / bfloat16.  Nothing here synchronises with the host: group sizes, norms and coefficients stay
 on the device, so the operators (and their gradients) can be captured into a HIP graph; a capture whose leaves an eager
 autograd graph still holds is refused.  Sums run in 32 bits or more and
-are rounded once, in a fixed order: the same inputs give the same bits.
+are rounded once, in a fixed order: the same inputs give the same bits.  Derivatives are reverse mode's: a dual tensor
+(torch.autograd.forward_ad) is refused with NotImplementedError.
 
 The module forms that the quantisation hooks attach to are module_wrappers.{ScaledEmbedding, GroupedMatmul,
 GroupedLinear}; the emulators clip through optimizer_step(optimizer, max_grad_norm=...).
@@ -17,7 +18,7 @@ GroupedLinear}; the emulators clip through optimizer_step(optimizer, max_grad_no
 import math
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from .pytquant.hip import _binding as _hip
@@ -47,6 +48,13 @@ def _native():
     """The C++ front of these operators (one call with checks, allocation, launches and the autograd node), or None:
     then the same kernels are reached through ctypes."""
     return None if _hip.tracing() else _hip.ext()
+
+
+def _refuse_tangents(who, *ts):
+    """The kernels read addresses: a dual tensor's result would come out without its tangent."""
+    for t in ts:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("%s: forward-mode derivatives are not supported (a dual tensor came in)" % who)
 
 
 def _refuse_capture(who, *ts):
@@ -89,6 +97,7 @@ class _Embedding(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        _refuse_tangents("embedding", grad)
         ids, = ctx.saved_tensors
         dweight = torch.empty(ctx.shape, dtype=grad.dtype, device=grad.device)
         return None, _hip.embedding_grad_(grad.contiguous(), ids, dweight, ctx.scale, ctx.padding), None, None
@@ -118,6 +127,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     ext = _native()
     if ext is not None:
         return ext.embedding(ids, weight, float(scale), padding)
+    _refuse_tangents(who, weight)
     _refuse_capture(who, weight)
     return _Embedding.apply(ids.contiguous(), weight, float(scale), padding)
 
@@ -147,6 +157,7 @@ class _GroupedMm(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        _refuse_tangents("grouped_mm", grad)
         x, w, offsets = ctx.saved_tensors
         grad = grad.contiguous()
         dx = dw = None
@@ -185,6 +196,7 @@ def grouped_mm(x, weight, offsets):
     ext = _native()
     if ext is not None:
         return ext.grouped_mm(x, weight, offsets)
+    _refuse_tangents(who, x, weight)
     _refuse_capture(who, x, weight)
     return _GroupedMm.apply(x, weight, offsets)
 
@@ -206,6 +218,7 @@ def _check_gradients(grads, who, what="a gradient"):
         if torch.is_tensor(g) and g.is_sparse:
             raise TypeError("%s: sparse gradients are not supported" % who)
         _floating(g, what, who)
+        _refuse_tangents(who, g)
     _one_device(who, *grads)
 
 

@@ -30,6 +30,26 @@ def test_cpu_tensors_raise(call):
         call()
 
 
+def test_dual_tensors_are_refused_before_anything_else():
+    """A forward-mode derivative would be lost in silence: both fronts refuse the tensor that carries one."""
+    from torch.autograd import forward_ad
+    fronts = [b.ext()] if b.ext() is not None else []
+    w3, offsets = torch.zeros(2, 4, 4), torch.tensor([0, 1, 4], dtype=torch.int32)
+    with forward_ad.dual_level():
+        for grad_mode in (True, False):
+            with torch.set_grad_enabled(grad_mode):
+                dual, dual3 = forward_ad.make_dual(FLT, torch.ones_like(FLT)), forward_ad.make_dual(w3, torch.ones_like(w3))
+                calls = [lambda: F._refuse_tangents("x", FLT, dual), lambda: F._check_gradients([FLT, dual], "x")]
+                for e in fronts:
+                    calls += [lambda: e.embedding(INT, dual, 1.0, -1), lambda: e.grouped_mm(dual, w3, offsets),
+                              lambda: e.grouped_mm(FLT, dual3, offsets), lambda: e.grouped_mm(FLT, dual3.transpose(1, 2), offsets),
+                              lambda: e.grad_norm([dual], b.NORM_2), lambda: e.clip_grads([FLT, dual], None, 1.0, b.NORM_2, False)]
+                for call in calls:
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call()
+        F._refuse_tangents("x", FLT)
+
+
 def test_values_refused_without_gpu():
     with pytest.raises(ValueError):
         F.grad_norm([], norm_type=3.0)

@@ -191,6 +191,28 @@ def test_embedding_refusals(front):
         torch.autograd.grad(g.sum(), (w,))
 
 
+@pytest.mark.parametrize("leaf", [False, True])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_forward_mode_derivatives_are_refused(front, leaf, grad_mode):
+    """No result without its tangent: of the calls, and of the gradients when only the incoming one carries it."""
+    from torch.autograd import forward_ad
+    table, x, w = randn((10, 8), torch.float32, 1), randn((6, 8), torch.float32, 2), randn((2, 8, 4), torch.float32, 3)
+    ids, o = torch.tensor([1, 3, 9], device=DEV), torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
+    y, h = F.grouped_mm(x.clone().requires_grad_(True), w.clone().requires_grad_(True), o), F.embedding(ids, table.clone().requires_grad_(True))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        def dual(t):
+            return forward_ad.make_dual(t.clone().requires_grad_(leaf), torch.ones_like(t))
+        for call in (lambda: F.embedding(ids, dual(table)), lambda: F.grouped_mm(dual(x), w, o), lambda: F.grouped_mm(x, dual(w), o),
+                     lambda: F.grouped_mm(x, dual(w.transpose(1, 2).contiguous()).transpose(1, 2), o),
+                     lambda: y.backward(dual(y.detach()), retain_graph=True), lambda: h.backward(dual(h.detach()), retain_graph=True),
+                     lambda: F.grad_norm([dual(x)]), lambda: F.clip_grads_([x.clone(), dual(x)], 1.0),
+                     lambda: F.clip_grads_([x], 1.0, out=[dual(x)])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    y.sum().backward()    # and everything else goes on
+    h.sum().backward()
+
+
 # ---- products by group --------------------------------------------------------------------------------------------------------
 def offsets_of(sizes, first=0, dtype=torch.int32):
     return torch.tensor([first] + [first + sum(sizes[:i + 1]) for i in range(len(sizes))], dtype=dtype, device=DEV)
