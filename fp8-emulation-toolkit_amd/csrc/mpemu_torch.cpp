@@ -13,11 +13,10 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
-#include <ATen/MemoryOverlap.h>
-
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <numeric>
 #include <unordered_map>
 #include <unordered_set>
 #include <vector>
@@ -361,23 +360,110 @@ std::vector<fpemu_grad_t> grad_table(const std::vector<at::Tensor> &in, const st
   return tab;
 }
 
-// true where an output shares memory with another entry's gradient or output
-bool overlap(const std::vector<fpemu_grad_t> &tab) {
-  struct Span { uintptr_t lo, hi; bool out; };
+// Do tensors share bytes?  An element's bytes lie at sum stride * index + byte; two sets of such places meet where one linear
+// equation has a solution within bounds.  Strides nest in practice, so the search below takes a few steps; one that takes more
+// than kSearch counts as "yes".
+struct Places {
+  struct Term { int64_t step, most; };   // step * (0 .. most)
+  static constexpr int kSearch = 20000;
+  std::vector<Term> terms;
+  std::vector<int64_t> reach, common;    // of the terms from k on: their largest sum, their steps' common divisor
+  int left = kSearch;
+
+  void add(int64_t step, int64_t most) {
+    if (most <= 0) return;
+    for (Term &t : terms)
+      if (t.step == step) { t.most += most; return; }
+    terms.push_back({step, most});
+  }
+  bool contain(int64_t target) {
+    std::sort(terms.begin(), terms.end(), [](const Term &a, const Term &b) { return a.step > b.step; });
+    reach.assign(terms.size() + 1, 0);
+    common.assign(terms.size() + 1, 0);
+    for (size_t k = terms.size(); k-- > 0;) {
+      reach[k] = reach[k + 1] + terms[k].step * terms[k].most;
+      common[k] = std::gcd(common[k + 1], terms[k].step);
+    }
+    return search(0, target);
+  }
+  bool search(size_t k, int64_t target) {
+    if (target < 0 || target > reach[k]) return false;
+    if (k == terms.size()) return true;
+    if (target % common[k]) return false;
+    const int64_t step = terms[k].step, over = target - reach[k + 1];
+    const int64_t lo = over > 0 ? (over + step - 1) / step : 0, hi = std::min(terms[k].most, target / step);
+    for (int64_t x = hi; x >= lo; x--) {
+      if (--left < 0 || search(k + 1, target - x * step)) return true;
+    }
+    return false;
+  }
+};
+
+// bytes from a tensor's first to behind its last element
+int64_t extent(const at::Tensor &t) {
+  if (t.is_non_overlapping_and_dense()) return t.numel() * (int64_t)t.element_size();
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); d++) last += (t.size(d) - 1) * t.stride(d);
+  return (last + 1) * (int64_t)t.element_size();
+}
+
+bool share_memory(const at::Tensor &a, const at::Tensor &b) {   // both with elements, extents that meet
+  if (a.is_non_overlapping_and_dense() && b.is_non_overlapping_and_dense()) return true;
+  Places p;
+  const at::Tensor *const both[] = {&a, &b};
+  for (const at::Tensor *t : both) {
+    for (int64_t d = 0; d < t->dim(); d++)
+      if (t->stride(d) > 0) p.add(t->stride(d) * (int64_t)t->element_size(), t->size(d) - 1);
+    p.add(1, (int64_t)t->element_size() - 1);
+  }
+  return p.contain((int64_t)((uintptr_t)b.data_ptr() - (uintptr_t)a.data_ptr()) + extent(b) - 1);   // b's indices backwards
+}
+
+bool shares_with_itself(const at::Tensor &t) {
+  if (t.is_non_overlapping_and_dense()) return false;
+  const int64_t es = (int64_t)t.element_size();
+  for (int64_t first = 0; first < t.dim(); first++) {   // two elements whose indices differ from this dimension on
+    if (t.size(first) < 2) continue;
+    if (t.stride(first) == 0) return true;
+    Places p;
+    int64_t target = es - 1 - t.stride(first) * es;
+    p.add(t.stride(first) * es, t.size(first) - 2);
+    p.add(1, 2 * (es - 1));
+    for (int64_t d = first + 1; d < t.dim(); d++) {
+      if (t.stride(d) == 0) continue;   // its own turn comes
+      p.add(t.stride(d) * es, 2 * (t.size(d) - 1));
+      target += t.stride(d) * es * (t.size(d) - 1);
+    }
+    if (p.contain(target)) return true;
+  }
+  return false;
+}
+
+// true where an output shares memory with another entry's gradient or output, or a gradient's elements with each other
+bool overlap(const std::vector<at::Tensor> &grads, const std::vector<at::Tensor> &outs) {
+  struct Span { uintptr_t lo, hi; const at::Tensor *t; bool out; };
   std::vector<Span> spans;
-  spans.reserve(2 * tab.size());
-  const auto bytes = [](const fpemu_grad_t &g, int32_t dt) { return (uintptr_t)g.n * (dt == FPEMU_F32 ? 4u : 2u); };
-  for (const fpemu_grad_t &g : tab) {
-    if (g.n == 0) continue;
-    spans.push_back({(uintptr_t)g.out, (uintptr_t)g.out + bytes(g, g.out_dtype), true});
-    if (g.in != g.out) spans.push_back({(uintptr_t)g.in, (uintptr_t)g.in + bytes(g, g.in_dtype), false});
+  spans.reserve(2 * grads.size());
+  const bool in_place = &grads == &outs;
+  for (size_t i = 0; i < grads.size(); i++) {
+    const at::Tensor &o = outs[i], &g = grads[i];
+    if (o.numel() == 0) continue;
+    if (shares_with_itself(o)) return true;
+    const uintptr_t lo = (uintptr_t)o.data_ptr();
+    spans.push_back({lo, lo + (uintptr_t)extent(o), &o, true});
+    if (in_place) continue;
+    const uintptr_t in = (uintptr_t)g.data_ptr();
+    if (in != lo || g.scalar_type() != o.scalar_type()) spans.push_back({in, in + (uintptr_t)extent(g), &g, false});
   }
   std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.lo < b.lo || (a.lo == b.lo && a.hi < b.hi); });
-  uintptr_t top = 0, top_out = 0;
+  std::vector<const Span *> open;   // spans before this one that reach over its beginning
+  uintptr_t top = 0;
   for (const Span &s : spans) {
-    if (s.lo < (s.out ? top : top_out)) return true;
+    if (s.lo >= top) open.clear();
+    for (const Span *o : open)
+      if (o->hi > s.lo && (o->out || s.out) && share_memory(*o->t, *s.t)) return true;
+    open.push_back(&s);
     top = std::max(top, s.hi);
-    if (s.out) top_out = std::max(top_out, s.hi);
   }
   return false;
 }
@@ -413,18 +499,16 @@ at::Tensor clip_grads(const std::vector<at::Tensor> &grads, const c10::optional<
                             (outs[i].scalar_type() == grads[i].scalar_type() || outs[i].scalar_type() == at::kFloat),
                         "clip_grads_: an output needs its gradient's shape, strides and device, and its type or float32");
   }
+  TORCH_CHECK_VALUE(!overlap(grads, outs), "clip_grads_: a gradient or output shares memory with another output (or with itself)");
   const std::vector<at::Tensor> dense = dense_list(grads);
   std::vector<at::Tensor> to;
   to.reserve(grads.size());
   for (size_t i = 0; i < grads.size(); i++) {
     const bool copied = !dense[i].is_same(grads[i]), in_place = outs[i].is_same(grads[i]);
     TORCH_CHECK_VALUE(!copied || in_place, "clip_grads_: out needs gradients that fill their memory without gaps");
-    TORCH_CHECK_VALUE(!copied || at::has_internal_overlap(grads[i]) != at::MemOverlap::Yes,
-                      "clip_grads_: a gradient or output shares memory with another output (or with itself)");
     to.push_back(in_place ? dense[i] : outs[i]);
   }
   const std::vector<fpemu_grad_t> tab = grad_table(dense, to);
-  TORCH_CHECK_VALUE(!overlap(tab), "clip_grads_: a gradient or output shares memory with another output (or with itself)");
   const OnStream on(grads[0]);
   at::Tensor sum = at::empty({1}, grads[0].options().dtype(at::kDouble));
   at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
@@ -457,6 +541,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding", &embedding, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("padding"));
   m.def("grouped_mm", &grouped_mm, py::arg("x"), py::arg("weight"), py::arg("offsets"));
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("order"));
+  m.def("overlap", &overlap, py::arg("grads"), py::arg("outs"));
   m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("outs").none(true), py::arg("max_norm"), py::arg("order"),
         py::arg("finite_only"));
 }

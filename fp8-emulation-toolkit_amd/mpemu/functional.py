@@ -229,20 +229,93 @@ def _dense(t):
     return t if t.is_contiguous() or t.permute(order).is_contiguous() else t.contiguous()
 
 
+def _places_meet(terms, target, most_steps=20000):
+    """Whether sum(step * x) = target has a solution with 0 <= x <= most over the terms (step, most).  Strides nest in
+    practice, so the search takes a few steps; one that takes more than most_steps counts as "yes"."""
+    merged = {}
+    for step, most in terms:
+        if most > 0:
+            merged[step] = merged.get(step, 0) + most
+    terms = sorted(merged.items(), reverse=True)
+    reach, common = [0], [0]    # of the terms from k on: their largest sum, their steps' common divisor
+    for step, most in reversed(terms):
+        reach.append(reach[-1] + step * most)
+        common.append(math.gcd(common[-1], step))
+    reach.reverse()
+    common.reverse()
+    todo = [(0, target)]
+    while todo:
+        k, t = todo.pop()
+        if t < 0 or t > reach[k] or (k < len(terms) and t % common[k]):
+            continue
+        if k == len(terms):
+            return True
+        step, most = terms[k]
+        lo, hi = max(0, -((reach[k + 1] - t) // step)), min(most, t // step)
+        most_steps -= max(0, hi - lo + 1)
+        if most_steps < 0:
+            return True
+        todo += [(k + 1, t - x * step) for x in range(lo, hi + 1)]
+    return False
+
+
+def _dims(t):
+    """(stride in bytes, size) of the dimensions in which t moves, and its element size."""
+    es = t.element_size()
+    return [(st * es, n) for st, n in zip(t.stride(), t.shape) if n > 1], es
+
+
+def _extent(t):
+    """Bytes from a tensor's first to behind its last element."""
+    if t.is_contiguous():
+        return t.numel() * t.element_size()
+    dims, es = _dims(t)
+    return sum(st * (n - 1) for st, n in dims) + es
+
+
+def _share_memory(a, b):
+    """Whether two tensors whose extents meet have a byte in common: one linear equation in their indices (b's backwards)."""
+    if a.is_contiguous() and b.is_contiguous():
+        return True    # asked of extents that meet
+    (da, ea), (db, eb) = _dims(a), _dims(b)
+    terms = [(st, n - 1) for st, n in da + db if st > 0] + [(1, ea + eb - 2)]
+    return _places_meet(terms, b.data_ptr() - a.data_ptr() + _extent(b) - 1)
+
+
+def _shares_with_itself(t):
+    if t.is_contiguous():
+        return False
+    dims, es = _dims(t)
+    if any(st == 0 for st, _ in dims):
+        return True
+    dims.sort()
+    if all(st >= sum(s * (n - 1) for s, n in dims[:k]) + es for k, (st, _) in enumerate(dims)):
+        return False
+    for k, (st, n) in enumerate(dims):    # two elements whose indices differ from dimension k on
+        rest = dims[k + 1:]
+        terms = [(st, n - 2), (1, 2 * (es - 1))] + [(s, 2 * (m - 1)) for s, m in rest]
+        if _places_meet(terms, es - 1 - st + sum(s * (m - 1) for s, m in rest)):
+            return True
+    return False
+
+
 def _overlap(grads, outs):
-    """True where an output shares memory with another entry's gradient or output."""
+    """True where an output shares memory with another entry's gradient or output, or its elements with each other."""
     spans = []
     for g, o in zip(grads, outs):
-        spans.append((o.data_ptr(), o.data_ptr() + o.numel() * o.element_size(), True))
-        if o.data_ptr() != g.data_ptr():
-            spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size(), False))
-    top = top_out = 0
-    for lo, hi, is_out in sorted(s for s in spans if s[1] > s[0]):
-        if lo < (top if is_out else top_out):
+        if g.numel() == 0:
+            continue
+        if _shares_with_itself(o):
             return True
-        top = max(top, hi)
-        if is_out:
-            top_out = max(top_out, hi)
+        spans.append((o.data_ptr(), o.data_ptr() + _extent(o), True, o))
+        if o.data_ptr() != g.data_ptr() or o.dtype != g.dtype:
+            spans.append((g.data_ptr(), g.data_ptr() + _extent(g), False, g))
+    reaching = []    # spans before this one that reach over its beginning
+    for lo, hi, is_out, t in sorted(spans, key=lambda s: s[:2]):
+        reaching = [r for r in reaching if r[0] > lo]
+        if any((is_out or other_out) and _share_memory(other, t) for _, other_out, other in reaching):
+            return True
+        reaching.append((hi, is_out, t))
     return False
 
 
@@ -287,8 +360,8 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
     on the device, before clipping).
 
     In place, or into `out`: a list of the same shapes and strides, each of the gradient's type or float32 (16-bit model
-    gradients clipped into fp32 master gradients in one pass).  No tensor may share memory with another one's output.  A
-    norm that is not finite gives what the arithmetic gives (NaN, or zeros and NaN), as
+    gradients clipped into fp32 master gradients in one pass).  No tensor may share memory with another one's output, nor
+    an output's elements with each other (views that interleave are told from views that overlap).  A norm that is not finite gives what the arithmetic gives (NaN, or zeros and NaN), as
     torch.nn.utils.clip_grad_norm_ does; error_if_nonfinite=True reads the norm on the host first and raises instead,
     with every gradient as it was.
 
@@ -314,6 +387,9 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
         for g, o in zip(grads, out):
             if o.shape != g.shape or o.stride() != g.stride() or o.device != g.device or o.dtype not in (g.dtype, torch.float32):
                 raise ValueError("clip_grads_: an output needs its gradient's shape, strides and device, and its type or float32")
+    overlap = _overlap if _hip.ext() is None else _hip.ext().overlap
+    if overlap(grads, grads if out is None else out):
+        raise ValueError("clip_grads_: a gradient or output shares memory with another output (or with itself)")
     dense = [_dense(g) for g in grads]
     if out is None:
         outs = dense
@@ -322,8 +398,6 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
         for d, g in zip(dense, grads):
             if d.data_ptr() != g.data_ptr():
                 raise ValueError("clip_grads_: out needs gradients that fill their memory without gaps")
-    if any(0 in g.stride() and g.numel() > 1 and d.data_ptr() != g.data_ptr() for g, d in zip(grads, dense)) or _overlap(dense, outs):
-        raise ValueError("clip_grads_: a gradient or output shares memory with another output (or with itself)")
     device = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
     total = torch.empty(1, dtype=torch.float64, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)

@@ -72,6 +72,78 @@ def test_overlap_rule():
     assert not F._overlap([t[:0], t[:0]], [t[:0], t[:0]])
 
 
+def _bytes(t):
+    """The address of every byte of t, with repetitions."""
+    places = [t.data_ptr()]
+    for st, n in zip(t.stride(), t.shape):
+        places = [p + st * t.element_size() * i for p in places for i in range(n)]
+    return [p + k for p in places for k in range(t.element_size())]
+
+
+def _overlap_by_enumeration(grads, outs):
+    taken = {}
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        own = _bytes(o)
+        if len(set(own)) < len(own):
+            return True
+        for p in own:
+            if p in taken:
+                return True
+            taken[p] = i
+    for g, o in zip(grads, outs):
+        if g.data_ptr() == o.data_ptr() and g.dtype == o.dtype:
+            continue
+        if any(p in taken for p in _bytes(g)):
+            return True
+    return False
+
+
+OVERLAPS = [F._overlap] + ([b.ext().overlap] if b.ext() is not None else [])
+
+
+@pytest.mark.parametrize("overlap", OVERLAPS)
+def test_overlap_of_tensors_with_gaps(overlap):
+    s = torch.zeros(40, 30)
+    shared = [[s[:, ::2], s[:, ::2]], [s[:, ::2], s], [s[::2], s[:, ::2]], [s[:, :11], s[:, 10:]], [s[:, :20:3], s.t()[3:]],
+              [torch.zeros(64).as_strided((4, 4), (2, 1))], [torch.zeros(64).as_strided((3, 4), (1, 2))], [s[:1].expand(9, 30)],
+              [s[3], s[:, 7]]]
+    apart = [[s[:, ::2], s[:, 1::2]], [s[:, :10], s[:, 10:]], list(s.unbind(1)), [s[::2], s[1::2, ::2], s[1::2, 1::2]],
+             [torch.zeros(64).as_strided((2, 3), (3, 2))], [s.t()], [s[:, None, ::3], s[:, 1::3], s.t()[2::3]], [s[:0], s]]
+    for want, lists in ((True, shared), (False, apart)):
+        for ts in lists:
+            assert _overlap_by_enumeration(ts, ts) == want
+            assert overlap(ts, ts) == want
+    wide = torch.zeros(1 << 20).as_strided((1 << 9, 1 << 9), (1 << 11, 2))    # no search over elements
+    assert overlap([wide, wide.t()], [wide, wide.t()]) and not overlap([wide], [wide])
+
+
+@pytest.mark.parametrize("overlap", OVERLAPS)
+def test_overlap_rule_on_random_views(overlap):
+    """Against the addresses of every byte: views of any strides, types mixed, in place and into other views."""
+    import random
+    rng = random.Random(5)
+    pool = torch.zeros(4096, dtype=torch.uint8)
+    seen = [0, 0]
+
+    def view(dtype=None, like=None):
+        dtype = dtype or rng.choice([torch.float32, torch.float16])
+        es = torch.empty(0, dtype=dtype).element_size()
+        base = pool[rng.randrange(0, 300) * es:]
+        base = base[:base.numel() // es * es].view(dtype)
+        if like is not None:
+            return base.as_strided(like.shape, like.stride())
+        shape = [rng.choice([1, 2, 3, 5]) for _ in range(rng.randint(0, 3))]
+        return base.as_strided(shape, [rng.choice([1, 2, 3, 4, 6, 10, 12, 30]) for _ in shape])
+
+    for _ in range(1500):
+        grads = [view() for _ in range(rng.randint(1, 3))]
+        outs = grads if rng.random() < 0.6 else [view(rng.choice([g.dtype, torch.float32]), g) for g in grads]
+        want = _overlap_by_enumeration(grads, outs)
+        seen[want] += 1
+        assert overlap(grads, outs) == want, [(t.shape, t.stride(), t.data_ptr() - pool.data_ptr()) for t in grads + outs]
+    assert min(seen) > 200
+
+
 def test_dense_views():
     w = torch.zeros(8, 6, 3, 3).contiguous(memory_format=torch.channels_last)
     assert F._dense(w).data_ptr() == w.data_ptr() and F._dense(w.t() if w.dim() == 2 else w).data_ptr() == w.data_ptr()

@@ -463,6 +463,18 @@ def test_clip_layouts_and_overlap(front):
             F.clip_grads_(grads, 1.0, out=out)
 
 
+def test_clip_refuses_shared_memory_in_gradients_with_gaps(front):
+    """Gradients that do not fill their memory are copied on their way: their own addresses count all the same."""
+    s, line = randn((40, 30), torch.float32, 2), randn((64,), torch.float32, 3)
+    kept = s.clone(), line.clone()
+    for grads in ([s[:, ::2], s], [s[:, ::2], s[:, ::2]], [line.as_strided((4, 4), (2, 1))], [s[:, :11], s[:, 10:]]):
+        with pytest.raises(ValueError, match="shares memory"):
+            F.clip_grads_(grads, 0.5)
+        assert torch.equal(s, kept[0]) and torch.equal(line, kept[1])
+    check_clip([s[:, 1::2], s[:, ::2]], 0.5, 2.0)     # side by side
+    check_clip([s[:, :10], s[:, 10:]], 0.1, 2.0)
+
+
 def test_clip_moves_the_version(front):
     """A gradient that autograd still needs must not change unseen."""
     a = randn((10,), torch.float32, 1).requires_grad_(True)
