@@ -1,7 +1,7 @@
 // fpemu_train.hip -- operators of a language model's training step that run beside the emulated cast: rows in the
 // order of their group (a router's experts, a vocabulary's entries), the scaled embedding lookup with the gradient of
 // its table, and the norm and clipping of a whole list of gradients.  Sums are held in 32 bits (table gradient) or
-// 64 bits (norms) and rounded once, when they are stored.  No floating-point atomics: every sum has one fixed order,
+// 64 bits (norms; squares of 16-bit values are added in fours in 32 bits first) and rounded once, when they are stored.  No floating-point atomics: every sum has one fixed order,
 // so a call repeated on the same inputs gives the same bits.
 #include <hip/hip_runtime.h>
 #include <math.h>

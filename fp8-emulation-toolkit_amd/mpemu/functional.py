@@ -338,7 +338,9 @@ def _over_ranks(total, order, group):
 
 def grad_norm(grads, norm_type=2.0):
     """The norm (1, 2 or inf) of all elements of a list of tensors as one vector: float32, 0-d, on the device.  The sum runs
-    in 64 bits, so neither large nor many elements overflow or drown it."""
+    in 64 bits, so neither large nor many elements overflow or drown it (squares of 16-bit elements, exact in fp32, are
+    added in fours there first wherever fp32's range holds them: two roundings of 2^-24 at most).  No derivative of the norm
+    is kept."""
     who = "grad_norm"
     order = _order(norm_type, who)
     grads = _list(grads)
@@ -361,9 +363,9 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None, error_if_nonfinite=Fal
 
     In place, or into `out`: a list of the same shapes and strides, each of the gradient's type or float32 (16-bit model
     gradients clipped into fp32 master gradients in one pass).  No tensor may share memory with another one's output, nor
-    an output's elements with each other (views that interleave are told from views that overlap).  A norm that is not finite gives what the arithmetic gives (NaN, or zeros and NaN), as
-    torch.nn.utils.clip_grad_norm_ does; error_if_nonfinite=True reads the norm on the host first and raises instead,
-    with every gradient as it was.
+    an output's elements with each other (views that interleave are told from views that overlap).  A norm that is not
+    finite gives what the arithmetic gives (NaN, or zeros and NaN), as torch.nn.utils.clip_grad_norm_ does;
+    error_if_nonfinite=True reads the norm on the host first and raises instead, with every gradient as it was.
 
     group: a torch.distributed process group over whose ranks the gradients are sharded: the norm is that of all ranks'
     gradients (one all-reduce of one word), every rank's list on one device of its own, an empty one included."""

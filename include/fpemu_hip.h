@@ -379,8 +379,9 @@ int fpemu_grouped_gemm_wgrad(void *dw, const void *a, const void *b, const int32
 
 /* Norm of a list of gradients as ONE vector, and their clipping; types may differ within a list.  `in` is the gradient,
  * `out` (fpemu_clip_multi only) receives the clipped one: the same buffer, or another one of the same type or fp32.
- *   fpemu_grad_norm_multi : *sum = sum of |g|^p (p = 1, 2) or max |g| (infinity) over all elements, in 64 bits; a NaN
- *                           stays a NaN.  norm (or NULL) receives the norm itself.  ws:
+ *   fpemu_grad_norm_multi : *sum = sum of |g|^p (p = 1, 2) or max |g| (infinity) over all elements, in 64 bits (p = 2:
+ *                           the exact squares of 16-bit elements are added in fours in fp32 first, where its range holds
+ *                           them: off by two roundings at most, 2^-23 of each four's sum); a NaN stays a NaN.  norm (or NULL) receives the norm itself.  ws:
  *                           fpemu_grad_norm_workspace_bytes(count) bytes, 8-byte aligned.
  *   fpemu_clip_multi      : out = in * min(1, max_norm / (norm + 1e-6)), the norm taken from *sum on the device (ranks
  *                           that hold shards add their sums up in between); norm (or NULL) receives it.

@@ -446,6 +446,58 @@ def test_clip_not_finite(p, front):
     assert float(g[0].abs().sum()) == 0.0 and bool(g[1].isnan().all())                       # inf * 0, as torch
 
 
+SIXTEEN = [torch.bfloat16, torch.float16]
+FOURS = {   # eight neighbours: two fours whose squares are added in fp32 where its range holds them, in 64 bits where not
+    torch.bfloat16: [[1e30] * 8, [1e-30] * 8, [1e30] * 4 + [0.0] * 4, [0.0] * 4 + [1e-30] * 4, [1e-30] * 4 + [1.0] * 4,
+                     [1.0] * 4 + [1e-38] * 4, [1e-39, 0, 0, 0, 0, 0, 1e-39, 0], [3e38, 0, 0, 0, 0, 0, 0, 0], [1e-20, 1e10, 3.0, 0, 0, 0, -7.0, 0],
+                     [2.0 ** -45] * 8, [2.0 ** -46] * 8, [0.75 * 2.0 ** -44, 0, 0, 0] * 2, [2.0 ** 61] * 8, [2.0 ** 61.5] * 8,
+                     [2.0 ** 63, 0, 0, 0, 1.0, 0, 0, 0], [1.9 * 2.0 ** 63, 0, 0, 0, 0, 0, 0, 2.0 ** -60]],
+    torch.float16: [[65504.0] * 8, [2.0 ** -24] * 8, [65504.0] * 4 + [0.0] * 4, [0.0] * 4 + [2.0 ** -24] * 4,
+                    [2.0 ** -24] * 4 + [65504.0] * 4, [2.0 ** -24, 0, 0, 0, 0, 0, 0, 0], [0.0] * 7 + [-60000.0], [2.0 ** -14, 6e-8, 1.0, -3e4] * 2]}
+
+
+@pytest.mark.parametrize("dtype,eight", [(t, e) for t in SIXTEEN for e in FOURS[t]])
+@pytest.mark.parametrize("repeat,tail", [(1, 0), (1, 5), (130, 3), (3000, 7)])
+def test_norm_of_16_bit_values_over_their_range(dtype, eight, repeat, tail):
+    """Squares beyond fp32's range, below it, and beside zeros.  A four's sum is off by two roundings, 2^-23 at most, its root
+    by half of that; the norm is rounded once more, 2^-24."""
+    values = (eight * (repeat + 1))[:8 * repeat + tail]
+    g = torch.tensor(values, dtype=torch.float64, device=DEV).to(dtype)
+    for p in (1.0, 2.0, math.inf):
+        want = norm_reference([g], p)
+        got = float(F.grad_norm([g], p))
+        if want >= 2.0 ** 128 * (1 - 2.0 ** -25):   # rounds to infinity
+            assert got == math.inf
+        else:
+            assert abs(got - want) <= want * (2.0 ** -23 + 2.0 ** -40) + 2.0 ** -150, (p, got, want)
+    want = norm_reference([g], 2.0)
+    if want < 2.0 ** 127:
+        limit = torch.tensor(0.3 * want).item()
+        coef = min(1.0, limit / (want + 1e-6))
+        v = g.double() * coef
+        F.clip_grads_([g], limit)
+        close(g, v, v.abs() * 2.0 ** -21)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("at", [0, 5, 4001, 9999])
+def test_clip_of_16_bit_values_not_finite(p, dtype, at, front):
+    g = torch.ones(10001, device=DEV, dtype=dtype)
+    g[at] = math.nan
+    kept = g.clone()
+    with pytest.raises(RuntimeError, match="norm of the gradients"):
+        F.clip_grads_([g], 1.0, p, error_if_nonfinite=True)
+    assert torch.equal(g.nan_to_num(5.0), kept.nan_to_num(5.0))
+    assert math.isnan(float(F.grad_norm([g], p)))
+    g[at] = -math.inf
+    assert float(F.clip_grads_([g], 1.0, p)) == math.inf
+    assert bool(g[at].isnan()) and float(g.nan_to_num(0.0).abs().sum()) == 0.0    # inf * 0, as torch
+    g = torch.ones(10001, device=DEV, dtype=dtype)
+    g[at], g[(at + 1) % 10001] = math.inf, math.nan
+    assert math.isnan(float(F.clip_grads_([g], 1.0, p))) and bool(g.isnan().all())
+
+
 def test_clip_layouts_and_overlap(front):
     conv = randn((8, 6, 3, 3), torch.float32, 1).contiguous(memory_format=torch.channels_last)
     strided = randn((40, 30), torch.float32, 2)
