@@ -179,10 +179,13 @@ def grouped_mm(x, weight, offsets):
     int64, groups + 1 entries, not decreasing, as group_rows returns them.  The sizes stay on the device.  Groups may be
     empty; rows outside every group are zero in y and in the gradient of x, and add to no gradient of weight.  16-bit types
     multiply on the matrix cores with fp32 sums; fp32 runs the k-ascending fmaf chain of the c-model
-    (mpemu.cmodel.simple, accumulation "fma"), whatever set_accumulation says.  Differentiable once, in x and weight."""
+    (mpemu.cmodel.simple, accumulation "fma"), whatever set_accumulation says.  Under torch.autocast x and weight are cast to
+    its type first, as torch's own matrix products do.  Differentiable once, in x and weight."""
     who = "grouped_mm"
     _floating(x, "x", who)
     _floating(weight, "weight", who)
+    if torch.is_autocast_enabled("cuda"):
+        x, weight = (t.to(torch.get_autocast_dtype("cuda")) for t in (x, weight))
     _integers(offsets, "offsets", who)
     _one_device(who, x, weight, offsets)
     if x.dtype != weight.dtype:

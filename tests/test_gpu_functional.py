@@ -15,6 +15,7 @@ from mpemu.pytquant.hip import _binding as hip
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
+SIXTEEN = TYPES[1:]
 TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}
 
 
@@ -337,6 +338,30 @@ def test_grouped_mm_strides_types_and_needs(front):
     close(x.grad[:10], (w.detach()[0].double().sum(1))[None].expand(10, 64).clone(), 64 * 64 * 2.0 ** -24)
 
 
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("given", TYPES)
+def test_grouped_linear_under_autocast(dtype, given, front):
+    """fp32 master weights, activations of any type: cast to autocast's type, as torch.nn.Linear does beside it."""
+    from mpemu.module_wrappers import GroupedLinear, GroupedMatmul
+    layer, lin, o = GroupedLinear(3, 40, 24, device=DEV), torch.nn.Linear(40, 24, device=DEV), offsets_of([10, 0, 21])
+    x = randn((31, 40), given, 1).requires_grad_(True)
+    dy = randn((31, 24), dtype, 2)
+    with torch.autocast("cuda", dtype=dtype):
+        y = layer(x, o)
+        assert y.dtype == lin(x).dtype == dtype
+        got = torch.autograd.grad(y, (x, layer.weight), dy)
+        assert torch.equal(GroupedMatmul()(x, layer.weight.transpose(1, 2), o), y)
+        with torch.no_grad():
+            assert torch.equal(layer(x, o), y)
+        with torch.autocast("cuda", enabled=False):
+            assert F.grouped_mm(x.float(), layer.weight.transpose(1, 2), o).dtype == torch.float32
+    a, w = x.detach().to(dtype).requires_grad_(True), layer.weight.detach().to(dtype).requires_grad_(True)
+    want = F.grouped_mm(a, w.transpose(1, 2), o)
+    assert torch.equal(y, want)
+    for g, t, d in zip(got, (x, layer.weight), torch.autograd.grad(want, (a, w), dy)):
+        assert g.dtype == t.dtype and torch.equal(g, d.to(t.dtype))
+
+
 def test_grouped_mm_gradient_against_differences():
     x, w, o = randn((5, 3), torch.float32, 1).requires_grad_(True), randn((2, 3, 4), torch.float32, 2).requires_grad_(True), offsets_of([2, 3])
     v = randn((5, 4), torch.float32, 3)
@@ -446,7 +471,6 @@ def test_clip_not_finite(p, front):
     assert float(g[0].abs().sum()) == 0.0 and bool(g[1].isnan().all())                       # inf * 0, as torch
 
 
-SIXTEEN = [torch.bfloat16, torch.float16]
 FOURS = {   # eight neighbours: two fours whose squares are added in fp32 where its range holds them, in 64 bits where not
     torch.bfloat16: [[1e30] * 8, [1e-30] * 8, [1e30] * 4 + [0.0] * 4, [0.0] * 4 + [1e-30] * 4, [1e-30] * 4 + [1.0] * 4,
                      [1.0] * 4 + [1e-38] * 4, [1e-39, 0, 0, 0, 0, 0, 1e-39, 0], [3e38, 0, 0, 0, 0, 0, 0, 0], [1e-20, 1e10, 3.0, 0, 0, 0, -7.0, 0],
