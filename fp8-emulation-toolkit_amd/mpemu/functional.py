@@ -61,7 +61,7 @@ def _refuse_capture(who, *ts):
     """Without the native front the stream of a leaf's accumulation node is unknown, and a captured backward pass of a leaf
     that an eager graph still holds ends the process: no captured gradients there."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts) and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("%s: capturing a backward pass needs the native extension (_mpemu_torch.so)" % who)
+        raise RuntimeError("%s: capturing a backward pass needs the native extension (_mpemu_torch.so), with tracing off" % who)
 
 
 # ---- rows by group ------------------------------------------------------------------------------------------------------
@@ -103,16 +103,24 @@ class _Embedding(Function):
         return None, _hip.embedding_grad_(grad.contiguous(), ids, dweight, ctx.scale, ctx.padding), None, None
 
 
+def _number(scale):
+    """scale as a float: a tensor that autograd follows would lose its derivative here."""
+    if torch.is_tensor(scale) and (scale.requires_grad or forward_ad.unpack_dual(scale).tangent is not None):
+        raise TypeError("embedding: scale is a number and has no derivative; multiply the result by a scale that is learned")
+    return float(scale)
+
+
 def embedding(ids, weight, scale=1.0, padding_idx=None):
     """scale * weight[ids]: ids of any shape, weight [entries, width]; the result has shape ids.shape + (width,).
 
     The gradient of the table is dense and deterministic: tokens are sorted by entry and every entry's rows are summed in
     fp32, in token order, and rounded once.  padding_idx (negative: from the end): that entry's gradient is zero.  An id
     outside the table is not an error that the device could raise: its row of the result is NaN, it adds to no gradient.
-    Differentiable once."""
+    Differentiable once, in weight; scale is a number."""
     who = "embedding"
     _integers(ids, "ids", who)
     _floating(weight, "weight", who)
+    scale = _number(scale)
     _one_device(who, ids, weight)
     if weight.dim() != 2:
         raise ValueError("embedding: weight must be 2-D, got %s" % (tuple(weight.shape),))
@@ -126,10 +134,10 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
         padding %= weight.shape[0]
     ext = _native()
     if ext is not None:
-        return ext.embedding(ids, weight, float(scale), padding)
+        return ext.embedding(ids, weight, scale, padding)
     _refuse_tangents(who, weight)
     _refuse_capture(who, weight)
-    return _Embedding.apply(ids.contiguous(), weight, float(scale), padding)
+    return _Embedding.apply(ids.contiguous(), weight, scale, padding)
 
 
 # ---- products by group ----------------------------------------------------------------------------------------------------

@@ -129,7 +129,7 @@ class ScaledEmbedding(nn.Embedding):
 
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, device=None, dtype=None):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
-        self.scale = float(scale)
+        self.scale = F._number(scale)
 
     def forward(self, input: torch.Tensor):
         return F.embedding(input, self.weight, scale=self.scale, padding_idx=self.padding_idx)

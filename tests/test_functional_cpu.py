@@ -50,6 +50,17 @@ def test_dual_tensors_are_refused_before_anything_else():
         F._refuse_tangents("x", FLT)
 
 
+def test_a_scale_to_learn_is_refused():
+    from torch.autograd import forward_ad
+    learned = torch.nn.Parameter(torch.tensor(2.0))
+    for call in (lambda: F.embedding(INT, FLT, scale=learned), lambda: ScaledEmbedding(4, 4, scale=learned)):
+        with pytest.raises(TypeError, match="scale"):
+            call()
+    with forward_ad.dual_level(), pytest.raises(TypeError, match="scale"):
+        F.embedding(INT, FLT, scale=forward_ad.make_dual(torch.tensor(2.0), torch.tensor(1.0)))
+    assert ScaledEmbedding(4, 4, scale=torch.tensor(2.0)).scale == ScaledEmbedding(4, 4, scale=2).scale == 2.0
+
+
 def test_values_refused_without_gpu():
     with pytest.raises(ValueError):
         F.grad_norm([], norm_type=3.0)
