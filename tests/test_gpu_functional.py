@@ -580,6 +580,39 @@ def test_clip_over_a_group_of_one(front, tmp_path):
         dist.destroy_process_group()
 
 
+def _one_rank_rccl(rank, store, out):
+    import os
+    import sys
+    import torch.distributed as dist
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fp8-emulation-toolkit_amd"))
+    from mpemu import functional
+    from mpemu.sharded import group_backend
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+    dist.init_process_group("nccl", init_method="file://" + store, rank=0, world_size=1, device_id=dev)
+    assert group_backend() == "nccl"
+    same = []
+    for p in (1.0, 2.0, math.inf):
+        for odd in (1.0, math.inf, math.nan):
+            g = [torch.linspace(-3, 2, 1000, device=dev).bfloat16(), torch.full((77,), 0.5, device=dev)]
+            g[1][5] = odd
+            twin = [t.clone() for t in g]
+            a, b = functional.clip_grads_(g, 0.5, p, group=dist.group.WORLD), functional.clip_grads_(twin, 0.5, p)
+            same += [torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) and torch.equal(x.isnan(), y.isnan())
+                     for x, y in zip([a] + g, [b] + twin)]
+    same.append(float(functional.clip_grads_([], 1.0, group=dist.group.WORLD)) == 0.0)
+    torch.save(same, out)
+    dist.destroy_process_group()
+
+
+def test_clip_over_an_rccl_group_of_one(tmp_path):
+    """The branch that reduces the word on the device, through a communicator of one rank."""
+    store, out = str(tmp_path / "store"), str(tmp_path / "out")
+    torch.multiprocessing.spawn(_one_rank_rccl, args=(store, out), nprocs=1)
+    same = torch.load(out, weights_only=True)
+    assert len(same) == 28 and all(same), same
+
+
 @pytest.mark.parametrize("sharded", [False, True])
 def test_clip_refuses_a_norm_beyond_float32(front, sharded, tmp_path):
     """Four times 3e38: the 64-bit sum is finite, the norm (6e38) is not a float32; 4e19: the sum of squares is not one, the norm is."""
@@ -613,6 +646,55 @@ def test_clip_grad_norm_of_parameters(front):
     for p, t in zip(ps, twin):
         v = t.double() * (1.5 / (want + 1e-6))
         close(p.grad, v, v.abs() * 2.0 ** -21)
+
+
+# ---- beyond 32 bits, and nothing at all --------------------------------------------------------------------------------------------
+def test_addresses_beyond_32_bits():
+    """Tables, rows and gradients of more than 2^31 elements (over 4 GB): the last ones are read and written where they are."""
+    vocab, width = (1 << 20) + 7, 2056
+    table = torch.zeros((vocab, width), dtype=torch.bfloat16, device=DEV)
+    ids = torch.tensor([vocab - 1, 0, vocab - 1, 1 << 20, vocab, 5], device=DEV)
+    table[ids[ids < vocab]] = randn((5, width), torch.bfloat16, 1)
+    table.requires_grad_(True)
+    out = F.embedding(ids, table, scale=2.0)
+    assert torch.equal(out[[0, 1, 2, 3, 5]], table.detach()[ids[[0, 1, 2, 3, 5]]] * 2.0) and bool(out[4].isnan().all())
+    dout = randn(out.shape, out.dtype, 2)
+    dt, = torch.autograd.grad(out, (table,), dout)
+    for v in (0, 5, 1 << 20, vocab - 1):
+        want = dout[ids == v].double().sum(0) * 2.0
+        close(dt[v], want, dout[ids == v].double().abs().sum(0) * 2.0 * 4 * 2.0 ** -24)
+    assert int(dt.count_nonzero()) == int(dt[[0, 5, 1 << 20, vocab - 1]].count_nonzero())
+    del out
+    norm = F.clip_grads_([dt], 0.5)
+    want = norm_reference([dt[[0, 5, 1 << 20, vocab - 1]]], 2.0)     # now clipped to 0.5; each element rounded to bf16, a few times fp32
+    assert abs(want - 0.5) <= 0.5 * (2.0 ** -8 + 2.0 ** -20) and float(norm) > 0.5
+    # the same memory as rows of a product: the last group lies behind 4 GB
+    x, w = table.detach(), randn((3, width, 40), torch.bfloat16, 3).requires_grad_(True)
+    first = vocab - 300
+    o = torch.tensor([7, first - 1000, first, vocab - 1], dtype=torch.int32, device=DEV)
+    y = F.grouped_mm(x.requires_grad_(True), w, o)
+    dy = randn(y.shape, y.dtype, 4)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    X, W, DY = x.detach()[first:vocab - 1].double(), w.detach()[2].double(), dy[first:vocab - 1].double()
+    close(y.detach()[first:vocab - 1], X @ W, (X.abs() @ W.abs()) * ((width + 1) * 2.0 ** -23))
+    close(dx[first:vocab - 1], DY @ W.t(), (DY.abs() @ W.t().abs()) * (41 * 2.0 ** -23))
+    close(dw[2], X.t() @ DY, (X.t().abs() @ DY.abs()) * (300 * 2.0 ** -23))
+    assert float(y.detach()[vocab - 1].abs().sum()) == 0.0 and float(dx[vocab - 1].abs().sum()) == 0.0 and float(dx[:7].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_columns_at_all(dtype, front):
+    """An empty contraction is zero; no columns are no results."""
+    o = offsets_of([2, 3])
+    for k, n in ((0, 8), (0, 5), (8, 0), (0, 0)):
+        x, w = torch.ones(6, k, dtype=dtype, device=DEV, requires_grad=True), torch.ones(2, k, n, dtype=dtype, device=DEV, requires_grad=True)
+        y = F.grouped_mm(x, w, o)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert y.shape == (6, n) and float(y.detach().abs().sum()) == float(dx.abs().sum()) == float(dw.abs().sum()) == 0.0
+        assert dx.shape == x.shape and dw.shape == w.shape
+    table = torch.ones(4, 0, dtype=dtype, device=DEV, requires_grad=True)
+    out = F.embedding(torch.tensor([1, 9], device=DEV), table)
+    assert out.shape == (2, 0) and torch.autograd.grad(out, (table,), torch.ones_like(out))[0].shape == (4, 0)
 
 
 # ---- streams, capture, repetition -------------------------------------------------------------------------------------------------
