@@ -41,11 +41,17 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // (the implicit-convolution operand: rows of the padded image shifted by the filter tap)
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int BK = 16;  // VALU kernel: 128 x 128 x 16 tiles (64 x 64 x 16 for small problems)
+constexpr int BK = 16;  // VALU kernel: 128 x 128 x 16 tiles (64 x 64 x 16 or 32 x 32 x 32 for small problems)
+template <int T> constexpr int seqk_depth() { return T < 64 ? 32 : BK; }
 #ifndef FPEMU_SEQK_T64_BELOW
-#define FPEMU_SEQK_T64_BELOW 1024  // fewer 128 x 128 tiles than this (per launch): 64 x 64 tiles.  Measured, fraction of the
-                                   // 78.6 TFLOP/s VALU peak with 128 / 64 tiles: 768x768x4096 0.077 / 0.205, 2048^3 0.54 / 0.61,
-                                   // 3072x3072x2048 (576 tiles) 0.55 / 0.65, 4096^3 (1024 tiles) 0.72 / 0.67
+#define FPEMU_SEQK_T64_BELOW 1024  // fewer 128 x 128 tiles than this (per launch): 64 x 64 tiles.  us with 128 / 64: 1536^3 437 / 204,
+                                   // 2048^3 (256 tiles) 582 / 371, 2944x2944x2048 (529) 977 / 730, 3584x3584x2048 (784) 1174 / 1040,
+                                   // 4096^3 (1024) 2456 / 2569
+#endif
+#ifndef FPEMU_SEQK_T32_MAX
+#define FPEMU_SEQK_T32_MAX 256     // up to this many 64 x 64 tiles (one per CU, so one wave per SIMD): 32 x 32 tiles.  us with 64 / 32:
+                                   // 768x768x768 (144 tiles) 76 / 45, 768x768x4096 392 / 224, 1024^3 (256) 100 / 74, 1152^3 (324)
+                                   // 114 / 133, 1536^3 (576) 198 / 240; transposed operands alike
 #endif
 #ifndef FPEMU_GEMM_MBK
 #define FPEMU_GEMM_MBK 32
@@ -75,7 +81,10 @@ struct Operand {
 // bounds tests in the loop.
 template <bool KCONT, int TBK, int ROWS>
 __device__ __forceinline__ void tile_coords(int h, int tid, int &r, int &k) {
-  if constexpr (KCONT) {  // thread -> (row, 4 consecutive k): 4 threads per row, 64 rows per pass
+  if constexpr (KCONT && ROWS < 64) {   // thread -> (row, 4 consecutive k): 32 rows and 32 k per pass
+    r = tid >> 3;
+    k = h * 32 + (tid & 7) * 4;
+  } else if constexpr (KCONT) {  // thread -> (row, 4 consecutive k): 4 threads per row, 64 rows per pass
     constexpr int RP = ROWS / 64;
     r = (h % RP) * 64 + (tid >> 2);
     k = (h / RP) * 16 + (tid & 3) * 4;
@@ -269,91 +278,96 @@ __device__ __forceinline__ float chain_start(const Batch &bt, const float *C, in
 // CHAIN = true : acc starts at C's current value and C = acc             (the conv kernels: MMEngine loads
 //                C, continues the chain and stores it back, simple_mm_engine.cpp:18-24)
 // T = tile edge: 128 (a lane owns 8 x 8 results: two 4-row and two 4-column groups 64 apart), or 64 (4 x 4) for problems
-// with fewer 128 x 128 tiles than CUs -- a chain cannot be split along k, so only smaller tiles spread them.
+// with fewer 128 x 128 tiles than CUs -- a chain cannot be split along k, so only smaller tiles spread them -- or 32
+// (2 x 2, k tiles of 32) where 64 x 64 ones would leave a SIMD a single wave, which issues no instruction every cycle it could.
 template <bool A_KCONT, bool B_KCONT, bool CHAIN, bool FULL, int T>
 __global__ __launch_bounds__(NT) void gemm_seqk_kernel(Operand A, Operand B, float *C, int64_t ldc,
                                                        int c_vec, float alpha, float beta,
                                                        int tiles_m, int tiles_n, Batch bt) {
-  static_assert(T == 128 || T == 64, "tile edge");
-  constexpr int H = T / 64;  // 4-row / 4-column groups per lane and dimension
+  static_assert(T == 128 || T == 64 || T == 32, "tile edge");
+  constexpr int G = T < 64 ? 2 : 4, H = T < 64 ? 1 : T / 64;  // H groups of G rows / columns per lane and dimension
+  constexpr int DK = seqk_depth<T>();
+  typedef float vec_g __attribute__((ext_vector_type(G)));
   A.p += (int64_t)blockIdx.y * bt.sa;
   B.p += (int64_t)blockIdx.y * bt.sb;
   C += (int64_t)blockIdx.y * bt.sc;
-  __shared__ __attribute__((aligned(16))) float As[2][BK * ldt<T>()];
-  __shared__ __attribute__((aligned(16))) float Bs[2][BK * ldt<T>()];
+  __shared__ __attribute__((aligned(16))) float As[2][DK * ldt<T>()];
+  __shared__ __attribute__((aligned(16))) float Bs[2][DK * ldt<T>()];
   const int tid = threadIdx.x;
   int tm, tn;
   tile_of_block(tiles_m, tiles_n, tm, tn);
   const int m0 = tm * T, n0 = tn * T;
-  const int ty = tid >> 4, tx = tid & 15;  // lane owns rows {ty*4.., 64+ty*4..} x cols {tx*4.., 64+tx*4..}
+  const int ty = tid >> 4, tx = tid & 15;  // lane owns rows {ty*G.., 64+ty*G..} x cols {tx*G.., 64+tx*G..}
   const int K = A.K;
 
-  f32x2 acc2[4 * H][2 * H];  // acc2[i][j] = outputs (i, 2j) and (i, 2j+1)
+  f32x2 acc2[G * H][G / 2 * H];  // acc2[i][j] = outputs (i, 2j) and (i, 2j+1)
 #pragma unroll
-  for (int i = 0; i < 4 * H; i++)
+  for (int i = 0; i < G * H; i++)
 #pragma unroll
-    for (int j = 0; j < 4 * H; j++) {
+    for (int j = 0; j < G * H; j++) {
       float v = 0.f;
       if constexpr (CHAIN) {
-        const int r = m0 + (i >> 2) * 64 + ty * 4 + (i & 3), c = n0 + (j >> 2) * 64 + tx * 4 + (j & 3);
+        const int r = m0 + i / G * 64 + ty * G + i % G, c = n0 + j / G * 64 + tx * G + j % G;
         if (r < A.R && c < B.R) v = chain_start(bt, C, (int64_t)r * ldc + c, r);
       }
       acc2[i][j >> 1][j & 1] = v;
     }
 
   constexpr int LDT = ldt<T>();
-  f32x4 pa[BK * T / 1024], pb[BK * T / 1024];
+  f32x4 pa[DK * T / 1024], pb[DK * T / 1024];
   const float *abase = A.p, *bbase = B.p;
-  tile_load<A_KCONT, FULL, BK, T>(A, abase, m0, 0, tid, pa);
-  tile_load<B_KCONT, FULL, BK, T>(B, bbase, n0, 0, tid, pb);
-  tile_store<A_KCONT, BK, T>(As[0], tid, pa);
-  tile_store<B_KCONT, BK, T>(Bs[0], tid, pb);
+  tile_load<A_KCONT, FULL, DK, T>(A, abase, m0, 0, tid, pa);
+  tile_load<B_KCONT, FULL, DK, T>(B, bbase, n0, 0, tid, pb);
+  tile_store<A_KCONT, DK, T>(As[0], tid, pa);
+  tile_store<B_KCONT, DK, T>(Bs[0], tid, pb);
   __syncthreads();
 
   int cur = 0;
-  const int kt = (K + BK - 1) / BK, total = kt * bt.nseg;
+  const int kt = (K + DK - 1) / DK, total = kt * bt.nseg;
   int nk0 = 0;  // k offset of the tile being prefetched
   for (int it = 0; it < total; it++) {
     const bool more = it + 1 < total;
     if (more) {
-      nk0 += BK;
+      nk0 += DK;
       if (nk0 >= K) {  // next k segment
         nk0 = 0;
         abase += bt.ka;
         bbase += bt.kb;
       }
-      tile_load<A_KCONT, FULL, BK, T>(A, abase, m0, nk0, tid, pa);
-      tile_load<B_KCONT, FULL, BK, T>(B, bbase, n0, nk0, tid, pb);
+      tile_load<A_KCONT, FULL, DK, T>(A, abase, m0, nk0, tid, pa);
+      tile_load<B_KCONT, FULL, DK, T>(B, bbase, n0, nk0, tid, pb);
     }
     const float *as = As[cur], *bs = Bs[cur];
 #pragma unroll 2
-    for (int kk = 0; kk < BK; kk++) {
-      float a[4 * H];
-      f32x2 b2[2 * H];
+    for (int kk = 0; kk < DK; kk++) {
+      float a[G * H];
+      f32x2 b2[G / 2 * H];
 #pragma unroll
       for (int h = 0; h < H; h++) {
-        const f32x4 av = *reinterpret_cast<const f32x4 *>(&as[kk * LDT + h * 64 + ty * 4]);
-        const f32x4 bv = *reinterpret_cast<const f32x4 *>(&bs[kk * LDT + h * 64 + tx * 4]);
+        const vec_g av = *reinterpret_cast<const vec_g *>(&as[kk * LDT + h * 64 + ty * G]);
+        const vec_g bv = *reinterpret_cast<const vec_g *>(&bs[kk * LDT + h * 64 + tx * G]);
 #pragma unroll
-        for (int e = 0; e < 4; e++) a[4 * h + e] = av[e];
-        b2[2 * h] = f32x2{bv[0], bv[1]};
-        b2[2 * h + 1] = f32x2{bv[2], bv[3]};
+        for (int e = 0; e < G; e++) a[G * h + e] = av[e];
+#pragma unroll
+        for (int e = 0; e < G; e += 2) b2[(G * h + e) / 2] = f32x2{bv[e], bv[e + 1]};
       }
-      // Two chains side by side.  (Packed fp32 instructions are switched off for every unit, see the Makefile: they ran this
-      // loop no faster, 55.6 TFLOP/s at 4096^3 with and without them.)
+      // Two chains side by side.  Packed fp32 instructions are switched off for every unit (see the Makefile), so each step is a
+      // multiply and an add of its own.  Where a SIMD has several waves that costs nothing (4096^3 55.6 TFLOP/s with and without
+      // them, 2048^3 39.9 -> 41.6); a single wave issues too few instructions then (768^3 14.1 -> 11.4), hence the 32 x 32 tiles
+      // for such problems (768^3 20).
 #pragma unroll
-      for (int i = 0; i < 4 * H; i++) {
+      for (int i = 0; i < G * H; i++) {
         const f32x2 ai = {a[i], a[i]};
 #pragma unroll
-        for (int j = 0; j < 2 * H; j++) {
+        for (int j = 0; j < G / 2 * H; j++) {
           const f32x2 p = ai * b2[j];      // rounded products: values of their own (contraction is off)
           acc2[i][j] = acc2[i][j] + p;     // k ascending, one add per step
         }
       }
     }
     if (more) {
-      tile_store<A_KCONT, BK, T>(As[cur ^ 1], tid, pa);
-      tile_store<B_KCONT, BK, T>(Bs[cur ^ 1], tid, pb);
+      tile_store<A_KCONT, DK, T>(As[cur ^ 1], tid, pa);
+      tile_store<B_KCONT, DK, T>(Bs[cur ^ 1], tid, pb);
     }
     __syncthreads();
     cur ^= 1;
@@ -369,34 +383,34 @@ __global__ __launch_bounds__(NT) void gemm_seqk_kernel(Operand A, Operand B, flo
 #pragma unroll
   for (int ih = 0; ih < H; ih++)
 #pragma unroll
-    for (int ii = 0; ii < 4; ii++) {
-      const int r = m0 + ih * 64 + ty_e * 4 + ii;
+    for (int ii = 0; ii < G; ii++) {
+      const int r = m0 + ih * 64 + ty_e * G + ii;
       if (r >= M) continue;
 #pragma unroll
       for (int jh = 0; jh < H; jh++) {
-        const int c = n0 + jh * 64 + tx_e * 4;
+        const int c = n0 + jh * 64 + tx_e * G;
         float *dst = C + (int64_t)r * ldc_e + c;
         if constexpr (CHAIN) {
 #pragma unroll
-          for (int jj = 0; jj < 4; jj++)
+          for (int jj = 0; jj < G; jj++)
             if (c + jj < N && (bt.nstore == 0 || c + jj < bt.nstore)) {
-              const float o = acc2[ih * 4 + ii][(jh * 4 + jj) >> 1][jj & 1];
+              const float o = acc2[ih * G + ii][(jh * G + jj) >> 1][jj & 1];
               dst[jj] = o;
               mx = max_u32(mx, abs_bits(o));
             }
-        } else if (c_vec && c + 3 < N) {
-          f32x4 ci = *reinterpret_cast<const f32x4 *>(dst), o;
+        } else if (c_vec && c + G - 1 < N) {
+          vec_g ci = *reinterpret_cast<const vec_g *>(dst), o;
 #pragma unroll
-          for (int jj = 0; jj < 4; jj++) {
-            o[jj] = epilogue(ci[jj], acc2[ih * 4 + ii][(jh * 4 + jj) >> 1][jj & 1], alpha, beta);
+          for (int jj = 0; jj < G; jj++) {
+            o[jj] = epilogue(ci[jj], acc2[ih * G + ii][(jh * G + jj) >> 1][jj & 1], alpha, beta);
             mx = max_u32(mx, abs_bits(o[jj]));
           }
-          *reinterpret_cast<f32x4 *>(dst) = o;
+          *reinterpret_cast<vec_g *>(dst) = o;
         } else {
 #pragma unroll
-          for (int jj = 0; jj < 4; jj++)
+          for (int jj = 0; jj < G; jj++)
             if (c + jj < N) {
-              const float o = epilogue(dst[jj], acc2[ih * 4 + ii][(jh * 4 + jj) >> 1][jj & 1], alpha, beta);
+              const float o = epilogue(dst[jj], acc2[ih * G + ii][(jh * G + jj) >> 1][jj & 1], alpha, beta);
               dst[jj] = o;
               mx = max_u32(mx, abs_bits(o));
             }
@@ -1598,7 +1612,8 @@ int launch_gemm_(const char *who, float *C, const float *A, const float *B, int6
   const int c_vec = aligned16(C) && (ldc % 4 == 0) && (bt.sc % 4 == 0) && (N % 4 == 0);
   if (bt.nseg < 1) return fail(FPEMU_EINVAL, "k_segments must be >= 1");
   if (bt.nseg > 1 && ((bt.ka % 4) || (bt.kb % 4))) a.vec = b.vec = 0;
-  const int tb = fpemu_gemm_tile_edge_(M, N, batch, variant);   // 16 / 32: the small-tile chain kernels
+  int tb = fpemu_gemm_tile_edge_(M, N, batch, variant);   // 16 / 32: the small-tile chain kernels
+  if (variant == 0 && tb == 64 && ((M + 63) / 64) * ((N + 63) / 64) * batch <= FPEMU_SEQK_T32_MAX) tb = 32;
   const bool tiny = tb == 16, small = tb <= 32;
   // Ragged M or N on the large-tile kernels: one ragged edge used to put EVERY tile on the bounds-checked loads
   // (4100 x 4090 x 4096: 0.56 of the MFMA peak against 0.88 whole).  Outputs are independent chains, so the problem is
@@ -1629,12 +1644,15 @@ int launch_gemm_(const char *who, float *C, const float *A, const float *B, int6
   if (nwg > 0x7FFFFFFF) return fail(FPEMU_EINVAL, "too many tiles");
   const float beta = 0.0f;  // simple_gemm.cpp:58
   // every tile whole and 16-byte loads everywhere: the kernels drop their bounds tests
-  const bool full = a.vec && b.vec && (M % tb == 0) && (N % tb == 0) && (K % (small ? SK : variant == 1 ? MBK : BK) == 0) && K > 0;
+  const bool full = a.vec && b.vec && (M % tb == 0) && (N % tb == 0) && (K % (variant == 0 ? (tb == 32 ? seqk_depth<32>() : BK) : small ? SK : MBK) == 0) && K > 0;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)nwg, (unsigned)batch);
   if (variant == 0) {
     seqk_fn fn;
-    if (tb == 64)
+    if (tb == 32)
+      fn = chain ? (full ? pick_seqk<true, true, 32>(a_kcont, b_kcont) : pick_seqk<true, false, 32>(a_kcont, b_kcont))
+                 : (full ? pick_seqk<false, true, 32>(a_kcont, b_kcont) : pick_seqk<false, false, 32>(a_kcont, b_kcont));
+    else if (tb == 64)
       fn = chain ? (full ? pick_seqk<true, true, 64>(a_kcont, b_kcont) : pick_seqk<true, false, 64>(a_kcont, b_kcont))
                  : (full ? pick_seqk<false, true, 64>(a_kcont, b_kcont) : pick_seqk<false, false, 64>(a_kcont, b_kcont));
     else

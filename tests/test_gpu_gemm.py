@@ -299,6 +299,30 @@ def test_gemm_amax_errors(hip):
     assert L.fpemu_gemm_f32_amax(C.data_ptr(), A.data_ptr(), B.data_ptr(), 4, 4, 3, 3, 4, 4, 1.0, 0, 0, 1, None, None) == -1
 
 
+@pytest.mark.parametrize("shape", [(1024, 1024, 33), (1024, 1000, 96), (1000, 1025, 64), (960, 1024, 32), (31, 33, 1), (2050, 20, 300)])
+@pytest.mark.parametrize("at,bt", [(False, False), (True, False), (False, True), (True, True)])
+def test_separate_roundings_around_one_tile_per_cu(hip, shape, at, bt):
+    """Up to 256 tiles of 64 x 64 the separate-rounding product takes 32 x 32 ones: both sides of the border, k tiles of 32
+    whole and ragged, an infinity, and the epilogue's maximum."""
+    M, N, K = shape
+    rng = np.random.default_rng(M + N + K)
+    A = rng.standard_normal((K, M) if at else (M, K)).astype(np.float32)
+    B = rng.standard_normal((N, K) if bt else (K, N)).astype(np.float32)
+    A.flat[::89] = -0.0
+    A.flat[5 % A.size] = np.inf
+    want = orc.gemm(A, B, a_trans=at, b_trans=bt, fused=False)
+    C, word = torch.zeros(M, N, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    hip.gemm_(C, _t(A), _t(B), 1.0, at, bt, 0, amax=word)
+    assert_bits_equal(C.cpu().numpy(), want, "separate %s" % (shape,))
+    assert int(word.item()) == int((want.view(np.uint32) & 0x7FFFFFFF).max())
+    wide = torch.zeros(M, N + 3, device=DEV)[:, :N]      # rows of C that are not 16-byte aligned
+    st = torch.cuda.current_stream().cuda_stream
+    a, b = _t(A), _t(B)
+    assert hip.lib().fpemu_gemm_f32(wide.data_ptr(), a.data_ptr(), b.data_ptr(), M, N, K, A.shape[1], B.shape[1], N + 3, 1.0,
+                                    int(at), int(bt), 0, st) == 0
+    assert_bits_equal(wide.cpu().numpy(), want, "rows of any length")
+
+
 @pytest.mark.parametrize("acc", ["fma", "separate"])
 def test_simple_matmul_leaves_its_maximum_for_quantize_tensor(hip, acc, monkeypatch):
     """mpemu.cmodel.simple with collect_output_amax(True): quantize_tensor of the product (per-tensor max) takes the
