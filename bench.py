@@ -588,7 +588,7 @@ def main():
             sj = torch.arange(3, M, 127, device=dev)[:64]
             ha, hbm = ga[si].cpu().numpy(), gb_[:, sj].contiguous().cpu().numpy()
             # compute ceilings timed in this process, right before the legs they price: the bare MFMA pipe and the
-            # bare packed multiply + add stream (tools/ceilings.hip), 10 untimed launches then two events around 10
+            # bare multiply + add stream (tools/ceilings.hip), 10 untimed launches then two events around 10
             cc = {}
             if C is not None:
                 sink = torch.zeros(1024, device=dev)
@@ -596,13 +596,13 @@ def main():
                 cm = time_batch(lambda: C.ceil_mfma(sink.data_ptr(), it_m, blk_m, stream), launches=10, warm=10)
                 cv = time_batch(lambda: C.ceil_valu(sink.data_ptr(), it_v, blk_v, stream), launches=10, warm=10)
                 cc["mfma_f32"] = round(blk_m * 4 * it_m * 64.0 * 4096.0 / (cm * 1e-3) / 1e12, 2)
-                cc["valu_pk_f32"] = round(blk_v * 256.0 * it_v * 4 * 16 * 2 * 2 / (cv * 1e-3) / 1e12, 2)
+                cc["valu_mul_add_f32"] = round(blk_v * 256.0 * it_v * 4 * 16 * 2 * 2 / (cv * 1e-3) / 1e12, 2)
                 extras.setdefault("ceilings", {})["TFLOP/s"] = dict(
-                    cc, how="bare v_mfma_f32_32x32x2_f32 chains (4 per wave, 2 waves per SIMD) / bare v_pk_mul_f32 + "
-                            "v_pk_add_f32 chains (16 per lane, 4 waves per SIMD), no memory traffic; same process, "
+                    cc, how="bare v_mfma_f32_32x32x2_f32 chains (4 per wave, 2 waves per SIMD) / bare v_mul_f32 + "
+                            "v_add_f32 chains (32 per lane, 4 waves per SIMD), no memory traffic; same process, "
                             "10 untimed launches then two events around 10")
             for name, variant, peak, fused, bare in (("gemm_8192_mfma_fma_chain", 1, 157.3, True, "mfma_f32"),
-                                                     ("gemm_8192_valu_separate", 0, 78.6, False, "valu_pk_f32")):
+                                                     ("gemm_8192_valu_separate", 0, 78.6, False, "valu_mul_add_f32")):
                 def gstep(variant=variant):
                     hip.gemm_(gc, ga, gb_, 1.0, False, False, variant)
 

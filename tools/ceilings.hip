@@ -39,8 +39,8 @@ __global__ __launch_bounds__(BLOCK) void k_copy(const u32x4 *in, u32x4 *out, uin
 // Compute ceilings for the c-model GEMM legs, timed in the bench process like the streams above:
 //   mfma : four independent v_mfma_f32_32x32x2_f32 accumulator chains per wave (the GEMM kernel's shape), no memory
 //          traffic -- what the fp32 MFMA pipe sustains at the clock this process gets;
-//   valu : sixteen independent packed chains per lane of a rounded product then a rounded sum (v_pk_mul_f32 +
-//          v_pk_add_f32, built with -ffp-contract=off) -- the separate-rounding GEMM's instruction mix, nothing else.
+//   valu : thirty-two independent chains per lane of a rounded product then a rounded sum (v_mul_f32 + v_add_f32, built
+//          with -ffp-contract=off and without packed fp32) -- the separate-rounding GEMM's instruction mix, nothing else.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
