@@ -129,8 +129,8 @@ __device__ __forceinline__ void banded(uint32_t id, uint32_t row_tiles, uint32_t
 // buffer.
 // The same kernel takes 16-bit operands whose rows are not whole 16-byte vectors: global loads need no more than element
 // alignment, and vectors that reach over an edge are put together element by element.
-// Measured, fp32: 2051 rows, 8 uneven groups, 768 x 1000: y 57, dx 62, dW 51 us (56 TFLOP/s: small tiles, each
-// a chain over all of k); 4096^3 114 to 124 TFLOP/s.
+// Measured, fp32: 2051 rows, 8 uneven groups, 768 x 1000: y 62, dx 57, dW 49 us (56 TFLOP/s: 64 x 64 tiles, each a chain over all
+// of k, 2.3 of them for a CU; the matrix units are busy 43 to 56 % of the time); 4096^3 113 to 136 TFLOP/s.
 // A stage is 128 bytes deep in k (64 16-bit or 32 fp32 elements).  LDS holds it as described for the tiles further down.
 typedef uint32_t vec_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -405,9 +405,11 @@ __global__ __launch_bounds__(256, 2) void grouped_wgrad_any_kernel(typename Stor
 // fetches and undone where the fragment is read.
 // Waves: WM x WN over the tile.
 // Bound by the matrix cores (by the clock they hold on data that is not zero) where K is long, by a tile's start and end (about
-// 10 us of a 256 x 256 tile) where it is not, by the weights' bytes for few rows.  Measured: 8192^3 bf16 1350 to 1400 TFLOP/s;
-// 16381 rows, 16 uneven groups, 2048 x 4096 fp16 296 us (928); 8197 rows, 16 groups, 1024 x 2816 bf16, y, dx and dW 199 us
-// (712); 64 rows, 32 groups, 2048 x 1408 36 to 39 us with the weights from memory (4.9 TB/s), 25 us with them in the cache.
+// 10 us of a 256 x 256 tile) where it is not, by the weights' bytes for few rows.  Measured: 8192^3 bf16 1330 to 1380 TFLOP/s,
+// fp16 1240 to 1270; 16381 rows, 16 uneven groups, 2048 x 4096 fp16 296 us (930); 8197 rows, 16 groups, 1024 x 2816 bf16, y, dx and
+// dW 203 us (700; 68, 75 and 63 alone); 64 rows, 32 groups of which 26 have rows, 2048 x 1408 39 us with their 152 MB of weights
+// from memory (3.9 TB/s), 25 us with them in the cache.  The matrix units are busy 57 % of the time in the first of these, 34 to 41 %
+// in the second; one workgroup fills a CU's LDS, so nothing runs while its tile starts or ends.
 constexpr int FK = 64;
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(const lds_char *)p; }
@@ -748,16 +750,19 @@ int launched(const char *who) {
 }
 
 // A shape's tiles cost nearly the same whether their rows are filled or not, so the large one needs groups of some rows, and tiles
-// for half of the CUs.  bf16, us with 256 x 256 / 128 x 128 tiles, operands from memory: 16 groups of about 1024 rows, 2048 x
-// 4096: 324 / 385; of about 512, 1024 x 2816 (352 large tiles): 68 / 83, 2816 x 1024 (128): 86 / 98; 8 of 256, 768 x 1024
-// (32): 20 / 11; 32 of 2 rows, 2048 x 1408: 5.3 / 6.2 TB/s of weights.
+// for half of the CUs.  bf16, us with 256 x 256 / 128 x 128 tiles, groups alike (and uneven, the largest twice the mean),
+// operands in the caches: 16 groups of about 1024 rows, 2048 x 4096: 233 / 307 (257 / 314); of 512, 1024 x 2816 (352 large
+// tiles): 54 / 53 (52 / 66), 2816 x 1024 (128): 54 / 45 (55 / 72); 8 of 256, 768 x 1024 (32): 19 / 10; 32 of 2 rows, 2048 x
+// 1408: 37 / 28.
 constexpr int64_t kLargeRows = 256, kLargeTiles = 128;
 bool large_tiles(int64_t rows_per_group, int64_t tiles) { return rows_per_group >= kLargeRows && tiles >= kLargeTiles; }
 
-// Fewer 128 x 128 tiles than CUs: 64 x 64 ones.  us with 128 / 64: fp32, 8 groups of 256, 768 x 1000 (128 tiles): 82 / 53; 16 of
-// 256, 1024 x 1024 (256 tiles): 109 / 112; bf16, 4 of 75, 512 x 1024 (24 tiles): 9.2 / 7.8; 16 of 256 (256 tiles): 17.9 / 20.3.
-// Through registers (`any`) below two tiles a CU: the longest group's tiles are what a small fp32 weight gradient waits for (8
-// groups, the largest twice the mean, 768 x 1000, 384 tiles: 92 / 58 us).
+// Fewer 128 x 128 tiles than CUs: 64 x 64 ones.  bf16, us with 128 / 64: 4 groups of 75, 512 x 1024 (24 tiles): 8.5 / 7.4; 8 of
+// 256, 768 x 1024 (128): 10.4 / 8.6; 16 of 256, 1024 x 1024 (256): 17.4 / 18.8, uneven 17.2 / 24.2.
+// Through registers (`any`) below two tiles a CU, because the longest group's tiles are what the others wait for.  fp32, us
+// with 128 / 64, groups alike, then uneven: 8 groups of 256, 768 x 1000, y (128 tiles): 90 / 51, 91 / 63, dW (384): 48 / 46,
+// 63 / 44; 16 of 256, 1024 x 1024 (256): 86 / 85, 148 / 104; 8 of 768, 1024 x 1024 (384): 149 / 126, 149 / 142; and from there on
+// 16 of 512, 768 x 1024 (512): 116 / 127, 171 / 140; 8 of 1024, 768 x 2048 (1024): 225 / 247, 278 / 258.
 constexpr int64_t kLittleTiles = 256;
 bool little_tiles(int64_t row_tiles, int64_t col_tiles, bool any) { return row_tiles * col_tiles < (any ? 2 : 1) * kLittleTiles; }
 
@@ -769,7 +774,9 @@ constexpr int64_t kStreamBytes = 64ll << 20;
 bool streams(int64_t bytes) { return bytes > kStreamBytes; }
 
 // Groups of few rows, staged through registers: tiles of 32 rows leave fewer matrix instructions to rows that are not there.
-// fp32, 32 groups, 2048 x 1408, us with 64 x 64 / 32 x 128 tiles: 2 rows a group 200 / 145, 32 rows 170 / 130, 64 rows 168 / 173.
+// fp32, 32 groups, 2048 x 1408, us with 64 x 64 / 32 x 128 tiles: 2 rows a group 129 / 95 (weights transposed 147 / 106), 32 rows
+// 133 / 95 (152 / 110), 38 rows 135 / 137 (151 / 158), 64 rows 139 / 142 (154 / 161).  bf16 at 2047 x 1409: 2 rows 62 / 72
+// (43 / 39), 32 rows 61 / 73 (42 / 40).
 bool flat_tiles(int64_t rows, int64_t groups) { return rows <= 32 * groups; }
 
 template <int DT>

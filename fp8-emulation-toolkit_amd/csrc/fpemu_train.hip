@@ -35,8 +35,9 @@ uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 // the equal digits before it is found wave by wave: ballots over the digit's bits give the lanes with the same digit, one
 // LDS counter per (wave, digit) carries the count from round to round.  The chain of rounds is what a small sort takes
 // (ballots, an LDS atomic and a shuffle each), so a workgroup is as wide as it can be: 16 waves, four rounds at most.
-// Measured: 1031 ids in 64 groups 4.6 us (one launch); 65536 ids in 30522 groups 34 us of kernels (two digits: count 3.4 and
-// place 11 us each, latency; offsets 5); 2^20 ids in 256 groups 22 us (count 5, scan 4, place 13: 4-byte stores at random).
+// Measured: 1031 ids in 64 groups 4.5 us (one launch); 65536 ids in 30522 groups 34 us of kernels (two digits: count 3.8 and
+// place 10.5 us each on 16 workgroups, latency; offsets 5.2, a binary search an entry); 2^20 ids in 256 groups 22 us (count 4.8,
+// scan 4.2, place 13.3: its 4-byte stores leave in the order of the lanes, not of the digits).
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortRounds = 4;
 constexpr int kSortTile = kSortThreads * kSortRounds;   // 4096 rows per workgroup
 constexpr int kMaxBits = 9;                             // digits of at most 512 values: 32 KB of counters
@@ -494,7 +495,8 @@ __device__ __forceinline__ int64_t id_at(const void *ids, int wide, uint64_t i) 
 
 // out[t] = scale * weight[ids[t]]: 2^lg_tpr threads a row, R rows a thread (their loads are in flight together).  A row whose
 // id is outside the table reads nothing of it and is NaN.  Bound by memory (each row read and written once): 32768 rows of 2048
-// bf16 in 41 us, 6.5 TB/s.  One row a thread where the launch is short (one token: 1.5 us).
+// bf16 in 42 us, 6.4 TB/s (of 134 MB read 86 miss the L2s: frequent tokens' rows).  One row a thread
+// where the launch is short (one token: 1.4 us).
 template <int DT, int R>
 __global__ __launch_bounds__(256) void embedding_kernel(const void *weight, const void *ids, int wide, void *out, uint64_t n,
                                                         uint64_t vocab, uint64_t width, float scale, int lg_tpr) {
@@ -546,8 +548,8 @@ __global__ __launch_bounds__(256) void embedding_kernel(const void *weight, cons
 // not whole vectors the last lane's vector begins earlier and shares columns with its neighbour's, which writes the same
 // values there; only rows shorter than a vector (WHOLE false) go element by element.
 // Bound by rows read at random, 4 KB at a time, with the cleared table on its way out.  Measured: 32768 tokens, entry v about as often as
-// 1 / (v + 1), 131072 x 2048 bf16: chunks 15 us, runs 37 us, behind a sort of 94 us that clears 537 MB meanwhile (5.7 TB/s); 1024
-// tokens, 30522 x 768 fp32: 3.7 and 6.1 us, behind 14 us for sort and clearing.
+// 1 / (v + 1), 131072 x 2048 bf16: chunks 15 us, runs 41 us, behind a sort of 94 us that clears 537 MB meanwhile (5.7 TB/s); 1024
+// tokens, 30522 x 768 fp32: 3.9 and 5.6 us, behind 14 us for sort and clearing.
 constexpr uint32_t kSub = 16;    // positions looked at together: their keys and tokens lie in the wave's lanes
 constexpr int kRows = 8;
 
@@ -746,8 +748,8 @@ uint32_t chunk_of(uint64_t n) {
 
 // ---- norm and clipping of a list of gradients -----------------------------------------------------------------------------
 // One pass of partial sums, one workgroup that joins them in order, one pass that scales; each is bound by memory.  Measured:
-// 182 M bf16 gradients, norm 69 us (5.3 TB/s), scaled into fp32 in 177 us (6.2 TB/s); 3.5 M fp32 elements in 51 tensors that
-// need no clipping: 6 + 2.4 + 3 us, launches.
+// 182 M bf16 gradients, norm 68 us (5.3 TB/s), scaled into fp32 in 176 us (6.2 TB/s); 3.5 M fp32 elements in 51 tensors that
+// need no clipping: 5.9 + 2.2 + 3.2 us, launches.
 constexpr int kGrads = 128;              // tensors per launch (the table travels in the kernel arguments)
 constexpr unsigned kNormBlocks = 2048;   // workgroups (= partial sums) per launch
 
@@ -966,7 +968,8 @@ int check_grads(const char *who, const fpemu_grad_t *grads, uint64_t count, int 
 }
 
 // the next launch's table, from grads[at]; returns where the one after begins.  Steps of 8192 elements, two batches of four
-// loads a thread: 182 M bf16 gradients into fp32 ones take 185 us so, 192 with steps of 16384, 212 with 65536.
+// loads a thread: 182 M bf16 gradients into fp32 ones take 187 us so, from before the first launch to behind the second, 197 with
+// steps of 16384, 218 with 65536.
 uint64_t fill_table(const fpemu_grad_t *grads, uint64_t count, uint64_t at, GradTable &tab, uint64_t &chunks) {
   tab.count = 0;
   uint64_t elems = 0;
