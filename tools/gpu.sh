@@ -67,7 +67,7 @@ profile)    # bench.py under rocprofv3: kernel stats, then FETCH_SIZE and WRITE_
   pmc $P/pmc_fetch FETCH_SIZE python3 bench.py --steps 3 --warmup 1 --no-extras
   pmc $P/pmc_write WRITE_SIZE python3 bench.py --steps 3 --warmup 1 --no-extras
   stats $P/gemm_stats 300 python3 tools/gemm_bench.py 8192x8192x8192 nn
-  python3 tools/summarize_prof.py $P ${1:-r03}
+  python3 tools/summarize_prof.py $P ${1:-cast}
   ;;
 tools)      # every tools/ benchmark in turn -> gpurun_out/tools.txt
   OUT=gpurun_out/tools.txt; : > $OUT
